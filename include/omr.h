@@ -442,6 +442,58 @@ int omr_msg_unpack_f32(const float* replies, const uint32_t* reply_imm, const vo
                        uint32_t num_parts, uint32_t round_capacity, uint32_t block_size, uint32_t num_lanes,
                        float* buf, omr_stream_t stream);
 
+/* ---------------------------------------------------------------- operators that make the gradient
+ *
+ * The two ends of a language model, whose parameter gradients are the tensors the all-reduce sums over the workers.
+ * Common to them:
+ *   - element types: OMR_F32, OMR_BF16, OMR_F16; arithmetic and sums in fp32, one rounding at the end;
+ *   - rows are a stride apart, in elements: for an output at least the row's length, for an input any (0: one row for
+ *     all); the elements of a row are consecutive.  Any alignment and length works; rows whose start and length are
+ *     whole 16-byte pieces run fastest;
+ *   - a row is at most OMR_MAX_DIM elements;
+ *   - every sum has a fixed order: the same inputs give the same bits;
+ *   - a workspace holds nothing from one call to the next and needs no initial value; calls that may run at the same
+ *     time (two streams, two captured graphs that are replayed side by side) need one each;
+ *   - outputs must not overlap inputs or each other unless a comment says so. */
+#define OMR_F32 0
+#define OMR_BF16 1
+#define OMR_F16 2
+#define OMR_MAX_DIM (1u << 24)
+
+/* Embedding lookup: out[t, :] = scale * table[ids[t], :] for t < num_ids.  ids: int32, or int64 with ids64 != 0; an id
+ * outside [0, num_rows) names no row (padding) and gives a row of zeros.  num_rows, num_ids < 2^31. */
+int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t dim, uint64_t row_stride, const void* ids,
+              int ids64, uint64_t num_ids, float scale, void* out, int out_dtype, uint64_t out_stride,
+              omr_stream_t stream);
+
+/* Its gradient: grad_table[v, :] = scale * (sum over the t with ids[t] == v, in order of t, of grad_out[t, :]), fp32;
+ * every row of grad_table is written (zeros where no token names it), or, with accumulate != 0, the sums are added to
+ * the rows that tokens name and the others are left as they are.  Tokens whose id names no row are skipped, whatever
+ * their row of grad_out holds.  (The sum of a row of more tokens than omr_embed_grad's chunk, 64 to 1024 by num_ids, is
+ * the sum of its chunks' sums.) */
+size_t omr_embed_grad_workspace_bytes(uint64_t num_ids, uint64_t num_rows, uint32_t dim);
+int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_stride, const void* ids, int ids64,
+                       uint64_t num_ids, uint64_t num_rows, uint32_t dim, float scale, float* grad_table,
+                       uint64_t table_stride, int accumulate, void* workspace, size_t workspace_bytes,
+                       omr_stream_t stream);
+
+/* Layer norm of each row: mean = mean(x), rstd = 1 / sqrt(mean((x - mean)^2) + eps), out = (x - mean) * rstd * weight +
+ * bias.  x and out: `dtype`; weight and bias: param_dtype, fp32 or dtype (NULL: ones / zeros); mean and rstd: fp32
+ * [rows].  out may be x. */
+int omr_layer_norm(const void* x, int dtype, uint64_t rows, uint32_t dim, uint64_t x_stride, const void* weight,
+                   const void* bias, int param_dtype, float eps, void* out, uint64_t out_stride, float* mean,
+                   float* rstd, omr_stream_t stream);
+
+/* Its backward pass, with the mean and rstd the forward left: with xh = (x - mean) rstd and g = grad_out * weight,
+ *   grad_x = rstd (g - mean(g) - xh mean(g xh))             (dtype; may be grad_out or x)
+ *   grad_weight[c] = sum over the rows of grad_out xh, grad_bias[c] = sum over the rows of grad_out
+ * in fp32 (NULL: not wanted; both NULL needs no workspace), or added to what is there with accumulate != 0. */
+size_t omr_layer_norm_grad_workspace_bytes(uint64_t rows, uint32_t dim);
+int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* x, int dtype, uint64_t rows,
+                        uint32_t dim, uint64_t x_stride, const float* mean, const float* rstd, const void* weight,
+                        int param_dtype, void* grad_x, uint64_t grad_x_stride, float* grad_weight, float* grad_bias,
+                        int accumulate, void* workspace, size_t workspace_bytes, omr_stream_t stream);
+
 /* ---------------------------------------------------------------- host-resident end-to-end path */
 
 /* The gradient lives in host memory (the reference's registered region, common.cc:873-914): H2D in row chunks,

@@ -1,0 +1,507 @@
+// omr_norm.hip — layer norm, forward and backward, with the reduction of the weight's and bias's gradients.
+//
+//   forward   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), y = (x - mu) r w + b
+//   backward  xh = (x - mu) r, g = dy w:
+//             dx = r (g - mean(g) - xh mean(g xh)),  dw (+)= sum over rows of dy xh,  db (+)= sum over rows of dy
+//
+// Both are bound by HBM (the forward reads and writes each element once, the backward reads two and writes one), so a
+// row is read once and held in registers: WPR waves hold a row, 16 columns a lane, and statistics are two-pass sums over
+// the registers (the mean first, then the squared distances), which lose nothing to a large mean.  Workgroups walk
+// several rows, so the parameters are loaded once into registers too, and the backward keeps its part of dw and db there
+// until its last row: one partial row a workgroup, which a second launch adds up in a fixed order.
+// Rows of more than 16384 columns take the *_any kernels, which read a row again instead of holding it.
+#include "omr_elem.h"
+
+#include <type_traits>
+
+using namespace omr_elem;
+
+namespace {
+
+constexpr int kCols = 16;  // columns a lane holds
+
+struct NormArgs {
+  const void* x;
+  uint64_t xstride;
+  const void* w;  // or null: ones
+  const void* b;  // or null: zeros
+  void* out;      // y, or dx
+  uint64_t ostride;
+  float* mean;
+  float* rstd;
+  const void* dy;
+  uint64_t dystride;
+  float* partial;  // [blocks][2][dim]: dw, db; or null
+  uint64_t rows;
+  uint32_t dim;
+  float eps, inv_dim;
+};
+
+// Sum over the WPR waves of a row, in every lane.  Each call site has LDS of its own, and between two uses of one there
+// is another's barrier (or, where a kernel has one call site, two alternating buffers).
+template <int WPR>
+__device__ __forceinline__ float row_sum(float v, float* lds) {
+  v = wave_sum(v);
+  if constexpr (WPR > 1) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) v += lds[w];
+  }
+  return v;
+}
+
+// A lane's columns: VEC consecutive ones of every piece j
+template <int WPR, int VEC>
+__device__ __forceinline__ uint32_t col_of(int j) {
+  const uint32_t t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  return (static_cast<uint32_t>(j) * 64 * WPR + t) * VEC;
+}
+
+template <class T, int WPR, int VEC>
+__device__ __forceinline__ void load_row(const T* p, uint32_t dim, float (&v)[kCols / VEC][VEC], float other) {
+#pragma unroll
+  for (int j = 0; j < kCols / VEC; ++j) {
+    const uint32_t c = col_of<WPR, VEC>(j);
+    if (c < dim) {
+      load_f32<T, VEC>(p + c, v[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j][i] = other;
+    }
+  }
+}
+
+template <class T, class P, int VEC, int WPR>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) {
+  constexpr int NV = kCols / VEC, RPB = WPR == 1 ? 4 : 1;
+  __shared__ float lds[2][WPR];
+  float w[NV][VEC], b[NV][VEC];
+  if (a.w != nullptr) {
+    load_row<P, WPR, VEC>(static_cast<const P*>(a.w), a.dim, w, 0.0f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[j][i] = 1.0f;
+  }
+  if (a.b != nullptr) {
+    load_row<P, WPR, VEC>(static_cast<const P*>(a.b), a.dim, b, 0.0f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) b[j][i] = 0.0f;
+  }
+  for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * RPB + (WPR == 1 ? threadIdx.x >> 6 : 0); row < a.rows;
+       row += static_cast<uint64_t>(gridDim.x) * RPB) {
+    float v[NV][VEC];
+    load_row<T, WPR, VEC>(static_cast<const T*>(a.x) + row * a.xstride, a.dim, v, 0.0f);
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s += v[j][i];
+    const float mean = row_sum<WPR>(s, lds[0]) * a.inv_dim;
+    float q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (col_of<WPR, VEC>(j) < a.dim) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          v[j][i] -= mean;
+          q += v[j][i] * v[j][i];
+        }
+      }
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<WPR>(q, lds[1]) * a.inv_dim + a.eps);
+    T* out = static_cast<T*>(a.out) + row * a.ostride;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t c = col_of<WPR, VEC>(j);
+      if (c < a.dim) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * rstd * w[j][i] + b[j][i];
+        store_f32<T, VEC>(out + c, v[j]);
+      }
+    }
+    if (WPR == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+  }
+}
+
+template <class T, class P, int VEC, int WPR>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm_grad(NormArgs a) {
+  constexpr int NV = kCols / VEC, RPB = WPR == 1 ? 4 : 1;
+  __shared__ float lds[2][2][WPR];
+  float w[NV][VEC], dw[NV][VEC] = {}, db[NV][VEC] = {};
+  if (a.w != nullptr) {
+    load_row<P, WPR, VEC>(static_cast<const P*>(a.w), a.dim, w, 0.0f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[j][i] = 1.0f;
+  }
+  int flip = 0;
+  for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * RPB + (WPR == 1 ? threadIdx.x >> 6 : 0); row < a.rows;
+       row += static_cast<uint64_t>(gridDim.x) * RPB) {
+    float v[NV][VEC], g[NV][VEC];
+    load_row<T, WPR, VEC>(static_cast<const T*>(a.x) + row * a.xstride, a.dim, v, 0.0f);
+    load_row<T, WPR, VEC>(static_cast<const T*>(a.dy) + row * a.dystride, a.dim, g, 0.0f);
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (col_of<WPR, VEC>(j) < a.dim) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float xh = (v[j][i] - mean) * rstd;
+          v[j][i] = xh;
+          dw[j][i] += g[j][i] * xh;
+          db[j][i] += g[j][i];
+          g[j][i] *= w[j][i];
+          s1 += g[j][i];
+          s2 += g[j][i] * xh;
+        }
+      }
+    }
+    // both sums behind one barrier; the buffers alternate, so a wave that is a row ahead writes the other one
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if constexpr (WPR > 1) {
+      if ((threadIdx.x & 63) == 0) {
+        lds[flip][0][threadIdx.x >> 6] = s1;
+        lds[flip][1][threadIdx.x >> 6] = s2;
+      }
+      __syncthreads();
+      s1 = lds[flip][0][0];
+      s2 = lds[flip][1][0];
+#pragma unroll
+      for (int k = 1; k < WPR; ++k) {
+        s1 += lds[flip][0][k];
+        s2 += lds[flip][1][k];
+      }
+      flip ^= 1;
+    }
+    s1 *= a.inv_dim;
+    s2 *= a.inv_dim;
+    T* out = static_cast<T*>(a.out) + row * a.ostride;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t c = col_of<WPR, VEC>(j);
+      if (c < a.dim) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) g[j][i] = (g[j][i] - s1 - v[j][i] * s2) * rstd;
+        store_f32<T, VEC>(out + c, g[j]);
+      }
+    }
+  }
+  if (a.partial == nullptr) return;
+  float* part = a.partial + static_cast<uint64_t>(blockIdx.x) * 2 * a.dim;
+  if constexpr (WPR == 1) {  // the four waves' rows, in wave order
+    __shared__ float sum[4][64 * kCols];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          sum[wave][(j * VEC + i) * 64 + lane] = which == 0 ? dw[j][i] : db[j][i];
+      __syncthreads();
+      // entry e of a wave's columns: piece j = e / 64 / VEC, element i, lane
+      for (uint32_t e = threadIdx.x; e < 64 * kCols; e += 256) {
+        const uint32_t ji = e >> 6, c = (ji / VEC * 64 + (e & 63)) * VEC + ji % VEC;
+        if (c < a.dim) part[which * a.dim + c] = ((sum[0][e] + sum[1][e]) + sum[2][e]) + sum[3][e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t c = col_of<WPR, VEC>(j);
+      if (c < a.dim) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          part[c + i] = dw[j][i];
+          part[a.dim + c + i] = db[j][i];
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- rows longer than the registers hold
+
+constexpr int kAnyWaves = 16;
+
+template <class T, class P>
+__global__ __launch_bounds__(64 * kAnyWaves) void k_norm_any(NormArgs a) {
+  __shared__ float lds[2][kAnyWaves];
+  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.xstride;
+    T* out = static_cast<T*>(a.out) + row * a.ostride;
+    float s = 0.0f;
+    for (uint32_t c = threadIdx.x; c < a.dim; c += 64 * kAnyWaves) s += static_cast<float>(x[c]);
+    const float mean = row_sum<kAnyWaves>(s, lds[0]) * a.inv_dim;
+    float q = 0.0f;
+    for (uint32_t c = threadIdx.x; c < a.dim; c += 64 * kAnyWaves) {
+      const float d = static_cast<float>(x[c]) - mean;
+      q += d * d;
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<kAnyWaves>(q, lds[1]) * a.inv_dim + a.eps);
+    for (uint32_t c = threadIdx.x; c < a.dim; c += 64 * kAnyWaves) {
+      const float w = a.w != nullptr ? static_cast<float>(static_cast<const P*>(a.w)[c]) : 1.0f;
+      const float b = a.b != nullptr ? static_cast<float>(static_cast<const P*>(a.b)[c]) : 0.0f;
+      out[c] = static_cast<T>((static_cast<float>(x[c]) - mean) * rstd * w + b);
+    }
+    if (threadIdx.x == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+  }
+}
+
+template <class T, class P>
+__global__ __launch_bounds__(64 * kAnyWaves) void k_norm_dx_any(NormArgs a) {
+  __shared__ float lds[2][kAnyWaves];
+  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.xstride;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dystride;
+    T* out = static_cast<T*>(a.out) + row * a.ostride;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float s1 = 0.0f, s2 = 0.0f;
+    for (uint32_t c = threadIdx.x; c < a.dim; c += 64 * kAnyWaves) {
+      const float w = a.w != nullptr ? static_cast<float>(static_cast<const P*>(a.w)[c]) : 1.0f;
+      const float g = static_cast<float>(dy[c]) * w;
+      s1 += g;
+      s2 += g * ((static_cast<float>(x[c]) - mean) * rstd);
+    }
+    s1 = row_sum<kAnyWaves>(s1, lds[0]) * a.inv_dim;
+    s2 = row_sum<kAnyWaves>(s2, lds[1]) * a.inv_dim;
+    for (uint32_t c = threadIdx.x; c < a.dim; c += 64 * kAnyWaves) {
+      const float w = a.w != nullptr ? static_cast<float>(static_cast<const P*>(a.w)[c]) : 1.0f;
+      const float xh = (static_cast<float>(x[c]) - mean) * rstd;
+      out[c] = static_cast<T>((static_cast<float>(dy[c]) * w - s1 - xh * s2) * rstd);
+    }
+  }
+}
+
+// 64 columns a workgroup, its 16 waves a row each in turn
+template <class T>
+__global__ __launch_bounds__(64 * kAnyWaves) void k_norm_params_any(NormArgs a) {
+  __shared__ float sum[2][kAnyWaves][64];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t c = blockIdx.x * 64 + lane;
+  float dw = 0.0f, db = 0.0f;
+  if (c < a.dim)
+    for (uint64_t row = static_cast<uint64_t>(blockIdx.y) * kAnyWaves + wave; row < a.rows;
+         row += static_cast<uint64_t>(gridDim.y) * kAnyWaves) {
+      const float g = static_cast<float>(static_cast<const T*>(a.dy)[row * a.dystride + c]);
+      const float x = static_cast<float>(static_cast<const T*>(a.x)[row * a.xstride + c]);
+      dw += g * ((x - a.mean[row]) * a.rstd[row]);
+      db += g;
+    }
+  sum[0][wave][lane] = dw;
+  sum[1][wave][lane] = db;
+  __syncthreads();
+  if (wave < 2 && c < a.dim) {
+    float s = 0.0f;
+    for (int w = 0; w < kAnyWaves; ++w) s += sum[wave][w][lane];
+    a.partial[(static_cast<uint64_t>(blockIdx.y) * 2 + wave) * a.dim + c] = s;
+  }
+}
+
+// ---------------------------------------------------------------- the partial rows' sum
+//
+// 64 columns a workgroup; wave w adds the partial rows w, w + 16, ..., and wave 0 the sixteen sums in wave order.
+__global__ __launch_bounds__(64 * kAnyWaves) void k_norm_params(const float* partial, uint32_t blocks, uint32_t dim,
+                                                                float* dw, float* db, int accumulate) {
+  __shared__ float sum[kAnyWaves][64];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t c = static_cast<uint64_t>(blockIdx.x) * 64 + lane, width = 2ull * dim;
+  float s = 0.0f;
+  if (c < width) {
+#pragma unroll 8
+    for (uint32_t k = wave; k < blocks; k += kAnyWaves) s += partial[k * width + c];
+  }
+  sum[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || c >= width) return;
+  for (int w = 1; w < kAnyWaves; ++w) s += sum[w][lane];
+  float* out = c < dim ? dw : db;
+  if (out == nullptr) return;
+  out += c < dim ? c : c - dim;
+  *out = accumulate ? *out + s : s;
+}
+
+__global__ __launch_bounds__(256) void k_zero(float* p, uint64_t n) {
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) p[i] = 0.0f;
+}
+
+int waves_per_row(uint32_t dim) {
+  int w = 1;
+  while (w <= 16 && static_cast<uint32_t>(w) * 64 * kCols < dim) w *= 2;
+  return w;  // 32: too long for registers
+}
+
+// Workgroups of the backward: enough to fill the CUs with their registers' worth of waves, few enough that the partial
+// rows (2 dim floats each) stay small beside the rows themselves.
+constexpr uint32_t kGradBlocks = 512;
+uint32_t grad_blocks(uint64_t rows, uint32_t dim) {
+  const int wpr = waves_per_row(dim);
+  const uint64_t want = wpr == 1 ? ceil_div(rows, 4) : wpr > 16 ? ceil_div(rows, kAnyWaves) : rows;
+  return static_cast<uint32_t>(want < kGradBlocks ? want : kGradBlocks);
+}
+
+// fn(VEC, WPR) as integral constants
+template <int W, class F>
+int with_shape(bool wide, int wpr, F&& fn) {
+  auto vec = [&](auto p) {
+    return wide ? fn(std::integral_constant<int, W>{}, p) : fn(std::integral_constant<int, 1>{}, p);
+  };
+  switch (wpr) {
+    case 1: return vec(std::integral_constant<int, 1>{});
+    case 2: return vec(std::integral_constant<int, 2>{});
+    case 4: return vec(std::integral_constant<int, 4>{});
+    case 8: return vec(std::integral_constant<int, 8>{});
+    default: return vec(std::integral_constant<int, 16>{});
+  }
+}
+
+int check_args(const char* what, int dtype, int param_dtype, uint64_t rows, uint32_t dim) {
+  if (!dtype_ok(dtype) || (param_dtype != OMR_F32 && param_dtype != dtype))
+    return efail("%s: elements are fp32, bf16 or fp16, and parameters fp32 or of the elements' type", what);
+  if (dim == 0 || dim > OMR_MAX_DIM) return efail("%s: dim must be 1..%u", what, OMR_MAX_DIM);
+  if (rows >= (1ull << 40)) return efail("%s: too many rows", what);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int omr_layer_norm(const void* x, int dtype, uint64_t rows, uint32_t dim, uint64_t x_stride, const void* weight,
+                   const void* bias, int param_dtype, float eps, void* out, uint64_t out_stride, float* mean,
+                   float* rstd, omr_stream_t stream) {
+  if (const int rc = check_args("layer_norm", dtype, param_dtype, rows, dim)) return rc;
+  if (out_stride < dim) return efail("layer_norm: the output's row stride is shorter than dim %u", dim);
+  if (!(eps >= 0.0f)) return efail("layer_norm: eps must not be negative");
+  if (rows == 0) return 0;
+  if (x == nullptr || out == nullptr || mean == nullptr || rstd == nullptr) return efail("layer_norm: NULL pointer");
+  NormArgs a{};
+  a.x = x;
+  a.xstride = x_stride;
+  a.w = weight;
+  a.b = bias;
+  a.out = out;
+  a.ostride = out_stride;
+  a.mean = mean;
+  a.rstd = rstd;
+  a.rows = rows;
+  a.dim = dim;
+  a.eps = eps;
+  a.inv_dim = 1.0f / static_cast<float>(dim);
+  const int wpr = waves_per_row(dim);
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    auto params = [&](auto p) {
+      using P = decltype(p);
+      if (wpr > 16) {
+        const unsigned grid = static_cast<unsigned>(rows < 2048 ? rows : 2048);
+        k_norm_any<T, P><<<grid, 64 * kAnyWaves, 0, S(stream)>>>(a);
+        return elaunch("omr_layer_norm");
+      }
+      constexpr int W = 16 / sizeof(T);
+      const bool wide = dim % W == 0 && x_stride % W == 0 && out_stride % W == 0 && aligned(x, 16) &&
+                        aligned(out, 16) && aligned(weight, W * sizeof(P) < 16 ? W * sizeof(P) : 16) &&
+                        aligned(bias, W * sizeof(P) < 16 ? W * sizeof(P) : 16);
+      return with_shape<W>(wide, wpr, [&](auto vec, auto waves) {
+        constexpr int VEC = decltype(vec)::value, WPR = decltype(waves)::value;
+        const uint64_t want = WPR == 1 ? ceil_div(rows, 4) : rows;
+        const uint64_t most = WPR <= 4 ? 2048 : 8192 / WPR;
+        k_norm<T, P, VEC, WPR><<<static_cast<unsigned>(want < most ? want : most), WPR == 1 ? 256 : 64 * WPR, 0,
+                                 S(stream)>>>(a);
+        return elaunch("omr_layer_norm");
+      });
+    };
+    return param_dtype == OMR_F32 ? params(float{}) : params(T{});
+  });
+}
+
+size_t omr_layer_norm_grad_workspace_bytes(uint64_t rows, uint32_t dim) {
+  return static_cast<size_t>(grad_blocks(rows, dim)) * 2 * dim * sizeof(float) + 16;
+}
+
+int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* x, int dtype, uint64_t rows,
+                        uint32_t dim, uint64_t x_stride, const float* mean, const float* rstd, const void* weight,
+                        int param_dtype, void* grad_x, uint64_t grad_x_stride, float* grad_weight, float* grad_bias,
+                        int accumulate, void* workspace, size_t workspace_bytes, omr_stream_t stream) {
+  if (const int rc = check_args("layer_norm_grad", dtype, param_dtype, rows, dim)) return rc;
+  if (grad_x_stride < dim) return efail("layer_norm_grad: grad_x's row stride is shorter than dim %u", dim);
+  const bool params = grad_weight != nullptr || grad_bias != nullptr;
+  if (rows == 0) {  // sums over no rows
+    for (float* p : {grad_weight, grad_bias})
+      if (p != nullptr && !accumulate) k_zero<<<static_cast<unsigned>(ceil_div(dim, 256)), 256, 0, S(stream)>>>(p, dim);
+    return elaunch("omr_layer_norm_grad");
+  }
+  if (grad_out == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || grad_x == nullptr)
+    return efail("layer_norm_grad: NULL pointer");
+  if (params && (workspace == nullptr || !aligned(workspace, 16)))
+    return efail("layer_norm_grad: the parameters' gradients need a 16-byte aligned workspace");
+  if (params && workspace_bytes < omr_layer_norm_grad_workspace_bytes(rows, dim))
+    return efail("layer_norm_grad: workspace of %zu bytes, %zu needed", workspace_bytes,
+                 omr_layer_norm_grad_workspace_bytes(rows, dim));
+  NormArgs a{};
+  a.x = x;
+  a.xstride = x_stride;
+  a.dy = grad_out;
+  a.dystride = grad_stride;
+  a.w = weight;
+  a.out = grad_x;
+  a.ostride = grad_x_stride;
+  a.mean = const_cast<float*>(mean);
+  a.rstd = const_cast<float*>(rstd);
+  a.partial = params ? static_cast<float*>(workspace) : nullptr;
+  a.rows = rows;
+  a.dim = dim;
+  a.inv_dim = 1.0f / static_cast<float>(dim);
+  const int wpr = waves_per_row(dim);
+  const uint32_t blocks = grad_blocks(rows, dim);
+  const int rc = with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    auto go = [&](auto p) {
+      using P = decltype(p);
+      if (wpr > 16) {  // (the parameters first: grad_x may be grad_out or x)
+        if (params) {
+          const dim3 grid(static_cast<unsigned>(ceil_div(dim, 64)), blocks);
+          k_norm_params_any<T><<<grid, 64 * kAnyWaves, 0, S(stream)>>>(a);
+          if (const int rc = elaunch("omr_layer_norm_grad (parameters)")) return rc;
+        }
+        k_norm_dx_any<T, P><<<static_cast<unsigned>(rows < 2048 ? rows : 2048), 64 * kAnyWaves, 0, S(stream)>>>(a);
+        return elaunch("omr_layer_norm_grad");
+      }
+      constexpr int W = 16 / sizeof(T);
+      const bool wide = dim % W == 0 && x_stride % W == 0 && grad_stride % W == 0 && grad_x_stride % W == 0 &&
+                        aligned(x, 16) && aligned(grad_out, 16) && aligned(grad_x, 16) &&
+                        aligned(weight, W * sizeof(P) < 16 ? W * sizeof(P) : 16);
+      return with_shape<W>(wide, wpr, [&](auto vec, auto waves) {
+        constexpr int VEC = decltype(vec)::value, WPR = decltype(waves)::value;
+        k_norm_grad<T, P, VEC, WPR><<<blocks, WPR == 1 ? 256 : 64 * WPR, 0, S(stream)>>>(a);
+        return elaunch("omr_layer_norm_grad");
+      });
+    };
+    return param_dtype == OMR_F32 ? go(float{}) : go(T{});
+  });
+  if (rc != 0 || !params) return rc;
+  k_norm_params<<<static_cast<unsigned>(ceil_div(2ull * dim, 64)), 64 * kAnyWaves, 0, S(stream)>>>(
+      a.partial, blocks, dim, grad_weight, grad_bias, accumulate != 0);
+  return elaunch("omr_layer_norm_grad (sum)");
+}
+
+}  // extern "C"

@@ -21,6 +21,7 @@ c_int = ctypes.c_int
 c_vp = ctypes.c_void_p
 c_dbl = ctypes.c_double
 c_size = ctypes.c_size_t
+c_f32 = ctypes.c_float
 
 OMR_EINVAL = -1
 OMR_MAX_WORKERS = 16
@@ -95,6 +96,15 @@ SIGNATURES = {
     "omr_msg_unpack_f32": (c_int, [c_vp, c_vp, c_vp, c_vp, c_u32, c_u32, c_u32, c_u32, c_vp, c_vp]),
     "omr_sparse_block_sum_f32": (c_int, [c_vp, c_vp, c_vp, c_u32, c_u64, c_vp, c_u64, c_u32, c_vp, c_u32, c_u32,
                                          c_vp, c_vp]),
+    "omr_embed": (c_int, [c_vp, c_int, c_u64, c_u32, c_u64, c_vp, c_int, c_u64, c_f32, c_vp, c_int, c_u64, c_vp]),
+    "omr_embed_grad_workspace_bytes": (c_size, [c_u64, c_u64, c_u32]),
+    "omr_embed_grad_f32": (c_int, [c_vp, c_int, c_u64, c_vp, c_int, c_u64, c_u64, c_u32, c_f32, c_vp, c_u64, c_int,
+                                   c_vp, c_size, c_vp]),
+    "omr_layer_norm": (c_int, [c_vp, c_int, c_u64, c_u32, c_u64, c_vp, c_vp, c_int, c_f32, c_vp, c_u64, c_vp, c_vp,
+                               c_vp]),
+    "omr_layer_norm_grad_workspace_bytes": (c_size, [c_u64, c_u32]),
+    "omr_layer_norm_grad": (c_int, [c_vp, c_u64, c_vp, c_int, c_u64, c_u32, c_u64, c_vp, c_vp, c_vp, c_int, c_vp,
+                                    c_u64, c_vp, c_vp, c_int, c_vp, c_size, c_vp]),
     "omr_host_last_error": (ctypes.c_char_p, []),
     "omr_host_register": (c_int, [c_vp, c_size]),
     "omr_host_unregister": (c_int, [c_vp]),

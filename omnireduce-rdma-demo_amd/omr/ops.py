@@ -282,6 +282,242 @@ def block_sum(inputs: Sequence[torch.Tensor], block_list: torch.Tensor, num: int
     return out
 
 
+# ------------------------------------------------------------------ operators that make the gradient
+
+# The two ends of a language model: their parameter gradients are the fp32 tensors the all-reduce sums.  Every output may
+# be given (a view of the flat gradient, say); what is not given is allocated on the call's stream.  Work runs on
+# `stream`, or on the current stream of the tensors' device.  A plan's workspace serves one call at a time: calls that
+# may overlap (two streams, two captured graphs replayed side by side) need a plan each, and a captured graph needs its
+# plan and its tensors for as long as it is replayed.
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class _Call:
+    """The device and stream of one call: every tensor must be on that device, which is made the current one."""
+
+    __slots__ = ("device", "stream", "ptr", "_guard")
+
+    def __init__(self, device: torch.device, stream: Optional[torch.cuda.Stream]):
+        if device.type != "cuda":
+            raise ValueError("expected a device (HIP) tensor")
+        self.device = device
+        if stream is not None and stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        self.stream = stream
+        self.ptr = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+        self._guard = None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.device.index:
+            self._guard = torch.cuda.device(self.device)
+            self._guard.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+        return False
+
+    def empty(self, shape, dtype) -> torch.Tensor:
+        if self.stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(self.stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def on(self, t: torch.Tensor, name: str) -> int:
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, expected {self.device}")
+        return t.data_ptr()
+
+    def rows(self, t: torch.Tensor, name: str, dim: Optional[int] = None, rows: Optional[int] = None,
+             dtype: Optional[torch.dtype] = None, out: bool = False):
+        """(pointer, rows, dim, row stride) of a tensor taken as rows of its last dimension."""
+        if t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
+            raise ValueError(f"{name}: element type {t.dtype}" + (f", expected {dtype}" if dtype is not None else ""))
+        ptr = self.on(t, name)
+        shape = t.shape
+        if t.dim() < 1 or shape[-1] == 0 or (dim is not None and shape[-1] != dim):
+            raise ValueError(f"{name}: rows of {dim if dim is not None else 'at least one'} elements expected, got "
+                             f"shape {tuple(shape)}")
+        d = shape[-1]
+        n = t.numel() // d
+        if rows is not None and n != rows:
+            raise ValueError(f"{name}: {rows} rows expected, got shape {tuple(shape)}")
+        if d > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name}: the elements of a row must be consecutive (stride {t.stride()})")
+        if n <= 1 or t.dim() == 1:
+            return ptr, n, d, d
+        if t.dim() == 2:
+            stride = t.stride(0)
+        elif t.is_contiguous():
+            stride = d
+        else:
+            raise ValueError(f"{name}: more than two dimensions must be contiguous (stride {t.stride()})")
+        if out and stride < d:
+            raise ValueError(f"{name}: an output's rows must not overlap (stride {t.stride()})")
+        return ptr, n, d, stride
+
+    def vector(self, t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype = torch.float32) -> Optional[int]:
+        if t is None:
+            return None
+        if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name}: expected contiguous {dtype}[{n}], got {t.dtype}{tuple(t.shape)}")
+        return self.on(t, name)
+
+    def ids(self, t: torch.Tensor, name: str):
+        if t.dtype not in (torch.int32, torch.int64) or not t.is_contiguous():
+            raise ValueError(f"{name}: expected contiguous int32 or int64, got {t.dtype} (stride {t.stride()})")
+        return self.on(t, name), int(t.dtype == torch.int64), t.numel()
+
+
+class _Workspace:
+    """Device memory of a plan: allocated once, lent to one call at a time."""
+
+    def __init__(self, nbytes: int, device):
+        self.bytes = nbytes
+        self.tensor = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+        self.device = self.tensor.device
+        self._home = torch.cuda.current_stream(self.device).cuda_stream
+
+    def lend(self, call: _Call) -> int:
+        if call.device != self.device:
+            raise ValueError(f"the plan is on {self.device}, the tensors on {call.device}")
+        if call.ptr != self._home:  # used away from the stream it was allocated on: not reused before that work is done
+            self.tensor.record_stream(call.stream if call.stream is not None
+                                      else torch.cuda.current_stream(call.device))
+        return self.tensor.data_ptr()
+
+
+def embed(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None,
+          out_dtype: Optional[torch.dtype] = None, stream=None) -> torch.Tensor:
+    """Embedding lookup: out[..., :] = scale * table[ids, :], rounded once to out's type (default: the table's).  An id
+    outside [0, rows) names no row (padding): a row of zeros."""
+    with _Call(table.device, stream) as call:
+        if table.dim() != 2:
+            raise ValueError(f"table: expected [rows, dim], got shape {tuple(table.shape)}")
+        tp, rows, dim, tstride = call.rows(table, "table")
+        ip, ids64, n = call.ids(ids, "ids")
+        if out is None:
+            out = call.empty((*ids.shape, dim), out_dtype if out_dtype is not None else table.dtype)
+        op, _, _, ostride = call.rows(out, "out", dim, n, out_dtype, out=True)
+        _lib.check(_lib.load().omr_embed(tp, _DTYPES[table.dtype], rows, dim, tstride, ip, ids64, n, scale, op,
+                                         _DTYPES[out.dtype], ostride, call.ptr), "omr_embed")
+    return out
+
+
+class EmbedGradPlan:
+    """The embedding table's fp32 gradient by sorted tokens, for at most max_tokens tokens a call."""
+
+    def __init__(self, max_tokens: int, num_rows: int, dim: int, device="cuda"):
+        self.max_tokens, self.num_rows, self.dim = max_tokens, num_rows, dim
+        self.workspace = _Workspace(_lib.load().omr_embed_grad_workspace_bytes(max_tokens, num_rows, dim), device)
+
+    def run(self, grad_out: torch.Tensor, ids: torch.Tensor, grad_table: Optional[torch.Tensor] = None,
+            scale: float = 1.0, accumulate: bool = False, stream=None) -> torch.Tensor:
+        """grad_table[v, :] = scale * (sum of grad_out's rows whose id is v, in token order), every row of it, or added
+        to the rows that tokens name (accumulate).  Ids outside [0, rows) contribute nothing."""
+        with _Call(grad_out.device, stream) as call:
+            ip, ids64, n = call.ids(ids, "ids")
+            if n > self.max_tokens:
+                raise ValueError(f"{n} tokens, the plan is for {self.max_tokens}")
+            gp, _, _, gstride = call.rows(grad_out, "grad_out", self.dim, n)
+            if grad_table is None:
+                if accumulate:
+                    raise ValueError("accumulate needs a grad_table")
+                grad_table = call.empty((self.num_rows, self.dim), torch.float32)
+            tp, _, _, tstride = call.rows(grad_table, "grad_table", self.dim, self.num_rows, torch.float32, out=True)
+            _lib.check(_lib.load().omr_embed_grad_f32(gp, _DTYPES[grad_out.dtype], gstride, ip, ids64, n, self.num_rows,
+                                                      self.dim, scale, tp, tstride, int(accumulate),
+                                                      self.workspace.lend(call), self.workspace.bytes, call.ptr),
+                       "omr_embed_grad_f32")
+        return grad_table
+
+
+@dataclass
+class LayerNormResult:
+    out: torch.Tensor
+    mean: torch.Tensor  # fp32, one a row
+    rstd: torch.Tensor
+
+
+@dataclass
+class LayerNormGrads:
+    grad_x: torch.Tensor
+    grad_weight: Optional[torch.Tensor]  # fp32 [dim]
+    grad_bias: Optional[torch.Tensor]
+
+
+def _param(call: _Call, t: Optional[torch.Tensor], name: str, x: torch.Tensor, dim: int):
+    if t is not None and t.dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"{name}: expected fp32 or {x.dtype}, got {t.dtype}")
+    return call.vector(t, name, dim, t.dtype if t is not None else torch.float32)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, out: Optional[torch.Tensor] = None, mean: Optional[torch.Tensor] = None,
+               rstd: Optional[torch.Tensor] = None, stream=None) -> LayerNormResult:
+    """Layer norm over the last dimension; out may be x.  mean and rstd (fp32, one a row) are what the gradient takes."""
+    with _Call(x.device, stream) as call:
+        xp, n, dim, xstride = call.rows(x, "x")
+        if weight is not None and bias is not None and weight.dtype != bias.dtype:
+            raise ValueError("weight and bias must have one element type")
+        wp, bp = _param(call, weight, "weight", x, dim), _param(call, bias, "bias", x, dim)
+        pdt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+        if out is None:
+            out = call.empty(x.shape, x.dtype)
+        op, _, _, ostride = call.rows(out, "out", dim, n, x.dtype, out=True)
+        if mean is None:
+            mean = call.empty(x.shape[:-1], torch.float32)
+        if rstd is None:
+            rstd = call.empty(x.shape[:-1], torch.float32)
+        _lib.check(_lib.load().omr_layer_norm(xp, _DTYPES[x.dtype], n, dim, xstride, wp, bp, _DTYPES[pdt], eps, op,
+                                              ostride, call.vector(mean, "mean", n), call.vector(rstd, "rstd", n),
+                                              call.ptr), "omr_layer_norm")
+    return LayerNormResult(out, mean, rstd)
+
+
+class LayerNormGradPlan:
+    """The layer norm's backward pass, with the reduction of the weight's and bias's gradients, for at most max_rows
+    rows a call."""
+
+    def __init__(self, max_rows: int, dim: int, device="cuda"):
+        self.max_rows, self.dim = max_rows, dim
+        self.workspace = _Workspace(_lib.load().omr_layer_norm_grad_workspace_bytes(max_rows, dim), device)
+
+    def run(self, grad_out: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+            weight: Optional[torch.Tensor] = None, grad_x: Optional[torch.Tensor] = None,
+            grad_weight: Optional[torch.Tensor] = None, grad_bias: Optional[torch.Tensor] = None,
+            accumulate: bool = False, params: bool = True, stream=None) -> LayerNormGrads:
+        """grad_x (may be grad_out or x), and the fp32 gradients of weight and bias, written or added to what is there
+        (accumulate).  params=False: grad_x alone."""
+        with _Call(x.device, stream) as call:
+            xp, n, dim, xstride = call.rows(x, "x", self.dim)
+            if n > self.max_rows:
+                raise ValueError(f"{n} rows, the plan is for {self.max_rows}")
+            gp, _, _, gstride = call.rows(grad_out, "grad_out", dim, n, x.dtype)
+            wp = _param(call, weight, "weight", x, dim)
+            pdt = weight.dtype if weight is not None else torch.float32
+            if grad_x is None:
+                grad_x = call.empty(x.shape, x.dtype)
+            op, _, _, ostride = call.rows(grad_x, "grad_x", dim, n, x.dtype, out=True)
+            if not params:
+                if grad_weight is not None or grad_bias is not None:
+                    raise ValueError("params=False takes no grad_weight or grad_bias")
+            elif accumulate:
+                if grad_weight is None and grad_bias is None:
+                    raise ValueError("accumulate needs a grad_weight or a grad_bias")
+            else:
+                grad_weight = grad_weight if grad_weight is not None else call.empty((dim,), torch.float32)
+                grad_bias = grad_bias if grad_bias is not None else call.empty((dim,), torch.float32)
+            _lib.check(_lib.load().omr_layer_norm_grad(
+                gp, gstride, xp, _DTYPES[x.dtype], n, dim, xstride, call.vector(mean, "mean", n),
+                call.vector(rstd, "rstd", n), wp, _DTYPES[pdt], op, ostride, call.vector(grad_weight, "grad_weight", dim),
+                call.vector(grad_bias, "grad_bias", dim), int(accumulate), self.workspace.lend(call),
+                self.workspace.bytes, call.ptr), "omr_layer_norm_grad")
+        return LayerNormGrads(grad_x, grad_weight, grad_bias)
+
+
 # ------------------------------------------------------------------ host-resident end-to-end path
 
 class HostPlan:

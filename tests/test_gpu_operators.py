@@ -1,0 +1,398 @@
+"""The operators that make the gradient (embedding lookup and its gradient, layer norm forward and backward, the
+vocabulary loss) against their formulas in 64 bits.
+
+Tolerances are worst-case rounding bounds: u = 2^-24 is half an fp32 step, a sum of n terms in any order is off by at
+most n u times the sum of their magnitudes, and a result rounded to type t adds finfo(t).eps / 2 of its magnitude (and
+half the smallest subnormal step, where fp16 underflows)."""
+import math
+
+import pytest
+import torch
+
+from omr import ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+NAN = float("nan")
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    return 2.0 ** -25 if t == F16 else 2.0 ** -149
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def rand(shape, dtype, g, std=1.0, mean=0.0):
+    return torch.empty(shape, dtype=F32, device="cuda").normal_(mean, std, generator=g).to(dtype)
+
+
+def within(got, ref, tol, what):
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    err = (got.double() - ref).abs()
+    bad = ~(err <= tol)
+    if bool(bad.any()):
+        i = torch.nonzero(bad.flatten())[0].item()
+        tol = tol.expand_as(err) if torch.is_tensor(tol) else torch.full_like(err, tol)
+        pytest.fail(f"{what}: {int(bad.sum())} of {bad.numel()} beyond the bound; first at {i}: got "
+                    f"{got.flatten()[i].item()!r}, formula {ref.flatten()[i].item()!r}, bound {tol.flatten()[i].item()!r}")
+
+
+def strided(t, pad, offset=0):
+    """The same rows `pad` elements further apart, beginning `offset` elements into the allocation."""
+    n, d = t.shape
+    buf = torch.full((offset + n * (d + pad),), -77.0, dtype=t.dtype, device=t.device)
+    v = buf[offset:].view(n, d + pad)[:, :d]
+    v.copy_(t)
+    return v, buf
+
+
+def make_ids(n, rows, g, kind):
+    if kind == "one":
+        return torch.full((n,), rows - 1, device="cuda")
+    if kind == "low":  # a few low ids take most tokens
+        return (torch.rand(n, generator=g, device="cuda") ** 6 * rows).long().clamp_(max=rows - 1)
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    if kind == "padded":
+        ids[torch.rand(n, generator=g, device="cuda") < 0.3] = -1
+        ids[torch.rand(n, generator=g, device="cuda") < 0.1] = rows
+        ids[torch.rand(n, generator=g, device="cuda") < 0.1] = -(2 ** 31) if n % 2 else 2 ** 31 - 1
+    return ids
+
+
+# ---------------------------------------------------------------------------------------------------- lookup
+
+def embed_ref(table, ids, scale):
+    ok = (ids >= 0) & (ids < table.shape[0])
+    out = torch.zeros(*ids.shape, table.shape[1], dtype=torch.float64, device=ids.device)
+    out[ok] = table.double()[ids[ok].long()] * scale
+    return out
+
+
+@pytest.mark.parametrize("n,rows,dim", [(1, 1, 1), (1, 50, 64), (3, 7, 5), (64, 100, 256), (257, 1000, 1000),
+                                        (1000, 333, 515), (2, 3, 20000), (5000, 70, 72)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embed(gpu, n, rows, dim, dtype):
+    g = gen(n + rows)
+    table = rand((rows, dim), dtype, g)
+    for kind, it, scale, ot in [("any", torch.int64, 1.0, dtype), ("padded", torch.int32, 5.656854, dtype),
+                                ("padded", torch.int64, -0.37, F32), ("any", torch.int32, 1.0, BF16)]:
+        ids = make_ids(n, rows, g, kind).to(it)
+        got = ops.embed(table, ids, scale=scale, out_dtype=ot)
+        scale32 = torch.tensor(scale, dtype=F32).item()
+        ref = embed_ref(table, ids.long(), scale32)
+        assert got.dtype == ot
+        within(got, ref, ref.abs() * (half(ot) + 2 * U) + tiny(ot), (kind, it, ot))
+
+
+@pytest.mark.parametrize("dim,pad,offset", [(64, 8, 0), (64, 3, 0), (64, 8, 1), (61, 3, 5)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embed_strides_shape_and_untouched_memory(gpu, dim, pad, offset, dtype):
+    g = gen(5)
+    table, _ = strided(rand((90, dim), dtype, g), pad, offset)
+    ids = make_ids(42, 90, g, "padded").view(6, 7)
+    out, buf = strided(torch.zeros(42, dim, dtype=dtype, device="cuda"), pad, offset)
+    before = buf.clone()
+    assert ops.embed(table, ids, out=out) is out
+    within(out, embed_ref(table, ids, 1.0).view(42, dim), 0.0, "strided")
+    out.fill_(0)
+    assert torch.equal(buf, before)  # nothing between or behind the rows
+    assert ops.embed(table, ids).shape == (6, 7, dim)
+    one = rand((1, dim), dtype, g).expand(30, dim)  # a broadcast table: rows a stride of 0 apart
+    assert torch.equal(ops.embed(one, ids.clamp(0, 29)), one[0].expand(6, 7, dim))
+
+
+def test_embed_empty_and_far(gpu):
+    table = torch.ones(4, 8, device="cuda")
+    assert ops.embed(table, torch.empty(0, dtype=torch.int64, device="cuda")).shape == (0, 8)
+    none = torch.empty(0, 8, device="cuda")
+    assert not ops.embed(none, torch.tensor([0, 1], device="cuda")).any()
+    # offsets past 2^32 elements: a table of 2^21 + 3 rows of 2050 in bf16 (8 GiB)
+    big = torch.empty((1 << 21) + 3, 2050, dtype=BF16, device="cuda")
+    ids = torch.tensor([big.shape[0] - 1, 0, 1 << 20], device="cuda")
+    for k, i in enumerate(ids.tolist()):
+        big[i] = torch.arange(2050, device="cuda") % 200 + k
+    assert torch.equal(ops.embed(big, ids), big[ids])
+
+
+# ---------------------------------------------------------------------------------------------------- its gradient
+
+def embed_grad_ref(grad, ids, rows, scale):
+    """The gradient and its bound: (terms + 2) u times the terms' magnitudes (the sums, the scale)."""
+    ok = (ids >= 0) & (ids < rows)
+    i, g = ids[ok].long(), grad[ok].double() * scale
+    ref = torch.zeros(rows, grad.shape[1], dtype=torch.float64, device=grad.device).index_put_((i,), g, accumulate=True)
+    mag = torch.zeros_like(ref).index_put_((i,), g.abs(), accumulate=True)
+    cnt = torch.bincount(i, minlength=rows).double()[:, None]
+    return ref, mag * (cnt + 2) * U, cnt[:, 0] > 0
+
+
+@pytest.mark.parametrize("n,rows,dim,kind", [
+    (0, 5, 8, "any"), (1, 1, 1, "any"), (1, 3000, 64, "any"), (64, 10, 4, "any"), (65, 10, 4, "one"),
+    (63, 1, 100, "one"), (4097, 1, 36, "one"), (1000, 17, 129, "padded"), (1000, 17, 1028, "low"),
+    (5000, 2000, 515, "low"), (4096, 300, 256, "padded"), (4097, 300, 256, "padded"), (20000, 1025, 96, "low"),
+    (3000, 300001, 20, "any"), (300, 2100, 5000, "padded"), (129, 2, 5000, "one"), (70000, 3, 12, "any")])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embed_grad(gpu, n, rows, dim, kind, dtype):
+    g = gen(n + dim)
+    grad = rand((n, dim), dtype, g)
+    ids = make_ids(n, rows, g, kind)
+    bad = (ids < 0) | (ids >= rows)
+    grad[bad] = NAN  # a padded token's gradient is not looked at
+    plan = ops.EmbedGradPlan(n, rows, dim)
+    for it, scale in [(torch.int64, 1.0), (torch.int32, 0.1)]:
+        scale32 = torch.tensor(scale, dtype=F32).item()
+        ref, tol, named = embed_grad_ref(grad, ids, rows, scale32)
+        got = torch.full((rows, dim), NAN, device="cuda")
+        plan.run(grad, ids.to(it), got, scale=scale)
+        within(got, ref, tol, (it, "write"))
+        base = rand((rows, dim), F32, g)
+        acc = base.clone()
+        plan.run(grad, ids.to(it), acc, scale=scale, accumulate=True)
+        within(acc, ref + base.double(), tol + U * (ref + base.double()).abs(), (it, "accumulate"))
+        assert torch.equal(acc[~named], base[~named])
+        again = torch.empty_like(got)
+        plan.run(grad, ids.to(it), again, scale=scale)
+        assert torch.equal(got, again)  # the same bits
+
+
+@pytest.mark.parametrize("dim,pad,offset", [(64, 4, 0), (64, 4, 1), (64, 1, 0), (33, 2, 3)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embed_grad_strides_and_untouched_memory(gpu, dim, pad, offset, dtype):
+    g = gen(9)
+    grad, _ = strided(rand((300, dim), dtype, g), pad, offset)
+    ids = make_ids(300, 40, g, "low")
+    out, buf = strided(torch.zeros(40, dim, device="cuda"), pad, offset)
+    before = buf.clone()
+    plan = ops.EmbedGradPlan(512, 40, dim)
+    plan.run(grad, ids, out)
+    ref, tol, _ = embed_grad_ref(grad, ids, 40, 1.0)
+    within(out, ref, tol, "strided")
+    out.fill_(0)
+    assert torch.equal(buf, before)
+    one = rand((1, dim), dtype, g).expand(300, dim)  # the gradient of a sum: one row for every token
+    ref, tol, _ = embed_grad_ref(one, ids, 40, 1.0)
+    within(plan.run(one, ids), ref, tol, "broadcast")
+
+
+def test_embed_grad_is_the_lookups(gpu):
+    """<grad(dy), E> = <dy, embed(E)> for any E: the backward is the forward's transpose (in 64 bits of its outputs)."""
+    g = gen(3)
+    table, dy = rand((500, 48), F32, g), rand((2000, 48), F32, g)
+    ids = make_ids(2000, 500, g, "padded")
+    a = (ops.EmbedGradPlan(2000, 500, 48).run(dy, ids, scale=3.0).double() * table.double()).sum().item()
+    b = (ops.embed(table, ids, scale=3.0).double() * dy.double()).sum().item()
+    # each output is off by at most (64 + 2) u of its terms (no row has 64 tokens' worth of more), the rest is exact
+    mag = (embed_ref(table, ids, 3.0).abs() * dy.double().abs()).sum().item()
+    assert torch.bincount(ids[(ids >= 0) & (ids < 500)]).max().item() <= 64
+    assert abs(a - b) <= 70 * U * mag
+
+
+# ---------------------------------------------------------------------------------------------------- layer norm
+
+def depth(dim):
+    """Additions behind each other in a row's sum: a lane's, the wave's six, the waves'."""
+    return (16 if dim <= 16384 else dim // 1024 + 1) + 6 + 16
+
+
+def norm_ref(x, w, b, eps):
+    x = x.double()
+    mean = x.mean(-1, keepdim=True)
+    var = (x - mean).square().mean(-1, keepdim=True)
+    rstd = 1 / torch.sqrt(var + eps)
+    xh = (x - mean) * rstd
+    w = torch.ones(x.shape[-1], device=x.device) if w is None else w
+    b = torch.zeros(x.shape[-1], device=x.device) if b is None else b
+    y = xh * w.double() + b.double()
+    # the mean is off by m = k u mean|x|; the squared distances by k + 4 roundings of u and m^2; half of that in rstd,
+    # with the root, the quotient and the two products behind it
+    k = depth(x.shape[-1]) + 2
+    m = k * U * x.abs().mean(-1, keepdim=True)
+    rel = ((k + 4) * U + m * m / (var + eps)) / 2 + 6 * U
+    tol_y = w.double().abs() * (xh.abs() * rel + m * rstd * (1 + rel)) + 2 * U * (y.abs() + b.double().abs())
+    return y, mean[..., 0], rstd[..., 0], tol_y, m[..., 0], (rel * rstd)[..., 0]
+
+
+SHAPES = [(1, 1), (1, 8), (5, 3), (3, 64), (7, 1000), (9, 1024), (2, 1025), (5, 2048), (4, 2056), (3, 4096), (2, 5003),
+          (3, 8192), (2, 16384), (2, 16385), (1, 40000), (2100, 72), (2500, 1032)]
+
+
+@pytest.mark.parametrize("rows,dim", SHAPES)
+@pytest.mark.parametrize("dtype,pdt", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+def test_layer_norm(gpu, rows, dim, dtype, pdt):
+    g = gen(rows + dim)
+    x = rand((rows, dim), dtype, g, std=2.0, mean=30.0)
+    w, b = rand((dim,), pdt, g, mean=1.0), rand((dim,), pdt, g)
+    for weight, bias in [(w, b), (None, None), (w, None)]:
+        r = ops.layer_norm(x, weight, bias, eps=1e-5)
+        y, mean, rstd, tol_y, tol_m, tol_r = norm_ref(x, weight, bias, torch.tensor(1e-5, dtype=F32).item())
+        within(r.mean, mean, tol_m + U * mean.abs(), "mean")
+        within(r.rstd, rstd, tol_r, "rstd")
+        within(r.out, y, tol_y * (1 + half(dtype)) + half(dtype) * y.abs() + tiny(dtype), "out")
+
+
+@pytest.mark.parametrize("rows,dim", SHAPES)
+@pytest.mark.parametrize("dtype,pdt", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+def test_layer_norm_grad(gpu, rows, dim, dtype, pdt):
+    g = gen(rows * 3 + dim)
+    x, dy = rand((rows, dim), dtype, g, std=2.0, mean=1.0), rand((rows, dim), dtype, g)
+    w = rand((dim,), pdt, g, mean=1.0)
+    plan = ops.LayerNormGradPlan(rows + 3, dim)
+    for weight in (w, None):
+        f = ops.layer_norm(x, weight)
+        r = plan.run(dy, x, f.mean, f.rstd, weight)
+        xh = (x.double() - f.mean.double()[:, None]) * f.rstd.double()[:, None]
+        d = dy.double()
+        gw = d * (weight.double() if weight is not None else 1.0)
+        s1, s2 = gw.mean(1, keepdim=True), (gw * xh).mean(1, keepdim=True)
+        rs = f.rstd.double()[:, None]
+        dx = (gw - s1 - xh * s2) * rs
+        k = depth(dim)
+        tol = rs * U * (4 * gw.abs() + (k + 6) * gw.abs().mean(1, keepdim=True) +
+                        (k + 10) * xh.abs() * (gw * xh).abs().mean(1, keepdim=True)) + 2 * U * dx.abs()
+        within(r.grad_x, dx, tol * (1 + half(dtype)) + half(dtype) * dx.abs() + tiny(dtype), "grad_x")
+        tol_w, tol_b = (rows + 4) * U * (d * xh).abs().sum(0), rows * U * d.abs().sum(0)
+        within(r.grad_weight, (d * xh).sum(0), tol_w, "grad_weight")
+        within(r.grad_bias, d.sum(0), tol_b, "grad_bias")
+        gw0, gb0 = rand((dim,), F32, g), rand((dim,), F32, g)
+        gw1, gb1 = gw0.clone(), gb0.clone()
+        r2 = plan.run(dy, x, f.mean, f.rstd, weight, grad_weight=gw1, grad_bias=gb1, accumulate=True)
+        assert torch.equal(r2.grad_x, r.grad_x)  # the same bits
+        assert torch.equal(gw1, gw0 + r.grad_weight) and torch.equal(gb1, gb0 + r.grad_bias)
+        alone = plan.run(dy, x, f.mean, f.rstd, weight, params=False)
+        assert alone.grad_weight is None and torch.equal(alone.grad_x, r.grad_x)
+        onto = dy.clone()
+        assert torch.equal(plan.run(onto, x, f.mean, f.rstd, weight, grad_x=onto).grad_weight, r.grad_weight)
+        assert torch.equal(onto, r.grad_x)
+
+
+def test_layer_norm_grad_is_the_slope(gpu):
+    """Directional differences of the forward's formula in 64 bits against the gradient (fp32 inputs)."""
+    g = gen(8)
+    x, dy, w, b = rand((6, 200), F32, g), rand((6, 200), F32, g), rand((200,), F32, g, mean=1.0), rand((200,), F32, g)
+    f = ops.layer_norm(x, w, b)
+    r = ops.LayerNormGradPlan(6, 200).run(dy, x, f.mean, f.rstd, w)
+
+    def loss(x, w, b):
+        return (norm_ref(x, w, b, 1e-5)[0] * dy.double()).sum().item()
+    h = 1e-4
+    for t, grad in ((0, r.grad_x), (1, r.grad_weight), (2, r.grad_bias)):
+        args = [x.double(), w.double(), b.double()]
+        v = torch.empty_like(args[t]).normal_(generator=g)
+        up, dn = list(args), list(args)
+        up[t], dn[t] = args[t] + h * v, args[t] - h * v
+        slope = (loss(*up) - loss(*dn)) / (2 * h)
+        got = (grad.double() * v).sum().item()
+        # central differences: h^2 of third derivatives (of order 10 here) and fp32 bounds of the 1200 products
+        assert abs(slope - got) <= 1e-5 * (grad.double() * v).abs().sum().item() + 1e-5
+
+
+@pytest.mark.parametrize("dim,pad,offset", [(256, 8, 0), (256, 1, 0), (256, 8, 3), (77, 2, 1)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_norm_strides_and_untouched_memory(gpu, dim, pad, offset, dtype):
+    g = gen(2)
+    x0, dy0 = rand((37, dim), dtype, g), rand((37, dim), dtype, g)
+    w, b = rand((dim,), F32, g), rand((dim,), F32, g)
+    x, _ = strided(x0, pad, offset)
+    dy, _ = strided(dy0, pad, offset)
+    out, buf = strided(torch.zeros_like(x0), pad, offset)
+    before = buf.clone()
+    f, plain = ops.layer_norm(x, w, b, out=out), ops.layer_norm(x0, w, b)
+    y, _, _, tol, _, _ = norm_ref(x0, w, b, torch.tensor(1e-5, dtype=F32).item())
+    within(out, y, tol * (1 + half(dtype)) + half(dtype) * y.abs() + tiny(dtype), "strided")
+    gx, gbuf = strided(torch.zeros_like(x0), pad, offset)
+    plan = ops.LayerNormGradPlan(37, dim)
+    r = plan.run(dy, x, plain.mean, plain.rstd, w, grad_x=gx)
+    q = plan.run(dy0, x0, plain.mean, plain.rstd, w)
+    # a lane's columns depend on the piece width, so sums differ in order: bounds as above on both sides
+    k = depth(dim)
+    for a, c in ((r.grad_x, q.grad_x), (r.grad_weight, q.grad_weight), (r.grad_bias, q.grad_bias)):
+        scale = c.double().abs().max().item() + 1
+        within(a, c.double(), (2 * (k + 60) * U * 20 + 2 * half(a.dtype)) * scale, "strided gradient")
+    for t, bb in ((out, buf), (gx, gbuf)):
+        t.fill_(0)
+        assert torch.equal(bb, before)
+    inplace = x0.clone()
+    assert torch.equal(ops.layer_norm(inplace, w, b, out=inplace).out, plain.out)
+
+
+def test_layer_norm_no_rows_and_shapes(gpu):
+    x = torch.empty(0, 96, device="cuda")
+    f = ops.layer_norm(x)
+    assert f.out.shape == (0, 96) and f.mean.shape == (0,)
+    plan = ops.LayerNormGradPlan(4, 96)
+    r = plan.run(x, x, f.mean, f.rstd)
+    assert not r.grad_weight.any() and not r.grad_bias.any()
+    keep = torch.ones(96, device="cuda")
+    plan.run(x, x, f.mean, f.rstd, grad_weight=keep, grad_bias=keep.clone(), accumulate=True)
+    assert torch.equal(keep, torch.ones(96, device="cuda"))
+    y = ops.layer_norm(torch.randn(2, 3, 96, device="cuda"))
+    assert y.out.shape == (2, 3, 96) and y.mean.shape == (2, 3)
+    inf = torch.randn(3, 96, device="cuda")
+    inf[1, 5] = float("inf")
+    out = ops.layer_norm(inf).out
+    assert not torch.isfinite(out[1]).any() and torch.isfinite(out[[0, 2]]).all()
+
+
+# ---------------------------------------------------------------------------------------------------- streams, graphs
+
+def test_operators_in_a_graph_and_on_streams(gpu):
+    """A captured lookup -> norm -> norm gradient -> table gradient, replayed on new inputs with eager work between the
+    replays, gives the eager bits each time; and two streams with a plan each do not disturb each other."""
+    g = gen(4)
+    T, V, D = 700, 500, 264
+    table, w, b = rand((V, D), BF16, g), rand((D,), F32, g), rand((D,), F32, g)
+    ids = make_ids(T, V, g, "low")
+    dy = rand((T, D), BF16, g)
+
+    class Step:
+        def __init__(self):
+            self.ng, self.eg = ops.LayerNormGradPlan(T, D), ops.EmbedGradPlan(T, V, D)
+            self.x = torch.empty(T, D, dtype=BF16, device="cuda")
+            self.y, self.gx = torch.empty_like(self.x), torch.empty_like(self.x)
+            self.mean, self.rstd = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+            self.flat = torch.empty(V * D + 2 * D, device="cuda")  # one flat gradient: table, weight, bias
+
+        def run(self, stream=None):
+            ops.embed(table, ids, scale=2.0, out=self.x, stream=stream)
+            f = ops.layer_norm(self.x, w, b, out=self.y, mean=self.mean, rstd=self.rstd, stream=stream)
+            gw, gb = self.flat[V * D:V * D + D], self.flat[V * D + D:]
+            self.ng.run(dy, self.x, f.mean, f.rstd, w, grad_x=self.gx, grad_weight=gw, grad_bias=gb, stream=stream)
+            self.eg.run(self.gx, ids, self.flat[:V * D].view(V, D), scale=2.0, stream=stream)
+
+        def outputs(self):
+            return [t.clone() for t in (self.x, self.y, self.gx, self.flat)]
+
+    eager, captured = Step(), Step()
+    captured.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.run()
+    for k in range(4):
+        ids.copy_(make_ids(T, V, gen(100 + k), ["low", "padded", "one", "any"][k]))
+        dy.copy_(rand((T, D), BF16, gen(200 + k)))
+        eager.run()
+        want = eager.outputs()
+        captured.flat.fill_(NAN)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, captured.outputs())), k
+    other = Step()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, step in zip(streams, (captured, other)):
+            step.run(stream=s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(want, captured.outputs()))
+    assert all(torch.equal(p, q) for p, q in zip(want, other.outputs()))
