@@ -494,6 +494,32 @@ int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* 
                         int param_dtype, void* grad_x, uint64_t grad_x_stride, float* grad_weight, float* grad_bias,
                         int accumulate, void* workspace, size_t workspace_bytes, omr_stream_t stream);
 
+/* Softmax cross entropy over a large vocabulary, without keeping the logits z = hidden weight^T:
+ *   lse[n] = log(sum over v of exp(z[n, v])),  loss[n] = lse[n] - z[n, targets[n]]     (fp32, both required)
+ * hidden [tokens, dim] and weight [vocab, dim]: bf16 or fp16 (`dtype`), dim <= 2^20.  targets: int32, or int64 with
+ * targets64 != 0; a target outside [0, vocab) is none: its loss is 0 (its lse is still that of its row).
+ * Rows of hidden and weight that are whole 16-byte pieces (dim, strides and addresses; strides below 2^22) are read as
+ * they are; others are laid out again in the workspace by each call, which then has to be asked for with pack != 0 (a
+ * dim that is no multiple of 8 implies it). */
+size_t omr_vocab_loss_workspace_bytes(uint64_t max_tokens, uint64_t vocab, uint32_t dim, int pack, int grads);
+int omr_vocab_loss(const void* hidden, uint64_t hidden_stride, const void* weight, uint64_t weight_stride, int dtype,
+                   uint64_t tokens, uint64_t vocab, uint32_t dim, const void* targets, int targets64, float* loss,
+                   float* lse, void* workspace, size_t workspace_bytes, omr_stream_t stream);
+
+/* Its backward pass, from the lse the forward left and grad_loss (fp32, a stride apart; 0: one value for every token):
+ * with G[n, v] = exp(z[n, v] - lse[n]) - (v == targets[n]), recomputed in pieces of the vocabulary and held in `dtype`,
+ *   grad_hidden[n, :] = grad_loss[n] * sum over v of G[n, v] weight[v, :]                                 (dtype)
+ *   grad_weight[v, :] = sum over n of G[n, v] grad_loss[n] hidden[n, :]        (grad_weight_dtype: fp32 or dtype)
+ * either may be NULL; accumulate != 0 adds to grad_weight.  Tokens without a target contribute nothing and get a row of
+ * zeros, whatever their hidden states and grad_loss hold.  An fp32 grad_weight (a bucket of the all-reduce) is summed
+ * in fp32 from terms of `dtype`'s precision.  The workspace needs grads != 0 above. */
+int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* weight, uint64_t weight_stride,
+                        int dtype, uint64_t tokens, uint64_t vocab, uint32_t dim, const void* targets, int targets64,
+                        const float* lse, const float* grad_loss, uint64_t grad_loss_stride, void* grad_hidden,
+                        uint64_t grad_hidden_stride, void* grad_weight, int grad_weight_dtype,
+                        uint64_t grad_weight_stride, int accumulate, void* workspace, size_t workspace_bytes,
+                        omr_stream_t stream);
+
 /* ---------------------------------------------------------------- host-resident end-to-end path */
 
 /* The gradient lives in host memory (the reference's registered region, common.cc:873-914): H2D in row chunks,

@@ -1,0 +1,765 @@
+// omr_loss.hip — softmax cross entropy over a large vocabulary, in pieces of the vocabulary, without the logits.
+//
+//   z = hidden weight^T                     [tokens, vocab]
+//   lse[n] = log sum_v exp z[n, v],  loss[n] = lse[n] - z[n, target[n]]     (0 where the target names no row)
+//   G[n, v] = exp(z[n, v] - lse[n]) - (v == target[n])
+//   grad_hidden[n] = grad_loss[n] sum_v G[n, v] weight[v],  grad_weight[v] (+)= sum_n G[n, v] grad_loss[n] hidden[n]
+//
+// Everything is matrix products on the 16-bit matrix instructions, bound by them from some 256 tokens on (below that by
+// reading the weight).  The forward product keeps no logits: a wave folds its piece of the vocabulary into a running
+// maximum and sum of exponentials a token, and k_merge joins the pieces.  The backward recomputes a piece of the logits
+// (2 T V D of 8 T V D operations), stores G of that piece in 16 bits, and multiplies it with the weight and with the
+// hidden states.
+//
+// Roundings to 16 bits, besides the outputs':
+//   - G, times 2^12 so that fp16 keeps the small probabilities normal (2^-26 and up).  grad_loss stays out of it: a mean's
+//     1 / tokens would shift every target's near -1 to the same place of a binade and bias the whole gradient by its one
+//     rounding error; near -1 itself the error is at most 2^-9 and random.
+//   - hidden[n] * (grad_loss[n] / max |grad_loss|) for grad_weight's sum over tokens: exact where grad_loss is the same
+//     for every token (the mean and the sum), else one rounding.
+// Sums are in fp32 throughout.
+#include "omr_elem.h"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+using namespace omr_elem;
+
+namespace {
+
+constexpr float kGScale = 4096.0f;
+constexpr uint32_t kMaxStride = 1u << 22;  // elements: a tile's 32-bit byte offsets hold 256 rows of it
+
+// 16 zero bytes: what lanes past the end of a product's inner dimension load
+__device__ __attribute__((aligned(16))) uint32_t g_zero[4];
+
+template <class T>
+using frag = vec_t<T, 8>;
+
+__device__ __forceinline__ v4f mma(const frag<__bf16>& a, const frag<__bf16>& b, const v4f& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mma(const frag<_Float16>& a, const frag<_Float16>& b, const v4f& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------- operand tiles
+//
+// C[m, n] = sum_k A(m, k) B(n, k).  An operand is stored with its inner dimension k consecutive (a "row" operand, element
+// (m, k) at p[m ld + k]) or with m consecutive (a "column" operand, p[k ld + m]); neither is transposed in memory.  A
+// workgroup's tile of ROWS x 64 goes from global memory straight into LDS in 16-byte pieces, which fill LDS in lane
+// order; which piece a lane fetches is permuted so that the reads below spread over the banks:
+//   row operand     LDS row m: 8 pieces, piece c at place c ^ (m & 7); a lane reads 8 consecutive k of its row (b128)
+//   column operand  LDS row k: ROWS / 8 pieces in pairs, pair p at p ^ h(k), h = bits 0, 1, 3, 4 of k: the 16 rows that a
+//                   transposing read (ds_read_b64_tr_b16: 4 k of one m a lane) touches at once lie in different banks
+constexpr int kBK = 64;
+
+__device__ __forceinline__ uint32_t pair_hash(uint32_t k) { return (k & 3) | ((k >> 3) & 3) << 2; }
+
+template <class T>
+struct Operand {
+  const T* p;
+  uint64_t ld;
+  uint32_t rows;  // m (or n) extent; a column operand's is a multiple of 8
+};
+
+template <class T, int ROWS, int NT, bool COL>
+struct Tile {
+  static constexpr int kPieces = ROWS * 8 / NT;
+  const char* base;          // this step's tile
+  uint32_t off[kPieces];     // bytes from there
+  uint32_t kfirst[kPieces];  // the piece's first k within a step
+  uint64_t inc;
+
+  __device__ __forceinline__ void init(const Operand<T>& o, uint32_t row0, uint64_t kbegin) {
+    const uint32_t t = threadIdx.x;
+    row0 = min(row0, o.rows - 1);  // (a tile that lies past the end altogether)
+    if constexpr (!COL) {
+      base = reinterpret_cast<const char*>(o.p + row0 * o.ld + kbegin);
+      inc = kBK * sizeof(T);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t q = i * NT + t, m = q >> 3, c = (q & 7) ^ (m & 7);
+        // rows past the end repeat the last one: they reach only results that are not stored
+        const uint32_t row = min(row0 + m, o.rows - 1) - row0;
+        off[i] = static_cast<uint32_t>((row * o.ld + c * 8) * sizeof(T));
+        kfirst[i] = c * 8;
+      }
+    } else {
+      base = reinterpret_cast<const char*>(o.p + kbegin * o.ld + row0);
+      inc = kBK * o.ld * sizeof(T);
+      constexpr uint32_t kRow = ROWS / 8;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t q = i * NT + t, k = q / kRow, c = q % kRow;
+        uint32_t m = ((c >> 1) ^ (pair_hash(k) % (kRow / 2))) * 16 + (c & 1) * 8;
+        if (row0 + m >= o.rows) m = 0;
+        off[i] = static_cast<uint32_t>((k * o.ld + m) * sizeof(T));
+        kfirst[i] = k;
+      }
+    }
+  }
+
+  // one step's tile into `lds`; left: how many k of the inner dimension there still are
+  __device__ __forceinline__ void load(T* lds, uint32_t left) {
+    const uint32_t wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const char* src = base + off[i];
+      if (left < kBK && kfirst[i] >= left) src = reinterpret_cast<const char*>(g_zero);
+      __builtin_amdgcn_global_load_lds(
+          reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
+          reinterpret_cast<__attribute__((address_space(3))) void*>(
+              reinterpret_cast<uintptr_t>(lds + (i * NT + wave * 64) * 8)),
+          16, 0, 0);
+    }
+    base += inc;
+  }
+};
+
+// A wave's fragments of NF times 16 rows from row `row0` on
+template <class T, int ROWS, int NF, bool COL>
+struct Frags {
+  uint32_t at[COL ? NF : 2];
+
+  __device__ __forceinline__ void init(uint32_t row0) {
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    if constexpr (!COL) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) at[s] = ((row0 + r) * 8 + ((s * 4 + g) ^ (r & 7))) * 8;
+    } else {
+      const uint32_t k = 8 * g + (r >> 2), h = pair_hash(k) % (ROWS / 16);
+#pragma unroll
+      for (int i = 0; i < NF; ++i) at[i] = k * ROWS + (((row0 >> 4) + i) ^ h) * 16 + (r & 3) * 4;
+    }
+  }
+
+  __device__ __forceinline__ frag<T> get(const T* lds, int i, int sub) const {
+    if constexpr (!COL) {
+      return *reinterpret_cast<const frag<T>*>(lds + at[sub] + i * 16 * kBK);
+    } else {
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      using lp = __attribute__((address_space(3))) s4*;
+      const T* p = lds + at[i] + sub * 32 * ROWS;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)(p));
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)(p + 4 * ROWS));
+      return __builtin_bit_cast(frag<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// ---------------------------------------------------------------- the product
+//
+// The workgroup's tile is BM x BN, WM x WN waves of (BM / WM) x (BN / WN); two LDS buffers, one barrier a step of 64:
+// behind it the next step's tile starts on its way into the buffer that the step before has done with.
+enum { kStats, kGrad, kHidden, kWeight };
+
+template <class T>
+struct GemmArgs {
+  Operand<T> a, b;
+  uint32_t k;               // inner extent
+  uint32_t mt, nt, splits;  // tiles; the inner dimension in `splits` parts of ksplit
+  uint32_t ksplit;
+  // kStats, kGrad: m = vocabulary rows of the piece (from v0 on), n = tokens
+  const void* targets;
+  int targets64;
+  uint32_t v0, vocab, tokens;
+  float* stats;             // [tokens][2 * pieces]: maximum and sum of each wave's part of the vocabulary
+  uint32_t pieces;
+  float* ztarget;           // [tokens]
+  const float* lse;
+  T* g;                     // [tokens][ldg]
+  uint32_t ldg;
+  // kHidden: m = columns, n = tokens; kWeight: m = columns, n = vocabulary rows of the piece
+  uint32_t dim;
+  float* acc;               // [splits][tokens][dim]
+  int first, last;          // the sum over the pieces begins; is complete and goes to `out`
+  const float* rowscale;    // [tokens]
+  const float* amax;        // [1]
+  void* out;
+  uint64_t ostride;
+  int out_f32, accumulate, wide;  // wide: out takes 4 elements at a time
+};
+
+template <class T>
+__device__ __forceinline__ int target_of(const GemmArgs<T>& a, uint32_t n) {
+  const int64_t t = a.targets64 ? static_cast<const int64_t*>(a.targets)[n] : static_cast<const int32_t*>(a.targets)[n];
+  return t >= 0 && t < a.vocab ? static_cast<int>(t) : -1;
+}
+
+// out[0..3] (+)= v, of which the first `n` exist
+template <class O>
+__device__ __forceinline__ void put4(O* out, v4f v, uint32_t n, int accumulate, int wide) {
+  if (wide && n >= 4) {
+    float f[4];
+    if (accumulate) {
+      load_f32<O, 4>(out, f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = f[i] + v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = v[i];
+    store_f32<O, 4>(out, f);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (static_cast<uint32_t>(i) < n) out[i] = static_cast<O>(accumulate ? static_cast<float>(out[i]) + v[i] : v[i]);
+}
+
+template <class T, int EPI, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
+  constexpr int NT = 64 * WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
+  constexpr bool AC = EPI == kHidden || EPI == kWeight, BC = EPI == kWeight;
+  __shared__ __attribute__((aligned(1024))) T la0[BM * kBK], la1[BM * kBK], lb0[BN * kBK], lb1[BN * kBK];
+  // Workgroup ids go round the 8 XCDs: give each XCD a contiguous stretch of tiles, and walk the stretch in groups of 8
+  // tile rows, so the tiles that run together on an XCD share operands in its L2.
+  uint32_t id = blockIdx.x;
+  const uint32_t all = a.mt * a.nt * a.splits, per = all / 8, rem = all % 8, xcd = id % 8;
+  id = xcd * per + min(xcd, rem) + id / 8;
+  const uint32_t split = id / (a.mt * a.nt);
+  id -= split * (a.mt * a.nt);
+  const uint32_t group = id / (8 * a.nt), gm = min(8u, a.mt - group * 8), in = id - group * 8 * a.nt;
+  const uint32_t m0 = (group * 8 + in % gm) * BM, n0 = in / gm * BN;
+  const uint64_t kbegin = static_cast<uint64_t>(split) * a.ksplit;
+  uint32_t left = min(a.ksplit, static_cast<uint32_t>(a.k - kbegin));
+
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t wm = wave % WM, wn = wave / WM;
+  Tile<T, BM, NT, AC> ta;
+  Tile<T, BN, NT, BC> tb;
+  ta.init(a.a, m0, kbegin);
+  tb.init(a.b, n0, kbegin);
+  Frags<T, BM, MF, AC> fa;
+  Frags<T, BN, NF, BC> fb;
+  fa.init(wm * (BM / WM));
+  fb.init(wn * (BN / WN));
+  v4f acc[MF][NF] = {};
+
+  auto step = [&](T* ca, T* cb, T* na, T* nb) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    left = left > kBK ? left - kBK : 0;
+    if (left != 0) {
+      ta.load(na, left);
+      tb.load(nb, left);
+    }
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      frag<T> x[MF], y[NF];
+#pragma unroll
+      for (int i = 0; i < MF; ++i) x[i] = fa.get(ca, i, sub);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) y[j] = fb.get(cb, j, sub);
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = mma(x[i], y[j], acc[i][j]);
+    }
+  };
+  ta.load(la0, left);
+  tb.load(lb0, left);
+  while (true) {
+    step(la0, lb0, la1, lb1);
+    if (left == 0) break;
+    step(la1, lb1, la0, lb0);
+    if (left == 0) break;
+  }
+
+  // acc[i][j][r] = C[m + 16 i + r, n + 16 j]
+  const uint32_t m = m0 + wm * (BM / WM) + 4 * (lane >> 4), n = n0 + wn * (BN / WN) + (lane & 15);
+  if constexpr (EPI == kStats || EPI == kGrad) {
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      const uint32_t tok = n + 16 * j;
+      const bool real = tok < a.tokens;
+      const int target = real ? target_of(a, tok) : -1;
+      const int at = target - static_cast<int>(a.v0 + m);  // the target's place among this lane's rows
+      if constexpr (EPI == kStats) {
+        float top = -INFINITY, z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (a.v0 + m + 16 * i + r >= a.vocab) acc[i][j][r] = -INFINITY;
+            top = fmaxf(top, acc[i][j][r]);
+          }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float from = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum += __expf(acc[i][j][r] - from);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        const bool here = target >= 0 && at >= 0 && at < 16 * MF && (at & 15) < 4;
+        if (__ballot(here)) {
+#pragma unroll
+          for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (at == 16 * i + r) z = acc[i][j][r];
+          if (here) a.ztarget[tok] = z;
+        }
+        if (real && lane < 16) {
+          const uint32_t piece = m0 / (BM / WM) + wm;
+          float* s = a.stats + (static_cast<uint64_t>(tok) * a.pieces + piece) * 2;
+          *reinterpret_cast<float2*>(s) = make_float2(top, sum);
+        }
+      } else {
+        const float lse = target >= 0 ? a.lse[tok] : 0.0f;
+        const bool here = target >= 0 && at >= 0 && at < 16 * MF && (at & 15) < 4;
+        const bool any = __ballot(here) != 0;
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+          vec_t<T, 4> o;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float p = __expf(acc[i][j][r] - lse);
+            if (any && at == 16 * i + r) p -= 1.0f;
+            if (target < 0 || a.v0 + m + 16 * i + r >= a.vocab) p = 0.0f;
+            o[r] = static_cast<T>(p * kGScale);
+          }
+          if (real) *reinterpret_cast<vec_t<T, 4>*>(a.g + static_cast<uint64_t>(tok) * a.ldg + m + 16 * i) = o;
+        }
+      }
+    }
+  } else if constexpr (EPI == kHidden) {
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      const uint32_t tok = n + 16 * j;
+      if (tok >= a.tokens) continue;
+      const float scale = a.last ? a.rowscale[tok] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        const uint32_t c = m + 16 * i;
+        if (c >= a.dim) continue;
+        float* sum = a.acc + (static_cast<uint64_t>(split) * a.tokens + tok) * a.dim + c;
+        v4f v = acc[i][j];
+        const uint32_t have = a.dim - c;
+        if (!a.first) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (static_cast<uint32_t>(r) < have) v[r] = sum[r] + v[r];
+        }
+        if (a.last) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = scale == 0.0f ? 0.0f : v[r] * scale;
+          put4<T>(static_cast<T*>(a.out) + static_cast<uint64_t>(tok) * a.ostride + c, v, have, 0, a.wide);
+        } else {
+          put4<float>(sum, v, have, 0, a.dim % 4 == 0);
+        }
+      }
+    }
+  } else {
+    const float scale = *a.amax / kGScale;
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      const uint32_t row = n + 16 * j;
+      if (a.v0 + row >= a.vocab) continue;
+      const uint64_t o = static_cast<uint64_t>(a.v0 + row) * a.ostride;
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        const uint32_t c = m + 16 * i;
+        if (c >= a.dim) continue;
+        const v4f v = acc[i][j] * scale;
+        if (a.out_f32)
+          put4<float>(static_cast<float*>(a.out) + o + c, v, a.dim - c, a.accumulate, a.wide);
+        else
+          put4<T>(static_cast<T*>(a.out) + o + c, v, a.dim - c, a.accumulate, a.wide);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the small kernels around it
+
+// A wave a token: joins the pieces' maxima and sums.
+template <class T>
+__global__ __launch_bounds__(256) void k_merge(GemmArgs<T> a, float* loss, float* lse) {
+  const uint32_t tok = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (tok >= a.tokens) return;
+  const float2* s = reinterpret_cast<const float2*>(a.stats) + static_cast<uint64_t>(tok) * a.pieces;
+  float top = -INFINITY, sum = 0.0f;
+  for (uint32_t p = lane; p < a.pieces; p += 64) {
+    const float2 v = s[p];
+    const float up = fmaxf(top, v.x), from = up == -INFINITY ? 0.0f : up;
+    sum = sum * expf(top - from) + v.y * expf(v.x - from);
+    top = up;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const float ot = __shfl_xor(top, d), os = __shfl_xor(sum, d);
+    const float up = fmaxf(top, ot), from = up == -INFINITY ? 0.0f : up;
+    sum = sum * expf(top - from) + os * expf(ot - from);
+    top = up;
+  }
+  if (lane != 0) return;
+  const float l = top + logf(sum);
+  lse[tok] = l;
+  loss[tok] = target_of(a, tok) >= 0 ? l - a.ztarget[tok] : 0.0f;
+}
+
+// The largest |grad_loss| of the tokens with a target (one workgroup), and each token's factor of grad_hidden.
+template <class T>
+__global__ __launch_bounds__(1024) void k_scales(GemmArgs<T> a, const float* grad_loss, uint64_t stride, float* amax,
+                                                 float* rowscale) {
+  __shared__ float top[16];
+  float m = 0.0f;
+  for (uint32_t n = threadIdx.x; n < a.tokens; n += 1024) {
+    const bool keep = target_of(a, n) >= 0;
+    const float g = keep ? grad_loss[n * stride] : 0.0f;
+    rowscale[n] = g / kGScale;
+    // (a NaN is kept: the gradient shall have it)
+    m = m != m || fabsf(g) <= m ? m : fabsf(g);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const float o = __shfl_xor(m, d);
+    m = m != m || o <= m ? m : o;
+  }
+  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 16; ++w) m = m != m || top[w] <= m ? m : top[w];
+  *amax = m;
+}
+
+// Rows copied into whole 16-byte pieces [rows][pdim], zeros behind dim.  With rowscale: each row times its share of the
+// largest grad_loss, and zeros for tokens without a target, whatever they hold.
+template <class T>
+__global__ __launch_bounds__(256) void k_pack(const T* src, uint64_t stride, uint32_t rows, uint32_t dim, uint32_t pdim,
+                                              const float* rowscale, const float* amax, T* dst, int wide) {
+  const uint32_t per = pdim / 8;
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const uint64_t row = i / per;
+  if (row >= rows) return;
+  const uint32_t c = static_cast<uint32_t>(i - row * per) * 8;
+  const T* s = src + row * stride + c;
+  float v[8];
+  float by = 1.0f;
+  if (rowscale != nullptr) by = rowscale[row] == 0.0f ? 0.0f : rowscale[row] * kGScale / *amax;
+  if (by == 0.0f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+  } else {
+    if (wide) {
+      load_f32<T, 8>(s, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = c + k < dim ? static_cast<float>(s[k]) : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= by;
+  }
+  store_f32<T, 8>(dst + row * pdim + c, v);
+}
+
+// grad_hidden = factor * (the parts' sums, in order)
+template <class T>
+__global__ __launch_bounds__(256) void k_join(GemmArgs<T> a) {
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<uint64_t>(a.tokens) * a.dim;
+  if (i >= all) return;
+  const uint32_t tok = static_cast<uint32_t>(i / a.dim), c = static_cast<uint32_t>(i - static_cast<uint64_t>(tok) * a.dim);
+  float v = 0.0f;
+  for (uint32_t s = 0; s < a.splits; ++s) v += a.acc[s * all + i];
+  const float scale = a.rowscale[tok];
+  static_cast<T*>(a.out)[tok * a.ostride + c] = static_cast<T>(scale == 0.0f ? 0.0f : v * scale);
+}
+
+template <class O>
+__global__ __launch_bounds__(256) void k_zero(O* out, uint64_t rows, uint32_t dim, uint64_t stride) {
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / dim;
+  if (row < rows) out[row * stride + (i - row * dim)] = static_cast<O>(0.0f);
+}
+
+// ---------------------------------------------------------------- launches
+
+uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+constexpr uint32_t kBig = 256, kSmall = 128;
+
+template <class T, int EPI>
+int launch(GemmArgs<T>& a, uint32_t m, uint32_t n, bool big, hipStream_t stream) {
+  const uint32_t t = big ? kBig : kSmall;
+  a.mt = static_cast<uint32_t>(ceil_div(m, t));
+  a.nt = static_cast<uint32_t>(ceil_div(n, t));
+  const uint64_t grid = static_cast<uint64_t>(a.mt) * a.nt * a.splits;
+  if (grid >= (1u << 22)) return efail("vocab_loss: too many tiles for one call");
+  if (big)
+    k_gemm<T, EPI, 256, 256, 2, 4><<<static_cast<unsigned>(grid), 512, 0, stream>>>(a);
+  else
+    k_gemm<T, EPI, 128, 128, 2, 2><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a);
+  return elaunch("omr_vocab_loss");
+}
+
+// Big tiles do twice the work for each byte that goes through LDS, small ones fill the CUs with less: big from one tile a
+// CU on.
+bool use_big(uint64_t m, uint64_t n) { return ceil_div(m, kBig) * ceil_div(n, kBig) >= 256; }
+
+// The piece of the vocabulary whose G is held at a time: about 256 MiB of it (what the last-level cache holds), at least
+// 1024 rows, in equal pieces of whole tiles.
+constexpr uint64_t kPieceBytes = 256ull << 20;
+uint32_t piece_rows(uint64_t tokens, uint64_t vocab) {
+  const uint64_t most = std::max<uint64_t>(1024, kPieceBytes / (2 * std::max<uint64_t>(1, tokens)) / 256 * 256);
+  const uint64_t pieces = ceil_div(vocab, most);
+  return static_cast<uint32_t>(up(ceil_div(vocab, pieces), 256));
+}
+uint64_t piece_bytes_most(uint64_t tokens, uint64_t vocab) {
+  return std::min(std::max(kPieceBytes, tokens * 1024 * 2), tokens * up(vocab, 256) * 2);
+}
+
+// Parts of grad_hidden's inner dimension (the vocabulary piece): enough to fill the CUs where its tiles do not, of no less
+// than 512 rows.
+uint32_t hidden_splits(uint64_t tokens, uint64_t dim, uint32_t piece) {
+  if (use_big(dim, tokens)) return 1;
+  const uint64_t tiles = ceil_div(dim, kSmall) * ceil_div(tokens, kSmall);
+  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(512 / std::min<uint64_t>(tiles, 512), piece / 512)));
+}
+uint64_t acc_bytes_most(uint64_t tokens, uint64_t dim) {
+  // splits * tokens * dim * 4 with splits <= 512 / tiles and tokens * dim <= tiles * 128^2
+  return std::max<uint64_t>(tokens * dim * 4, 512ull * kSmall * kSmall * 4);
+}
+
+struct Space {
+  uint64_t w, h, rest, bytes;  // packed weight, packed hidden states, then the pass's own
+};
+Space layout(uint64_t tokens, uint64_t vocab, uint64_t dim, bool pack, bool grads) {
+  Space s;
+  const uint64_t pdim = up(dim, 8);
+  s.w = 0;
+  s.h = s.w + (pack ? up(vocab * pdim * 2, 256) : 0);
+  s.rest = s.h + (pack ? up(tokens * pdim * 2, 256) : 0);
+  uint64_t fwd = up(tokens * 4, 256) + tokens * ceil_div(vocab, 64) * 8 + tokens * 32;
+  uint64_t bwd = 256 + up(tokens * 4, 256) + up(tokens * pdim * 2, 256) + up(piece_bytes_most(tokens, vocab), 256) +
+                 acc_bytes_most(tokens, dim);
+  s.bytes = s.rest + (grads ? std::max(fwd, bwd) : fwd) + 256;
+  return s;
+}
+
+bool rows_ok(const void* p, uint64_t stride) { return aligned(p, 16) && stride % 8 == 0 && stride < kMaxStride; }
+
+int check(const char* what, int dtype, uint64_t tokens, uint64_t vocab, uint32_t dim) {
+  if (dtype != OMR_BF16 && dtype != OMR_F16) return efail("%s: hidden and weight are bf16 or fp16", what);
+  if (dim == 0 || dim > (1u << 20)) return efail("%s: dim must be 1..%u", what, 1u << 20);
+  if (vocab == 0 || vocab >= (1ull << 31) - 256) return efail("%s: vocab must be 1..2^31 - 257", what);
+  if (tokens >= (1ull << 31) - 256) return efail("%s: tokens must be below 2^31 - 256", what);
+  return 0;
+}
+
+template <class T>
+int pack_rows(const void* src, uint64_t stride, uint64_t rows, uint32_t dim, const float* rowscale, const float* amax,
+              T* dst, hipStream_t stream) {
+  const uint32_t pdim = static_cast<uint32_t>(up(dim, 8));
+  const uint64_t blocks = ceil_div(rows * (pdim / 8), 256);
+  if (blocks >= (1u << 24)) return efail("vocab_loss: too many elements to lay out in one call");
+  const int wide = dim % 8 == 0 && stride % 8 == 0 && aligned(src, 16);
+  k_pack<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T*>(src), stride,
+                                                               static_cast<uint32_t>(rows), dim, pdim, rowscale, amax,
+                                                               dst, wide);
+  return elaunch("omr_vocab_loss (layout)");
+}
+
+// hidden and weight as row operands of whole 16-byte pieces: the caller's, or copies in the workspace
+template <class T>
+int operands(const void* hidden, uint64_t hstride, const void* weight, uint64_t wstride, uint64_t tokens, uint64_t vocab,
+             uint32_t dim, const Space& sp, char* ws, Operand<T>* h, Operand<T>* w, hipStream_t stream) {
+  const uint32_t pdim = static_cast<uint32_t>(up(dim, 8));
+  *h = {static_cast<const T*>(hidden), hstride, static_cast<uint32_t>(tokens)};
+  *w = {static_cast<const T*>(weight), wstride, static_cast<uint32_t>(vocab)};
+  if (dim % 8 != 0 || !rows_ok(weight, wstride)) {
+    T* to = reinterpret_cast<T*>(ws + sp.w);
+    if (const int rc = pack_rows<T>(weight, wstride, vocab, dim, nullptr, nullptr, to, stream)) return rc;
+    w->p = to;
+    w->ld = pdim;
+  }
+  if (dim % 8 != 0 || !rows_ok(hidden, hstride)) {
+    T* to = reinterpret_cast<T*>(ws + sp.h);
+    if (const int rc = pack_rows<T>(hidden, hstride, tokens, dim, nullptr, nullptr, to, stream)) return rc;
+    h->p = to;
+    h->ld = pdim;
+  }
+  return 0;
+}
+
+int check_space(const char* what, const void* hidden, uint64_t hstride, const void* weight, uint64_t wstride,
+                uint64_t tokens, uint64_t vocab, uint32_t dim, bool grads, const void* workspace, size_t bytes,
+                Space* sp) {
+  const bool pack = dim % 8 != 0 || !rows_ok(hidden, hstride) || !rows_ok(weight, wstride);
+  *sp = layout(tokens, vocab, dim, pack, grads);
+  if (workspace == nullptr || !aligned(workspace, 16)) return efail("%s: the workspace must be 16-byte aligned", what);
+  if (bytes < sp->bytes)
+    return efail("%s: workspace of %zu bytes, %llu needed%s", what, bytes, static_cast<unsigned long long>(sp->bytes),
+                 pack ? " (rows that are not whole 16-byte pieces are laid out again: ask for it with pack)" : "");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t omr_vocab_loss_workspace_bytes(uint64_t max_tokens, uint64_t vocab, uint32_t dim, int pack, int grads) {
+  return layout(max_tokens, vocab, dim, pack || dim % 8 != 0, grads).bytes;
+}
+
+int omr_vocab_loss(const void* hidden, uint64_t hidden_stride, const void* weight, uint64_t weight_stride, int dtype,
+                   uint64_t tokens, uint64_t vocab, uint32_t dim, const void* targets, int targets64, float* loss,
+                   float* lse, void* workspace, size_t workspace_bytes, omr_stream_t stream) {
+  if (const int rc = check("vocab_loss", dtype, tokens, vocab, dim)) return rc;
+  if (tokens == 0) return 0;
+  if (hidden == nullptr || weight == nullptr || targets == nullptr || loss == nullptr || lse == nullptr)
+    return efail("vocab_loss: NULL pointer");
+  Space sp;
+  if (const int rc = check_space("vocab_loss", hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, false,
+                                 workspace, workspace_bytes, &sp))
+    return rc;
+  char* ws = static_cast<char*>(workspace);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    GemmArgs<T> a{};
+    if (const int rc = operands<T>(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, sp, ws, &a.b, &a.a,
+                                   S(stream)))
+      return rc;
+    const bool big = use_big(vocab, tokens);
+    a.k = dim;
+    a.splits = 1;
+    a.ksplit = dim;
+    a.targets = targets;
+    a.targets64 = targets64;
+    a.vocab = static_cast<uint32_t>(vocab);
+    a.tokens = static_cast<uint32_t>(tokens);
+    a.ztarget = reinterpret_cast<float*>(ws + sp.rest);
+    a.stats = reinterpret_cast<float*>(ws + sp.rest + up(tokens * 4, 256));
+    a.pieces = static_cast<uint32_t>(big ? ceil_div(vocab, 256) * 2 : ceil_div(vocab, 128) * 2);
+    if (const int rc = launch<T, kStats>(a, a.vocab, a.tokens, big, S(stream))) return rc;
+    k_merge<T><<<static_cast<unsigned>(ceil_div(tokens, 4)), 256, 0, S(stream)>>>(a, loss, lse);
+    return elaunch("omr_vocab_loss");
+  };
+  return dtype == OMR_BF16 ? go(__bf16{}) : go(_Float16{});
+}
+
+int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* weight, uint64_t weight_stride,
+                        int dtype, uint64_t tokens, uint64_t vocab, uint32_t dim, const void* targets, int targets64,
+                        const float* lse, const float* grad_loss, uint64_t grad_loss_stride, void* grad_hidden,
+                        uint64_t grad_hidden_stride, void* grad_weight, int grad_weight_dtype,
+                        uint64_t grad_weight_stride, int accumulate, void* workspace, size_t workspace_bytes,
+                        omr_stream_t stream) {
+  if (const int rc = check("vocab_loss_grad", dtype, tokens, vocab, dim)) return rc;
+  if (grad_weight != nullptr && grad_weight_dtype != OMR_F32 && grad_weight_dtype != dtype)
+    return efail("vocab_loss_grad: grad_weight is fp32 or of the weight's type");
+  if ((grad_hidden != nullptr && grad_hidden_stride < dim) || (grad_weight != nullptr && grad_weight_stride < dim))
+    return efail("vocab_loss_grad: an output's row stride is shorter than dim %u", dim);
+  if (tokens != 0 && (hidden == nullptr || weight == nullptr || targets == nullptr || lse == nullptr ||
+                      grad_loss == nullptr))
+    return efail("vocab_loss_grad: NULL pointer");
+  if (tokens == 0) {  // a sum over no tokens
+    if (grad_weight == nullptr || accumulate) return 0;
+    const uint64_t blocks = ceil_div(vocab * dim, 256);
+    if (blocks >= (1u << 24)) return efail("vocab_loss_grad: the weight is too large for one call");
+    if (grad_weight_dtype == OMR_F32)
+      k_zero<float><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(static_cast<float*>(grad_weight), vocab, dim,
+                                                                          grad_weight_stride);
+    else  // (a zero has the same bits in both 16-bit types)
+      k_zero<__bf16><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(static_cast<__bf16*>(grad_weight), vocab, dim,
+                                                                           grad_weight_stride);
+    return elaunch("omr_vocab_loss_grad");
+  }
+  Space sp;
+  if (const int rc = check_space("vocab_loss_grad", hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim,
+                                 true, workspace, workspace_bytes, &sp))
+    return rc;
+  char* ws = static_cast<char*>(workspace);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    const uint32_t pdim = static_cast<uint32_t>(up(dim, 8));
+    Operand<T> h, w;
+    if (const int rc = operands<T>(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, sp, ws, &h, &w,
+                                   S(stream)))
+      return rc;
+    uint64_t at = sp.rest;
+    auto take = [&](uint64_t bytes) {
+      char* p = ws + at;
+      at += up(bytes, 256);
+      return p;
+    };
+    float* amax = reinterpret_cast<float*>(take(4));
+    float* rowscale = reinterpret_cast<float*>(take(tokens * 4));
+    T* clean = reinterpret_cast<T*>(take(tokens * pdim * 2));
+    T* g = reinterpret_cast<T*>(take(piece_bytes_most(tokens, vocab)));
+    float* acc = reinterpret_cast<float*>(take(acc_bytes_most(tokens, dim)));
+    GemmArgs<T> a{};
+    a.targets = targets;
+    a.targets64 = targets64;
+    a.vocab = static_cast<uint32_t>(vocab);
+    a.tokens = static_cast<uint32_t>(tokens);
+    a.dim = dim;
+    k_scales<T><<<1, 1024, 0, S(stream)>>>(a, grad_loss, grad_loss_stride, amax, rowscale);
+    if (const int rc = elaunch("omr_vocab_loss_grad (scales)")) return rc;
+    if (grad_weight != nullptr)
+      if (const int rc = pack_rows<T>(hidden, hidden_stride, tokens, dim, rowscale, amax, clean, S(stream))) return rc;
+    const uint32_t piece = piece_rows(tokens, vocab);
+    a.lse = lse;
+    a.g = g;
+    a.ldg = piece;
+    a.acc = acc;
+    a.rowscale = rowscale;
+    a.amax = amax;
+    const uint32_t whole = static_cast<uint32_t>(std::min<uint64_t>(piece, vocab));
+    const uint32_t ksplit = static_cast<uint32_t>(up(ceil_div(whole, hidden_splits(tokens, dim, piece)), kBK));
+    const uint32_t splits = static_cast<uint32_t>(ceil_div(whole, ksplit));  // of a whole piece; the last may have fewer
+    for (uint64_t v0 = 0; v0 < vocab; v0 += piece) {
+      const uint32_t rows = static_cast<uint32_t>(std::min<uint64_t>(piece, vocab - v0));
+      const uint32_t cols = static_cast<uint32_t>(up(rows, 256));  // columns of G that are written (zeros behind rows)
+      a.v0 = static_cast<uint32_t>(v0);
+      GemmArgs<T> z = a;
+      z.a = {w.p + v0 * w.ld, w.ld, rows};
+      z.b = h;
+      z.k = dim;
+      z.ksplit = dim;
+      z.splits = 1;
+      if (const int rc = launch<T, kGrad>(z, cols, z.tokens, use_big(cols, tokens), S(stream))) return rc;
+      if (grad_hidden != nullptr) {
+        GemmArgs<T> x = a;
+        x.a = {w.p + v0 * w.ld, w.ld, pdim};
+        x.b = {g, piece, x.tokens};
+        x.k = rows;
+        x.ksplit = ksplit;
+        x.splits = static_cast<uint32_t>(ceil_div(rows, ksplit));
+        x.first = v0 == 0;
+        const bool done = v0 + piece >= vocab;
+        x.last = done && splits == 1;
+        x.out = grad_hidden;
+        x.ostride = grad_hidden_stride;
+        x.wide = grad_hidden_stride % 4 == 0 && aligned(grad_hidden, 8);
+        if (const int rc = launch<T, kHidden>(x, dim, x.tokens, use_big(dim, tokens), S(stream))) return rc;
+        if (done && splits > 1) {
+          x.splits = splits;
+          const uint64_t blocks = ceil_div(tokens * dim, 256);
+          k_join<T><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(x);
+          if (const int rc = elaunch("omr_vocab_loss_grad (join)")) return rc;
+        }
+      }
+      if (grad_weight != nullptr) {
+        GemmArgs<T> y = a;
+        y.a = {clean, pdim, pdim};
+        y.b = {g, piece, cols};
+        y.k = y.tokens;
+        y.ksplit = y.tokens;
+        y.splits = 1;
+        y.out = grad_weight;
+        y.ostride = grad_weight_stride;
+        y.out_f32 = grad_weight_dtype == OMR_F32;
+        y.accumulate = accumulate != 0;
+        y.wide = grad_weight_stride % 4 == 0 && aligned(grad_weight, y.out_f32 ? 16 : 8);
+        if (const int rc = launch<T, kWeight>(y, dim, cols, use_big(dim, cols), S(stream))) return rc;
+      }
+    }
+    return 0;
+  };
+  return dtype == OMR_BF16 ? go(__bf16{}) : go(_Float16{});
+}
+
+}  // extern "C"

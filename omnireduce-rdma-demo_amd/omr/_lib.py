@@ -105,6 +105,11 @@ SIGNATURES = {
     "omr_layer_norm_grad_workspace_bytes": (c_size, [c_u64, c_u32]),
     "omr_layer_norm_grad": (c_int, [c_vp, c_u64, c_vp, c_int, c_u64, c_u32, c_u64, c_vp, c_vp, c_vp, c_int, c_vp,
                                     c_u64, c_vp, c_vp, c_int, c_vp, c_size, c_vp]),
+    "omr_vocab_loss_workspace_bytes": (c_size, [c_u64, c_u64, c_u32, c_int, c_int]),
+    "omr_vocab_loss": (c_int, [c_vp, c_u64, c_vp, c_u64, c_int, c_u64, c_u64, c_u32, c_vp, c_int, c_vp, c_vp, c_vp,
+                               c_size, c_vp]),
+    "omr_vocab_loss_grad": (c_int, [c_vp, c_u64, c_vp, c_u64, c_int, c_u64, c_u64, c_u32, c_vp, c_int, c_vp, c_vp,
+                                    c_u64, c_vp, c_u64, c_vp, c_int, c_u64, c_int, c_vp, c_size, c_vp]),
     "omr_host_last_error": (ctypes.c_char_p, []),
     "omr_host_register": (c_int, [c_vp, c_size]),
     "omr_host_unregister": (c_int, [c_vp]),

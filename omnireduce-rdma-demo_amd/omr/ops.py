@@ -518,6 +518,90 @@ class LayerNormGradPlan:
         return LayerNormGrads(grad_x, grad_weight, grad_bias)
 
 
+class VocabLossPlan:
+    """Softmax cross entropy of hidden [tokens, dim] against the output layer's weight [vocab, dim] (bf16 or fp16),
+    forward and backward, without keeping the logits, for at most max_tokens tokens a call.
+
+    pack: room to lay rows out again that are not whole 16-byte pieces (implied by a dim that is no multiple of 8).
+    grads=False: forward only."""
+
+    def __init__(self, max_tokens: int, vocab: int, dim: int, dtype: torch.dtype = torch.bfloat16, device="cuda",
+                 grads: bool = True, pack: bool = False):
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"dtype: bfloat16 or float16, got {dtype}")
+        if min(max_tokens, vocab, dim) < 0 or vocab == 0 or dim == 0:
+            raise ValueError(f"no such sizes: {max_tokens} tokens, vocab {vocab}, dim {dim}")
+        self.max_tokens, self.vocab, self.dim, self.dtype, self.grads = max_tokens, vocab, dim, dtype, grads
+        self.workspace = _Workspace(_lib.load().omr_vocab_loss_workspace_bytes(max_tokens, vocab, dim, int(pack),
+                                                                               int(grads)), device)
+
+    def _inputs(self, call: _Call, hidden, weight, targets):
+        hp, n, _, hstride = call.rows(hidden, "hidden", self.dim, None, self.dtype)
+        wp, _, _, wstride = call.rows(weight, "weight", self.dim, self.vocab, self.dtype)
+        tp, t64, nt = call.ids(targets, "targets")
+        if nt != n:
+            raise ValueError(f"targets: {n} expected, got shape {tuple(targets.shape)}")
+        if n > self.max_tokens:
+            raise ValueError(f"{n} tokens, the plan is for {self.max_tokens}")
+        return (hp, hstride, wp, wstride, _DTYPES[self.dtype], n, self.vocab, self.dim, tp, t64), n
+
+    def forward(self, hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                loss: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, stream=None):
+        """(loss, lse), fp32, one a token: loss = lse - logit of the target; 0 where the target names no row."""
+        with _Call(hidden.device, stream) as call:
+            args, n = self._inputs(call, hidden, weight, targets)
+            if loss is None:
+                loss = call.empty(targets.shape, torch.float32)
+            if lse is None:
+                lse = call.empty(targets.shape, torch.float32)
+            _lib.check(_lib.load().omr_vocab_loss(*args, call.vector(loss, "loss", n), call.vector(lse, "lse", n),
+                                                  self.workspace.lend(call), self.workspace.bytes, call.ptr),
+                       "omr_vocab_loss")
+        return loss, lse
+
+    def backward(self, hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
+                 grad_loss: torch.Tensor, grad_hidden: Optional[torch.Tensor] = None,
+                 grad_weight: Optional[torch.Tensor] = None, accumulate: bool = False, need_hidden: bool = True,
+                 need_weight: bool = True, stream=None):
+        """(grad_hidden, grad_weight) for grad_loss (fp32, one a token, or one for all).  grad_weight is fp32 or of the
+        weight's type (default), written or added to (accumulate); need_hidden / need_weight=False leave one out."""
+        if not self.grads:
+            raise ValueError("the plan was made with grads=False")
+        with _Call(hidden.device, stream) as call:
+            args, n = self._inputs(call, hidden, weight, targets)
+            if grad_loss.dtype != torch.float32 or grad_loss.numel() not in (n, 1):
+                raise ValueError(f"grad_loss: fp32, {n} or one, got {grad_loss.dtype}{tuple(grad_loss.shape)}")
+            if grad_loss.numel() == 1 or all(s == 0 for s in grad_loss.stride()):
+                gstride = 0  # (also the gradient of a sum: one value, expanded)
+            elif grad_loss.is_contiguous():
+                gstride = 1
+            else:
+                raise ValueError(f"grad_loss must be contiguous or one value (stride {grad_loss.stride()})")
+            hp = wp = None
+            hstride = wstride = self.dim
+            if need_hidden:
+                if grad_hidden is None:
+                    grad_hidden = call.empty(hidden.shape, self.dtype)
+                hp, _, _, hstride = call.rows(grad_hidden, "grad_hidden", self.dim, n, self.dtype, out=True)
+            elif grad_hidden is not None:
+                raise ValueError("need_hidden=False takes no grad_hidden")
+            if need_weight:
+                if grad_weight is None:
+                    if accumulate:
+                        raise ValueError("accumulate needs a grad_weight")
+                    grad_weight = call.empty(weight.shape, self.dtype)
+                if grad_weight.dtype not in (torch.float32, self.dtype):
+                    raise ValueError(f"grad_weight: fp32 or {self.dtype}, got {grad_weight.dtype}")
+                wp, _, _, wstride = call.rows(grad_weight, "grad_weight", self.dim, self.vocab, out=True)
+            elif grad_weight is not None or accumulate:
+                raise ValueError("need_weight=False takes no grad_weight")
+            _lib.check(_lib.load().omr_vocab_loss_grad(
+                *args, call.vector(lse, "lse", n), call.on(grad_loss, "grad_loss"), gstride, hp, hstride, wp,
+                _DTYPES[grad_weight.dtype] if wp is not None else 0, wstride, int(accumulate),
+                self.workspace.lend(call), self.workspace.bytes, call.ptr), "omr_vocab_loss_grad")
+        return grad_hidden, grad_weight
+
+
 # ------------------------------------------------------------------ host-resident end-to-end path
 
 class HostPlan:

@@ -343,6 +343,167 @@ def test_layer_norm_no_rows_and_shapes(gpu):
     assert not torch.isfinite(out[1]).any() and torch.isfinite(out[[0, 2]]).all()
 
 
+# ---------------------------------------------------------------------------------------------------- vocabulary loss
+
+def loss_inputs(T, V, D, dtype, g, none=0.1):
+    """Hidden states that lean towards their target's row; tokens without a target hold NaN."""
+    w = rand((V, D), dtype, g, std=D ** -0.5)
+    t = torch.randint(0, V, (T,), generator=g, device="cuda")
+    h = (rand((T, D), F32, g) + 4 * torch.rand(T, 1, generator=g, device="cuda") * w[t].float()).to(dtype)
+    off = torch.rand(T, generator=g, device="cuda") < none
+    t[off] = torch.where(torch.rand(T, generator=g, device="cuda") < 0.5, -100, V)[off]
+    return h, w, t, off
+
+
+def loss_ref(h, w, t, off):
+    """Logits, lse and loss in 64 bits, with the bounds: a logit's dim products are exact in fp32 and their sum is off by
+    dim u of their magnitudes (e); the exponentials' arguments by that and u, __expf by 2 u (|argument| + 2), so the sum
+    by e + (100 + vocab depth) u, and as much the lse."""
+    z = h.double() @ w.double().t()
+    e = (h.double().abs() @ w.double().abs().t()).amax(1) * h.shape[1] * U
+    lse = torch.logsumexp(z, 1)
+    zt = z.gather(1, t.clamp(0, w.shape[0] - 1).long()[:, None])[:, 0]
+    loss = torch.where(off, 0.0, lse - zt)
+    spread = (z.amax(1) - lse).abs() + 40  # arguments below -40 do not count at this precision
+    tol = e + (2 * spread + 600) * U + 2 * U * lse.abs()
+    return z, lse, loss, tol
+
+
+LOSS_SIZES = [(1, 1, 8), (1, 7, 1), (3, 300, 72), (17, 129, 264), (64, 1000, 128), (130, 257, 61), (257, 2000, 200),
+              (300, 5003, 520), (1025, 700, 96), (16, 40000, 64), (700, 70000, 64), (2048, 8192, 256), (5, 256, 4096)]
+
+
+@pytest.mark.parametrize("T,V,D", LOSS_SIZES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_vocab_loss(gpu, T, V, D, dtype):
+    g = gen(T + V + D)
+    h, w, t, off = loss_inputs(T, V, D, dtype, g)
+    plan = ops.VocabLossPlan(T + 5, V, D, dtype=dtype)
+    fwd = ops.VocabLossPlan(T, V, D, dtype=dtype, grads=False)
+    z, lse, loss, tol = loss_ref(h, w, t, off)
+    for p, it in ((plan, torch.int64), (fwd, torch.int32)):
+        got, got_lse = p.forward(h, w, t.to(it))
+        within(got_lse, lse, tol, "lse")
+        within(got, loss, torch.where(off, 0.0, 2 * tol + U * loss.abs()), "loss")
+
+    # the gradient of sum(up * loss), with tokens of no target holding NaN everywhere
+    for up in (torch.full((T,), 1.0 / max(1, T), device="cuda"), rand((T,), F32, g)):
+        hn, upn = h.clone(), up.clone()
+        hn[off], upn[off] = NAN, NAN
+        _, l32 = plan.forward(h, w, t)
+        ll = l32.clone()
+        ll[off] = NAN
+        G = torch.exp(z - l32.double()[:, None])
+        G[torch.arange(T, device="cuda")[~off], t[~off]] -= 1
+        G[off] = 0
+        upd = torch.where(off, 0.0, up.double())
+        gh_ref = upd[:, None] * (G @ w.double())
+        gw_ref = (G * upd[:, None]).t() @ torch.where(off[:, None], 0.0, h.double())
+        # G: a logit is off by e, the exponential by 2 u (|argument| + 2), then rounded to the type (its magnitude, and
+        # fp16's underflow at 2^-25 / 2^12); hidden times its share of the largest factor rounds once more; sums of V
+        # (T) terms in fp32
+        e = ((h.double().abs() @ w.double().abs().t()).amax(1) * D * U)[:, None] + 100 * U
+        P = torch.exp(z - l32.double()[:, None])
+        dG = torch.where(off[:, None], 0.0, P * 2 * e + G.abs() * half(dtype) + 2.0 ** -36)
+        tol_h = upd.abs()[:, None] * (dG @ w.double().abs() + (V + 4) * U * (G.abs() @ w.double().abs()))
+        hm = torch.where(off[:, None], 0.0, h.double().abs())
+        wt = (upd.abs()[:, None] * (dG + G.abs() * ((T + 4) * U + half(dtype)))).t() @ hm
+        wt = wt + T * tiny(dtype) * upd.abs().max()
+        gh, gw = plan.backward(hn, w, t, ll, upn)
+        within(gh, gh_ref, tol_h * (1 + half(dtype)) + half(dtype) * gh_ref.abs() + tiny(dtype), "grad_hidden")
+        within(gw, gw_ref, wt * (1 + half(dtype)) + half(dtype) * gw_ref.abs() + tiny(dtype), "grad_weight")
+        assert not gh[off].any()
+        base = rand((V, D), F32, g)
+        acc = base.clone()
+        none, gw32 = plan.backward(hn, w, t, ll, upn, grad_weight=acc, accumulate=True, need_hidden=False)
+        assert none is None and gw32 is acc
+        within(acc, gw_ref + base.double(), wt + 2 * U * (gw_ref.abs() + base.double().abs()), "accumulated")
+        gh2, none = plan.backward(hn, w, t, ll, upn, need_weight=False)
+        assert none is None and torch.equal(gh2, gh)
+        again = plan.backward(hn, w, t, ll, upn)
+        assert torch.equal(again[0], gh) and torch.equal(again[1], gw)  # the same bits
+
+
+def test_vocab_loss_no_targets_no_tokens_and_one_factor(gpu):
+    g = gen(1)
+    h, w, t, off = loss_inputs(40, 500, 64, BF16, g, none=0.0)
+    plan = ops.VocabLossPlan(40, 500, 64)
+    nothing = torch.full_like(t, -1)
+    loss, lse = plan.forward(h, w, nothing)
+    assert not loss.any() and torch.isfinite(lse).all()
+    gh, gw = plan.backward(h, w, nothing, lse, torch.ones(40, device="cuda"))
+    assert not gh.any() and not gw.any()
+    keep = torch.ones(500, 64, device="cuda")
+    plan.backward(h, w, nothing, lse, torch.ones(40, device="cuda"), grad_weight=keep, accumulate=True)
+    assert (keep == 1).all()
+    empty = plan.forward(h[:0], w, t[:0])
+    assert empty[0].shape == (0,)
+    for dt in (BF16, F32):
+        out = torch.full((500, 64), NAN, dtype=dt, device="cuda")
+        plan.backward(h[:0], w, t[:0], empty[1], torch.empty(0, device="cuda"), grad_weight=out)
+        assert not out.any()
+    loss, lse = plan.forward(h, w, t)
+    one = torch.tensor(0.25, device="cuda")
+    a = plan.backward(h, w, t, lse, one)
+    b = plan.backward(h, w, t, lse, one.expand(40))
+    c = plan.backward(h, w, t, lse, torch.full((40,), 0.25, device="cuda"))
+    for x, y, q in zip(a, b, c):
+        assert torch.equal(x, y) and torch.equal(x, q)
+    zero = plan.backward(h, w, t, lse, torch.zeros(40, device="cuda"))
+    assert not zero[0].any() and not zero[1].any()
+
+
+@pytest.mark.parametrize("D,pad,offset", [(64, 8, 0), (64, 3, 0), (64, 8, 1), (61, 3, 5)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_vocab_loss_strides_and_untouched_memory(gpu, D, pad, offset, dtype):
+    """Rows apart, unaligned and ragged: the same bits as the packed tensors' (the products see the same tiles)."""
+    g = gen(6)
+    T, V = 150, 400
+    h0, w0, t, off = loss_inputs(T, V, D, dtype, g)
+    up = rand((T,), F32, g)
+    h, _ = strided(h0, pad, offset)
+    w, _ = strided(w0, pad, offset)
+    plain, plan = ops.VocabLossPlan(T, V, D, dtype=dtype), ops.VocabLossPlan(T, V, D, dtype=dtype, pack=True)
+    want = [*plain.forward(h0, w0, t)]
+    want += plain.backward(h0, w0, t, want[1], up)
+    gh, hbuf = strided(torch.zeros_like(h0), pad, offset)
+    gw, wbuf = strided(torch.zeros_like(w0), pad, offset)
+    before = hbuf.clone(), wbuf.clone()
+    got = [*plan.forward(h, w, t)]
+    got += plan.backward(h, w, t, got[1], up, grad_hidden=gh, grad_weight=gw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    gh.fill_(0)
+    gw.fill_(0)
+    assert torch.equal(hbuf, before[0]) and torch.equal(wbuf, before[1])
+    if (D + pad) % 8 or offset:
+        if D % 8 == 0:
+            with pytest.raises(ops._lib.OmrError, match="pack"):  # (too little room for that without asking)
+                ops.VocabLossPlan(T, V, D, dtype=dtype, grads=False).forward(h, w, t)
+
+
+def test_vocab_loss_pieces(gpu, dtype=BF16):
+    """More logits than one piece holds (tokens x vocabulary x 2 bytes over 256 MiB): three pieces, the last ragged."""
+    g = gen(12)
+    T, V, D = 4100, 70001, 32
+    h, w, t, off = loss_inputs(T, V, D, dtype, g)
+    plan = ops.VocabLossPlan(T, V, D)
+    loss, lse = plan.forward(h, w, t)
+    up = rand((T,), F32, g)
+    gh, gw = plan.backward(h, w, t, lse, up, grad_weight=torch.empty(V, D, device="cuda"))
+    z = (h.float() @ w.float().t()).double()
+    G = torch.exp(z - lse.double()[:, None])
+    ok = ~off
+    G[torch.arange(T, device="cuda")[ok], t[ok]] -= 1
+    G[off] = 0
+    upd = torch.where(off, 0.0, up.double())
+    gh_ref, gw_ref = upd[:, None] * (G @ w.double()), (G * upd[:, None]).t() @ h.double()
+    aG = G.abs()
+    th = upd.abs()[:, None] * (aG @ w.double().abs()) * (half(dtype) * 1.1 + (V + 4) * U) + 1e-6
+    tw = ((aG * upd.abs()[:, None]).t() @ h.double().abs()) * (2 * half(dtype) * 1.1 + (T + 4) * U) + 1e-6
+    within(gh, gh_ref, th + half(dtype) * gh_ref.abs(), "grad_hidden")
+    within(gw, gw_ref, tw, "grad_weight")
+
+
 # ---------------------------------------------------------------------------------------------------- streams, graphs
 
 def test_operators_in_a_graph_and_on_streams(gpu):
