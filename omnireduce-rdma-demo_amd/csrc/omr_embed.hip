@@ -69,36 +69,54 @@ __global__ __launch_bounds__(256) void k_embed(const T* table, uint32_t rows, ui
 // Groups the tokens by row in ONE launch without any exchange between workgroups: workgroup p owns the rows
 // [p R, p R + R) and reads ALL ids itself (they sit in the L2s: 64 KiB for 8192 int64 ids), counting its own and how
 // many are below its range, which is where its piece of the sorted list begins.
-//   pass 1  wave w counts the ids of its contiguous sixteenth of the tokens in hist[w][id - lo]
+//   pass 1  wave w counts the ids of its contiguous sixteenth of the tokens in hist[w][id - lo], and notes the tokens it
+//           counted, in order, in a list of its own
 //   scan    start[v] = ids below v; hist[w][.] = where wave w's first token of that row goes
-//   pass 2  the waves walk their tokens again and place them: within 64 tokens the lanes of equal ids rank themselves
-//           by lane (match by ballots over the bits of the local id), so the order within a row is token order
-// A radix sort by 8 bits took the launches of three passes (about nine); this is one, and its work, T ids per
-// workgroup, is hidden in the L2 up to some 100 k tokens.
+//   pass 2  the waves walk their lists (or, where a list is full, their tokens again) and place them: within 64 tokens
+//           the lanes of equal ids rank themselves by lane (match by ballots over the bits of the local id), so the
+//           order within a row is token order
+// Every workgroup reads T ids: hidden in the L2 up to some 100 k tokens, where a radix sort would take three launches
+// for each of three digits.
 constexpr int kSortWaves = 16;
-constexpr int kSortRange = 1024;      // rows per workgroup at most: 64 KiB of histogram, two workgroups a CU
+constexpr int kSortRange = 1024;  // rows per workgroup at most: 64 KiB of histogram
 constexpr int kSortBits = 10;
+constexpr uint32_t kSortList = 512;  // tokens a wave notes: 32 KiB
 
 template <class I>
 __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, uint32_t tokens, uint32_t rows,
                                                                uint32_t range, uint32_t* start, uint32_t* perm) {
   __shared__ uint32_t hist[kSortWaves * kSortRange];
+  __shared__ uint32_t list[kSortWaves][kSortList];  // (token - the wave's first) << 10 | local id
   __shared__ uint32_t wsum[kSortWaves], below_w[kSortWaves];
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t lo = blockIdx.x * range, n = min(range, rows - lo);
-  for (uint32_t i = tid; i < kSortWaves * kSortRange; i += 64 * kSortWaves) hist[i] = 0;
+  for (uint32_t i = tid; i < kSortWaves * range; i += 64 * kSortWaves) hist[i] = 0;
   const uint32_t span = (tokens + 64 * kSortWaves - 1) / (64 * kSortWaves) * 64;  // tokens of a wave
   const uint32_t t0 = min(wave * span, tokens), t1 = min(t0 + span, tokens);
-  uint32_t* mine = hist + wave * kSortRange;
-  uint32_t below = 0;
+  uint32_t* mine = hist + wave * range;
+  uint32_t below = 0, noted = 0;
   __syncthreads();
-#pragma unroll 4
-  for (uint32_t t = t0 + lane; t < t1; t += 64) {
-    const I id = ids[t];
-    if (id_ok(id, rows)) {
-      const uint32_t v = static_cast<uint32_t>(id);
+  constexpr int K = 8;  // loads in flight
+  for (uint32_t t = t0; t < t1; t += 64 * K) {
+    I id[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const uint32_t at = t + 64 * k + lane;
+      id[k] = at < t1 ? ids[at] : static_cast<I>(-1);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const uint32_t v = id_ok(id[k], rows) ? static_cast<uint32_t>(id[k]) : ~0u;
       below += v < lo;
-      if (v - lo < n) atomicAdd(&mine[v - lo], 1u);
+      const bool in = v - lo < n;
+      const uint64_t who = __ballot(in);
+      if (who == 0) continue;
+      const uint32_t at = noted + __popcll(who & ((1ull << lane) - 1));
+      if (in) {
+        atomicAdd(&mine[v - lo], 1u);
+        if (at < kSortList) list[wave][at] = (t + 64 * k + lane - t0) << kSortBits | (v - lo);
+      }
+      noted += static_cast<uint32_t>(__popcll(who));
     }
   }
 #pragma unroll
@@ -107,7 +125,10 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
   __syncthreads();
   // exclusive scan over the range's rows of their totals, then over the waves within a row
   uint32_t total = 0;
-  for (int w = 0; w < kSortWaves; ++w) total += hist[w * kSortRange + tid];
+  if (tid < n) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) total += hist[w * range + tid];
+  }
   uint32_t incl = total;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -117,23 +138,35 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
   if (lane == 63) wsum[wave] = incl;
   __syncthreads();
   uint32_t at = incl - total;
+#pragma unroll
   for (uint32_t w = 0; w < kSortWaves; ++w) {
     at += below_w[w];
     if (w < wave) at += wsum[w];
   }
-  if (tid < n) start[lo + tid] = at;
-  if (lo + n == rows && tid == n - 1) start[rows] = at + total;
-  for (int w = 0; w < kSortWaves; ++w) {
-    const uint32_t c = hist[w * kSortRange + tid];
-    hist[w * kSortRange + tid] = at;
-    at += c;
+  if (tid < n) {
+    start[lo + tid] = at;
+    if (lo + tid == rows - 1) start[rows] = at + total;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = hist[w * range + tid];
+      hist[w * range + tid] = at;
+      at += c;
+    }
   }
   __syncthreads();
-  for (uint32_t t = t0; t < t1; t += 64) {
-    uint32_t v = ~0u;
-    if (t + lane < t1) {
-      const I id = ids[t + lane];
-      if (id_ok(id, rows)) v = static_cast<uint32_t>(id) - lo;
+  // (a list holds token distances of 22 bits)
+  const bool listed = noted <= kSortList && span <= 1u << (32 - kSortBits);
+  const uint32_t steps = listed ? noted : t1 - t0;
+  for (uint32_t i = 0; i < steps; i += 64) {
+    uint32_t v = ~0u, t = t0 + i + lane;
+    if (i + lane < steps) {
+      if (listed) {
+        const uint32_t e = list[wave][i + lane];
+        v = e & (kSortRange - 1);
+        t = t0 + (e >> kSortBits);
+      } else if (id_ok(ids[t], rows)) {
+        v = static_cast<uint32_t>(ids[t]) - lo;
+      }
     }
     const bool in = v < n;
     uint64_t same = __ballot(in);
@@ -148,95 +181,38 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
     uint32_t base = 0;
     if (in && lane == leader) base = atomicAdd(&mine[v], static_cast<uint32_t>(__popcll(same)));
     base = __shfl(base, static_cast<int>(leader));
-    if (in) perm[base + __popcll(same & ((1ull << lane) - 1))] = t + lane;
+    if (in) perm[base + __popcll(same & ((1ull << lane) - 1))] = t;
   }
 }
 
 // ---------------------------------------------------------------- sums
 //
 // Bound by HBM: grad_out is read once and the table's gradient written once (65536 x 1024 fp32: 256 MiB), most of it
-// zeros.  k_embed_rows gives a group of lanes one row and lets it add the row's tokens up, or store zeros.  A row with
-// more than `chunk` tokens (a frequent word) would hold its wave for long, so such rows are summed in pieces: the
-// sorted list is cut into chunks, k_embed_partial adds up each chunk's tokens of such rows (at most two: one that began
-// earlier and one that goes on), and a workgroup of k_embed_rows's launch adds the row's pieces up in order.
+// zeros.  Two kinds of workgroups of one launch share the rows:
+//   - row workgroups: a group of lanes takes four consecutive rows and stores the sums of those of at most kFew tokens,
+//     most of them zeros;
+//   - chunk workgroups: the sorted list in chunks of 64 positions, one a lane; the chunk's rows of more than kFew tokens
+//     are added up there.  A row that lies within its chunk is done; of one that goes on (a frequent word) the chunk's
+//     piece goes to `partial`, and k_embed_join adds its pieces up in order, a launch later.
+// So no wave adds up more than 64 rows behind each other.  (Rows of up to 128 tokens in the row workgroups held the
+// launch for 122 us at 8192 tokens of 65536 x 1024, whose bytes take 55.)
+constexpr uint32_t kChunk = 64, kFew = 8;
+constexpr int kRows = 4;  // consecutive rows of a lane group
+static_assert(kFew <= 8, "a lane group, 8 lanes at least, holds the tokens of a row of few");
+
 struct SumArgs {
   const void* grad_out;
   uint64_t gstride;
   const void* ids;
   const uint32_t* start;  // [rows + 1]
   const uint32_t* perm;   // the valid tokens by row
-  float* partial;         // [2 * chunks][dim]
+  float* partial;         // [2 * chunks][dim]: the piece of the row that began before the chunk; of the one that goes on
   float* out;
   uint64_t ostride;
-  uint32_t rows, dim, chunk, chunks, tiles;  // tiles of columns
+  uint32_t rows, dim, chunks, tiles;  // tiles of columns of a chunk workgroup
   float scale;
   int accumulate;
 };
-
-template <class I>
-__device__ __forceinline__ uint32_t row_at(const SumArgs& a, uint32_t pos) {
-  return static_cast<uint32_t>(static_cast<const I*>(a.ids)[a.perm[pos]]);
-}
-
-// acc += the rows of grad_out of the sorted positions [p0, p1), in order, at columns c + j * step
-template <class T, int VEC, int NJ>
-__device__ __forceinline__ void add_tokens(const SumArgs& a, uint32_t p0, uint32_t p1, uint32_t c, uint32_t step,
-                                           float (&acc)[NJ][VEC]) {
-  const T* g = static_cast<const T*>(a.grad_out) + c;
-  constexpr int K = NJ >= 4 ? 2 : 8;  // tokens in flight
-  uint32_t p = p0;
-  for (; p + K <= p1; p += K) {
-    float v[K][NJ][VEC];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const T* r = g + static_cast<uint64_t>(a.perm[p + k]) * a.gstride;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        if (c + j * step < a.dim) load_f32<T, VEC>(r + j * step, v[k][j]);
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        if (c + j * step < a.dim)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[j][i] += v[k][j][i];
-  }
-  for (; p < p1; ++p) {
-    const T* r = g + static_cast<uint64_t>(a.perm[p]) * a.gstride;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      if (c + j * step < a.dim) {
-        float v[VEC];
-        load_f32<T, VEC>(r + j * step, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[j][i] += v[i];
-      }
-  }
-}
-
-// one wave: columns [wave tile), one chunk's piece(s)
-template <class T, class I, int VEC>
-__global__ __launch_bounds__(256) void k_embed_partial(SumArgs a) {
-  const uint32_t valid = a.start[a.rows];
-  const uint32_t k = blockIdx.x;
-  const uint32_t p0 = k * a.chunk, p1 = min(p0 + a.chunk, valid);
-  if (p0 >= p1) return;
-  const uint32_t c = (blockIdx.y * 256 + threadIdx.x) * VEC;
-  const uint32_t r0 = row_at<I>(a, p0), r1 = row_at<I>(a, p1 - 1);
-  const uint32_t s0 = a.start[r0], e0 = a.start[r0 + 1], s1 = a.start[r1], e1 = a.start[r1 + 1];
-  if (c >= a.dim) return;
-  if (e0 - s0 > a.chunk) {  // the row at the chunk's first position
-    float acc[1][VEC] = {};
-    add_tokens<T, VEC, 1>(a, p0, min(e0, p1), c, 0, acc);
-    store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k) * a.dim + c, acc[0]);
-  }
-  if (r1 != r0 && e1 - s1 > a.chunk) {  // the row that goes on behind it
-    float acc[1][VEC] = {};
-    add_tokens<T, VEC, 1>(a, s1, p1, c, 0, acc);
-    store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k + 1) * a.dim + c, acc[0]);
-  }
-}
 
 template <int VEC>
 __device__ __forceinline__ void put(const SumArgs& a, uint32_t row, uint32_t c, float (&v)[VEC]) {
@@ -252,77 +228,128 @@ __device__ __forceinline__ void put(const SumArgs& a, uint32_t row, uint32_t c, 
   store_f32<float, VEC>(o, v);
 }
 
-constexpr int kRowsNJ = 4;
-
-// blocks [0, chunks * tiles): the rows of many tokens; behind them: `lpr` lanes a row, every other row
-template <class T, class I, int VEC>
-__global__ __launch_bounds__(256) void k_embed_rows(SumArgs a, uint32_t join_blocks, uint32_t lpr_log) {
-  if (blockIdx.x < join_blocks) {
-    // The row that begins in chunk k and goes on behind it, columns of this tile; the four waves each take a quarter
-    // of its pieces (in order), and wave 0 adds the quarters up.
-    __shared__ float sums[4][64 * VEC];
-    const uint32_t valid = a.start[a.rows];
-    const uint32_t k = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
-    const uint32_t p0 = k * a.chunk, p1 = min(p0 + a.chunk, valid);
-    if (p0 >= p1) return;
-    const uint32_t row = row_at<I>(a, p1 - 1), s = a.start[row], e = a.start[row + 1];
-    if (e - s <= a.chunk || s < p0) return;
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const uint32_t c = (tile * 64 + lane) * VEC;
-    const uint32_t pieces = (e - 1) / a.chunk - k + 1, quarter = (pieces + 3) / 4;
-    const uint32_t q0 = min(wave * quarter, pieces), q1 = min(q0 + quarter, pieces);
-    float acc[VEC] = {};
-    if (c < a.dim) {
-      for (uint32_t q = q0; q < q1; q += 8) {  // eight pieces in flight, added in order
-        float v[8][VEC];
+// acc += rows of grad_out, in order, at columns c + j * step: the tokens that lanes [l0, l0 + n) of this lane's group of
+// `width` lanes hold
+template <class T, int VEC, int NJ, int K>
+__device__ __forceinline__ void add_tokens(const SumArgs& a, uint32_t held, uint32_t l0, uint32_t n, uint32_t width,
+                                           uint32_t c, uint32_t step, float (&acc)[NJ][VEC]) {
+  const T* g = static_cast<const T*>(a.grad_out) + c;
+  for (uint32_t p = 0; p < n; p += K) {
+    float v[K][NJ][VEC];
 #pragma unroll
-        for (uint32_t k8 = 0; k8 < 8; ++k8) {
-          const uint32_t at = q + k8;
-          const uint32_t slot = 2 * (k + at) + (at == 0 && s != p0 ? 1 : 0);
-          if (at < q1) load_f32<float, VEC>(a.partial + static_cast<uint64_t>(slot) * a.dim + c, v[k8]);
-        }
+    for (int k = 0; k < K; ++k) {
+      const uint32_t t = __shfl(held, static_cast<int>(l0 + (p + k < n ? p + k : n - 1)), static_cast<int>(width));
+      const T* r = g + static_cast<uint64_t>(t) * a.gstride;
 #pragma unroll
-        for (uint32_t k8 = 0; k8 < 8; ++k8)
-          if (q + k8 < q1)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] += v[k8][i];
-      }
+      for (int j = 0; j < NJ; ++j)
+        if (p + k < n && c + j * step < a.dim) load_f32<T, VEC>(r + j * step, v[k][j]);
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sums[wave][lane * VEC + i] = acc[i];
-    __syncthreads();
-    if (wave == 0 && c < a.dim) {
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int w = 1; w < 4; ++w)
+      for (int j = 0; j < NJ; ++j)
+        if (p + k < n && c + j * step < a.dim)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += sums[w][lane * VEC + i];
-      put<VEC>(a, row, c, acc);
+          for (int i = 0; i < VEC; ++i) acc[j][i] += v[k][j][i];
+  }
+}
+
+constexpr int kRowsNJ = 4;
+
+// blocks [0, chunks * tiles): chunks; behind them: rows, 2^lpr_log lanes a row
+template <class T, class I, int VEC>
+__global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blocks, uint32_t lpr_log) {
+  if (blockIdx.x < chunk_blocks) {
+    const uint32_t valid = a.start[a.rows];
+    const uint32_t k = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles, lane = threadIdx.x & 63;
+    const uint32_t p0 = k * kChunk, p1 = min(p0 + kChunk, valid);
+    if (p0 >= p1) return;
+    const uint32_t c = (tile * 256 + threadIdx.x) * VEC;
+    // each lane: the token at its position and that token's row; a row's first position here speaks for it
+    const uint32_t held = a.perm[min(p0 + lane, p1 - 1)];
+    const uint32_t row = static_cast<uint32_t>(static_cast<const I*>(a.ids)[held]);
+    const uint32_t s = a.start[row], e = a.start[row + 1];
+    uint64_t todo = __ballot(p0 + lane < p1 && e - s > kFew && p0 + lane == max(s, p0));
+    while (todo != 0) {
+      const int l = __ffsll(static_cast<unsigned long long>(todo)) - 1;
+      todo &= todo - 1;
+      const uint32_t r = __shfl(row, l), rs = __shfl(s, l), re = __shfl(e, l);
+      float acc[1][VEC] = {};
+      add_tokens<T, VEC, 1, 8>(a, held, l, min(re, p1) - (p0 + l), 64, c, 0, acc);
+      if (c < a.dim) {
+        if (rs >= p0 && re <= p1)
+          put<VEC>(a, r, c, acc[0]);
+        else
+          store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k + (rs >= p0 ? 1 : 0)) * a.dim + c, acc[0]);
+      }
     }
     return;
   }
-  const uint32_t lpr = 1u << lpr_log;
-  const uint64_t unit = (static_cast<uint64_t>(blockIdx.x - join_blocks) * 256 + threadIdx.x) >> lpr_log;
-  const uint32_t sub = threadIdx.x & (lpr - 1), step = lpr * VEC;
+  const uint32_t lpr = 1u << lpr_log, sub = threadIdx.x & (lpr - 1), step = lpr * VEC;
+  const uint64_t unit = (static_cast<uint64_t>(blockIdx.x - chunk_blocks) * 256 + threadIdx.x) >> lpr_log;
   const uint32_t tiles = (a.dim + step * kRowsNJ - 1) / (step * kRowsNJ);
-  const uint64_t row64 = unit / tiles;
-  if (row64 >= a.rows) return;
-  const uint32_t row = static_cast<uint32_t>(row64);
-  const uint32_t c = static_cast<uint32_t>(unit - row64 * tiles) * step * kRowsNJ + sub * VEC;
-  const uint32_t s = a.start[row], e = a.start[row + 1];
-  if (e - s > a.chunk || (a.accumulate && s == e)) return;
-  float acc[kRowsNJ][VEC] = {};
-  if (s != e) add_tokens<T, VEC, kRowsNJ>(a, s, e, c, step, acc);
+  const uint64_t four = unit / tiles;
+  const uint32_t c = static_cast<uint32_t>(unit - four * tiles) * step * kRowsNJ + sub * VEC;
+  uint32_t at[kRows + 1];
 #pragma unroll
-  for (int j = 0; j < kRowsNJ; ++j)
-    if (c + j * step < a.dim) put<VEC>(a, row, c + j * step, acc[j]);
+  for (int q = 0; q <= kRows; ++q) at[q] = a.start[min(four * kRows + q, static_cast<uint64_t>(a.rows))];
+#pragma unroll
+  for (int q = 0; q < kRows; ++q) {
+    const uint64_t row = four * kRows + q;
+    const uint32_t n = at[q + 1] - at[q];
+    if (row >= a.rows || n > kFew || (a.accumulate && n == 0)) continue;
+    float acc[kRowsNJ][VEC] = {};
+    if (n != 0) {
+      const uint32_t held = a.perm[at[q] + min(sub, n - 1)];
+      add_tokens<T, VEC, kRowsNJ, 4>(a, held, 0, n, lpr, c, step, acc);
+    }
+#pragma unroll
+    for (int j = 0; j < kRowsNJ; ++j)
+      if (c + j * step < a.dim) put<VEC>(a, static_cast<uint32_t>(row), c + j * step, acc[j]);
+  }
 }
 
-// Tokens of a chunk: a row of n tokens is added up by one wave until n > chunk, and by n / chunk pieces of chunk
-// tokens and then one chain of n / chunk pieces beyond, so the longest chain is about chunk + tokens / chunk.
-uint32_t chunk_tokens(uint64_t tokens) {
-  uint32_t c = 64;
-  while (c < 1024 && static_cast<uint64_t>(c) * c < tokens) c *= 2;
-  return c;
+// The row that begins in chunk k and goes on behind it, 64 VEC columns; the four waves each take a quarter of its pieces
+// (in order), and wave 0 adds the quarters up.
+template <class I, int VEC>
+__global__ __launch_bounds__(256) void k_embed_join(SumArgs a, uint32_t tiles) {
+  __shared__ float sums[4][64 * VEC];
+  const uint32_t valid = a.start[a.rows];
+  const uint32_t k = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+  const uint32_t p0 = k * kChunk, p1 = p0 + kChunk;
+  if (p1 >= valid) return;  // nothing goes on behind the last chunk
+  const uint32_t row = static_cast<uint32_t>(static_cast<const I*>(a.ids)[a.perm[p1 - 1]]);
+  const uint32_t s = a.start[row], e = a.start[row + 1];
+  if (e - s <= kFew || s < p0 || e <= p1) return;
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t c = (tile * 64 + lane) * VEC;
+  const uint32_t pieces = (e - 1) / kChunk - k + 1, quarter = (pieces + 3) / 4;
+  const uint32_t q0 = min(wave * quarter, pieces), q1 = min(q0 + quarter, pieces);
+  float acc[VEC] = {};
+  if (c < a.dim) {
+    for (uint32_t q = q0; q < q1; q += 8) {  // eight pieces in flight, added in order
+      float v[8][VEC];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t slot = 2 * (k + q + i) + (q + i == 0 ? 1 : 0);
+        if (q + i < q1) load_f32<float, VEC>(a.partial + static_cast<uint64_t>(slot) * a.dim + c, v[i]);
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i)
+        if (q + i < q1)
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) acc[x] += v[i][x];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sums[wave][lane * VEC + i] = acc[i];
+  __syncthreads();
+  if (wave != 0 || c >= a.dim) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] += sums[w][lane * VEC + i];
+  put<VEC>(a, row, c, acc);
 }
 
 uint64_t round16(uint64_t b) { return (b + 15) / 16 * 16; }
@@ -379,12 +406,7 @@ int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t di
 }
 
 size_t omr_embed_grad_workspace_bytes(uint64_t num_ids, uint64_t num_rows, uint32_t dim) {
-  // (a call of fewer tokens may take smaller chunks, and more of them: the space is for any call of up to num_ids)
-  uint64_t chunks = 0;
-  for (uint64_t c = 64; c <= 1024; c *= 2) {
-    const uint64_t n = num_ids < c * c || c == 1024 ? num_ids : c * c;
-    if (n > chunk_tokens(n)) chunks = std::max(chunks, ceil_div(n, chunk_tokens(n)));
-  }
+  const uint64_t chunks = num_ids > kFew ? ceil_div(num_ids, kChunk) : 0;
   return round16(4 * (num_rows + 1)) + round16(4 * num_ids) + 2 * chunks * round16(4ull * dim);
 }
 
@@ -417,8 +439,7 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   a.ostride = table_stride;
   a.rows = static_cast<uint32_t>(num_rows);
   a.dim = dim;
-  a.chunk = chunk_tokens(num_ids);
-  a.chunks = num_ids > a.chunk ? static_cast<uint32_t>(ceil_div(num_ids, a.chunk)) : 0;
+  a.chunks = num_ids > kFew ? static_cast<uint32_t>(ceil_div(num_ids, kChunk)) : 0;
   a.scale = scale;
   a.accumulate = accumulate != 0;
   const uint32_t tokens = static_cast<uint32_t>(num_ids);
@@ -441,21 +462,21 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
     auto go = [&](auto i, auto vec) {
       using I = decltype(i);
       constexpr int VEC = decltype(vec)::value;
-      if (a.chunks != 0) {
-        const dim3 grid(a.chunks, static_cast<unsigned>(ceil_div(dim, 256 * VEC)));
-        k_embed_partial<T, I, VEC><<<grid, 256, 0, S(stream)>>>(a);
-        if (const int rc = elaunch("omr_embed_grad_f32 (partial)")) return rc;
-      }
-      a.tiles = static_cast<uint32_t>(ceil_div(dim, 64 * VEC));
-      uint32_t lpr_log = 6;
-      while (lpr_log > 2 && (1u << (lpr_log - 1)) * VEC * kRowsNJ >= dim) --lpr_log;
-      const uint64_t join = static_cast<uint64_t>(a.chunks) * a.tiles;
-      const uint64_t units = num_rows * ceil_div(dim, (static_cast<uint64_t>(VEC) << lpr_log) * kRowsNJ);
-      const uint64_t blocks = join + ceil_div(units, 256u >> lpr_log);
+      a.tiles = static_cast<uint32_t>(ceil_div(dim, 256 * VEC));
+      uint32_t lpr_log = 6;  // the fewest lanes that hold a row, and its tokens
+      while (lpr_log > 3 && (1u << (lpr_log - 1)) * VEC * kRowsNJ >= dim) --lpr_log;
+      const uint64_t first = static_cast<uint64_t>(a.chunks) * a.tiles;
+      const uint64_t units = ceil_div(num_rows, kRows) * ceil_div(dim, (static_cast<uint64_t>(VEC) << lpr_log) * kRowsNJ);
+      const uint64_t blocks = first + ceil_div(units, 256u >> lpr_log);
       if (blocks > kMaxBlocks) return efail("embed_grad: the table is too large for one call");
-      k_embed_rows<T, I, VEC><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(a, static_cast<uint32_t>(join),
-                                                                                   lpr_log);
-      return elaunch("omr_embed_grad_f32");
+      k_embed_sum<T, I, VEC><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(a, static_cast<uint32_t>(first),
+                                                                                  lpr_log);
+      if (const int rc = elaunch("omr_embed_grad_f32")) return rc;
+      if (a.chunks <= 1) return 0;
+      const uint32_t tiles = static_cast<uint32_t>(ceil_div(dim, 64 * VEC));
+      if (static_cast<uint64_t>(a.chunks) * tiles > kMaxBlocks) return efail("embed_grad: too many tokens for one call");
+      k_embed_join<I, VEC><<<a.chunks * tiles, 256, 0, S(stream)>>>(a, tiles);
+      return elaunch("omr_embed_grad_f32 (join)");
     };
     if (wide)
       return ids64 ? go(int64_t{}, std::integral_constant<int, 4>{}) : go(int32_t{}, std::integral_constant<int, 4>{});

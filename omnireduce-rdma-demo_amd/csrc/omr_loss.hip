@@ -69,8 +69,13 @@ struct Tile {
   static constexpr int kPieces = ROWS * 8 / NT;
   const char* base;          // this step's tile
   uint32_t off[kPieces];     // bytes from there
-  uint32_t kfirst[kPieces];  // the piece's first k within a step
   uint64_t inc;
+
+  // the piece's first k within a step
+  __device__ __forceinline__ uint32_t kfirst(int i) const {
+    const uint32_t q = i * NT + threadIdx.x;
+    return COL ? q / (ROWS / 8) : ((q & 7) ^ (q >> 3 & 7)) * 8;
+  }
 
   __device__ __forceinline__ void init(const Operand<T>& o, uint32_t row0, uint64_t kbegin) {
     const uint32_t t = threadIdx.x;
@@ -84,7 +89,6 @@ struct Tile {
         // rows past the end repeat the last one: they reach only results that are not stored
         const uint32_t row = min(row0 + m, o.rows - 1) - row0;
         off[i] = static_cast<uint32_t>((row * o.ld + c * 8) * sizeof(T));
-        kfirst[i] = c * 8;
       }
     } else {
       base = reinterpret_cast<const char*>(o.p + kbegin * o.ld + row0);
@@ -96,23 +100,34 @@ struct Tile {
         uint32_t m = ((c >> 1) ^ (pair_hash(k) % (kRow / 2))) * 16 + (c & 1) * 8;
         if (row0 + m >= o.rows) m = 0;
         off[i] = static_cast<uint32_t>((k * o.ld + m) * sizeof(T));
-        kfirst[i] = k;
       }
     }
   }
 
-  // one step's tile into `lds`; left: how many k of the inner dimension there still are
+  // One step's tile into `lds`; left: how many k of the inner dimension there still are.
+  // In inline assembly, and not as the builtin, because the compiler waits for all such loads in flight before any
+  // transposing read from LDS; the product's own wait stands in front of the barrier behind which a tile is read.  The
+  // loads write no register, and m0 (the LDS address) is set in the same block, with the wait state it needs.
   __device__ __forceinline__ void load(T* lds, uint32_t left) {
-    const uint32_t wave = threadIdx.x >> 6;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t to = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) T*)(lds))) + wave * 1024;
+    if (left >= kBK) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const char* src = base + off[i];
-      if (left < kBK && kfirst[i] >= left) src = reinterpret_cast<const char*>(g_zero);
-      __builtin_amdgcn_global_load_lds(
-          reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
-          reinterpret_cast<__attribute__((address_space(3))) void*>(
-              reinterpret_cast<uintptr_t>(lds + (i * NT + wave * 64) * 8)),
-          16, 0, 0);
+      for (int i = 0; i < kPieces; ++i)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(to + i * NT * 16), "v"(off[i]), "s"(base)
+                     : "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const char* src = kfirst(i) < left ? base + off[i] : reinterpret_cast<const char*>(g_zero);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                     :
+                     : "s"(to + i * NT * 16), "v"(src)
+                     : "memory");
+      }
     }
     base += inc;
   }

@@ -133,39 +133,56 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
   }
 }
 
+// A workgroup of 8 waves holds 8 / WPR rows at a time (WPR 16: one row of 16 waves), in lockstep where a row is more
+// than a wave.
 template <class T, class P, int VEC, int WPR>
-__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm_grad(NormArgs a) {
-  constexpr int NV = kCols / VEC, RPB = WPR == 1 ? 4 : 1;
-  __shared__ float lds[2][2][WPR];
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void k_norm_grad(NormArgs a) {
+  constexpr int NV = kCols / VEC, RPB = WPR == 16 ? 1 : 8 / WPR, WAVES = RPB * WPR, NT = 64 * WAVES;
+  __shared__ float lds[2][2][WAVES];
+  __shared__ float sum[RPB > 1 ? WAVES * 64 * kCols : 1];
+  const uint32_t wave = threadIdx.x >> 6, slot = wave / WPR, t = threadIdx.x - slot * 64 * WPR;
+  auto col = [&](int j) { return (static_cast<uint32_t>(j) * 64 * WPR + t) * VEC; };
   float w[NV][VEC], dw[NV][VEC] = {}, db[NV][VEC] = {};
-  if (a.w != nullptr) {
-    load_row<P, WPR, VEC>(static_cast<const P*>(a.w), a.dim, w, 0.0f);
-  } else {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    if (a.w != nullptr && col(j) < a.dim) {
+      load_f32<P, VEC>(static_cast<const P*>(a.w) + col(j), w[j]);
+    } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) w[j][i] = 1.0f;
+    }
   }
   int flip = 0;
-  for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * RPB + (WPR == 1 ? threadIdx.x >> 6 : 0); row < a.rows;
-       row += static_cast<uint64_t>(gridDim.x) * RPB) {
+  for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * RPB; first < a.rows;
+       first += static_cast<uint64_t>(gridDim.x) * RPB) {
+    const uint64_t row = first + slot;
+    const bool real = row < a.rows;
     float v[NV][VEC], g[NV][VEC];
-    load_row<T, WPR, VEC>(static_cast<const T*>(a.x) + row * a.xstride, a.dim, v, 0.0f);
-    load_row<T, WPR, VEC>(static_cast<const T*>(a.dy) + row * a.dystride, a.dim, g, 0.0f);
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float s1 = 0.0f, s2 = 0.0f;
+    float mean = 0.0f, rstd = 0.0f, s1 = 0.0f, s2 = 0.0f;
+    if (real) {
+      const T* x = static_cast<const T*>(a.x) + row * a.xstride;
+      const T* dy = static_cast<const T*>(a.dy) + row * a.dystride;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (col_of<WPR, VEC>(j) < a.dim) {
+      for (int j = 0; j < NV; ++j)
+        if (col(j) < a.dim) {
+          load_f32<T, VEC>(x + col(j), v[j]);
+          load_f32<T, VEC>(dy + col(j), g[j]);
+        }
+      mean = a.mean[row];
+      rstd = a.rstd[row];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float xh = (v[j][i] - mean) * rstd;
-          v[j][i] = xh;
-          dw[j][i] += g[j][i] * xh;
-          db[j][i] += g[j][i];
-          g[j][i] *= w[j][i];
-          s1 += g[j][i];
-          s2 += g[j][i] * xh;
+      for (int j = 0; j < NV; ++j) {
+        if (col(j) < a.dim) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float xh = (v[j][i] - mean) * rstd;
+            v[j][i] = xh;
+            dw[j][i] += g[j][i] * xh;
+            db[j][i] += g[j][i];
+            g[j][i] *= w[j][i];
+            s1 += g[j][i];
+            s2 += g[j][i] * xh;
+          }
         }
       }
     }
@@ -174,63 +191,58 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm_grad(NormArg
     s2 = wave_sum(s2);
     if constexpr (WPR > 1) {
       if ((threadIdx.x & 63) == 0) {
-        lds[flip][0][threadIdx.x >> 6] = s1;
-        lds[flip][1][threadIdx.x >> 6] = s2;
+        lds[flip][0][wave] = s1;
+        lds[flip][1][wave] = s2;
       }
       __syncthreads();
-      s1 = lds[flip][0][0];
-      s2 = lds[flip][1][0];
+      s1 = lds[flip][0][slot * WPR];
+      s2 = lds[flip][1][slot * WPR];
 #pragma unroll
       for (int k = 1; k < WPR; ++k) {
-        s1 += lds[flip][0][k];
-        s2 += lds[flip][1][k];
+        s1 += lds[flip][0][slot * WPR + k];
+        s2 += lds[flip][1][slot * WPR + k];
       }
       flip ^= 1;
     }
+    if (!real) continue;
     s1 *= a.inv_dim;
     s2 *= a.inv_dim;
     T* out = static_cast<T*>(a.out) + row * a.ostride;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const uint32_t c = col_of<WPR, VEC>(j);
-      if (c < a.dim) {
+      if (col(j) < a.dim) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) g[j][i] = (g[j][i] - s1 - v[j][i] * s2) * rstd;
-        store_f32<T, VEC>(out + c, g[j]);
+        store_f32<T, VEC>(out + col(j), g[j]);
       }
     }
   }
   if (a.partial == nullptr) return;
   float* part = a.partial + static_cast<uint64_t>(blockIdx.x) * 2 * a.dim;
-  if constexpr (WPR == 1) {  // the four waves' rows, in wave order
-    __shared__ float sum[4][64 * kCols];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
+  for (int which = 0; which < 2; ++which) {
+    float(&mine)[NV][VEC] = which == 0 ? dw : db;
+    if constexpr (RPB > 1) {  // the slots' sums, in slot order
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          sum[wave][(j * VEC + i) * 64 + lane] = which == 0 ? dw[j][i] : db[j][i];
+        for (int i = 0; i < VEC; ++i) sum[((slot * NV + j) * VEC + i) * 64 * WPR + t] = mine[j][i];
       __syncthreads();
-      // entry e of a wave's columns: piece j = e / 64 / VEC, element i, lane
-      for (uint32_t e = threadIdx.x; e < 64 * kCols; e += 256) {
-        const uint32_t ji = e >> 6, c = (ji / VEC * 64 + (e & 63)) * VEC + ji % VEC;
-        if (c < a.dim) part[which * a.dim + c] = ((sum[0][e] + sum[1][e]) + sum[2][e]) + sum[3][e];
-      }
-    }
-  } else {
+      constexpr uint32_t kWidth = 64 * WPR * kCols;  // entry e of a slot: piece j, element i, lane
+      for (uint32_t e = threadIdx.x; e < kWidth; e += NT) {
+        const uint32_t ji = e / (64 * WPR), c = (ji / VEC * 64 * WPR + e % (64 * WPR)) * VEC + ji % VEC;
+        float s = sum[e];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const uint32_t c = col_of<WPR, VEC>(j);
-      if (c < a.dim) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          part[c + i] = dw[j][i];
-          part[a.dim + c + i] = db[j][i];
-        }
+        for (int r = 1; r < RPB; ++r) s += sum[r * kWidth + e];
+        if (c < a.dim) part[which * a.dim + c] = s;
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (col(j) < a.dim)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) part[which * a.dim + col(j) + i] = mine[j][i];
     }
   }
 }
@@ -355,7 +367,7 @@ int waves_per_row(uint32_t dim) {
 constexpr uint32_t kGradBlocks = 512;
 uint32_t grad_blocks(uint64_t rows, uint32_t dim) {
   const int wpr = waves_per_row(dim);
-  const uint64_t want = wpr == 1 ? ceil_div(rows, 4) : wpr > 16 ? ceil_div(rows, kAnyWaves) : rows;
+  const uint64_t want = wpr > 16 ? ceil_div(rows, kAnyWaves) : wpr == 16 ? rows : ceil_div(rows, 8 / wpr);
   return static_cast<uint32_t>(want < kGradBlocks ? want : kGradBlocks);
 }
 
@@ -492,7 +504,7 @@ int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* 
                         aligned(weight, W * sizeof(P) < 16 ? W * sizeof(P) : 16);
       return with_shape<W>(wide, wpr, [&](auto vec, auto waves) {
         constexpr int VEC = decltype(vec)::value, WPR = decltype(waves)::value;
-        k_norm_grad<T, P, VEC, WPR><<<blocks, WPR == 1 ? 256 : 64 * WPR, 0, S(stream)>>>(a);
+        k_norm_grad<T, P, VEC, WPR><<<blocks, WPR == 16 ? 1024 : 512, 0, S(stream)>>>(a);
         return elaunch("omr_layer_norm_grad");
       });
     };
