@@ -104,64 +104,69 @@ struct Tile {
     }
   }
 
-  // One step's tile into `lds`; left: how many k of the inner dimension there still are.
+  __device__ __forceinline__ uint32_t place(const T* lds) const {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) T*)(lds))) +
+           wave * 1024;
+  }
+
+  // This lane's piece i of a whole step's tile into `lds` (place() of it).
   // In inline assembly, and not as the builtin, because the compiler waits for all such loads in flight before any
   // transposing read from LDS; the product's own wait stands in front of the barrier behind which a tile is read.  The
   // loads write no register, and m0 (the LDS address) is set in the same block, with the wait state it needs.
-  __device__ __forceinline__ void load(T* lds, uint32_t left) {
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t to = static_cast<uint32_t>(
-        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) T*)(lds))) + wave * 1024;
-    if (left >= kBK) {
+  __device__ __forceinline__ void load(int i, uint32_t to) const {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(to + i * NT * 16), "v"(off[i]), "s"(base)
+                 : "memory");
+  }
+  __device__ __forceinline__ void advance() { base += inc; }
+
+  // a tile of `left` k, zeros behind them
+  __device__ __forceinline__ void load_end(uint32_t to, uint32_t left) const {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                     :
-                     : "s"(to + i * NT * 16), "v"(off[i]), "s"(base)
-                     : "memory");
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const char* src = kfirst(i) < left ? base + off[i] : reinterpret_cast<const char*>(g_zero);
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                     :
-                     : "s"(to + i * NT * 16), "v"(src)
-                     : "memory");
-      }
+    for (int i = 0; i < kPieces; ++i) {
+      const char* src = kfirst(i) < left ? base + off[i] : reinterpret_cast<const char*>(g_zero);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                   :
+                   : "s"(to + i * NT * 16), "v"(src)
+                   : "memory");
     }
-    base += inc;
   }
 };
 
-// A wave's fragments of NF times 16 rows from row `row0` on
+// A wave's fragments of NF times 16 rows from row `row0` (a multiple of 16 NF) on.  Their places differ by an exclusive
+// or with a constant: one register holds the first, and the others are formed at each read (kept from being formed once
+// and spilled).
 template <class T, int ROWS, int NF, bool COL>
 struct Frags {
-  uint32_t at[COL ? NF : 2];
+  uint32_t at;
 
   __device__ __forceinline__ void init(uint32_t row0) {
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     if constexpr (!COL) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) at[s] = ((row0 + r) * 8 + ((s * 4 + g) ^ (r & 7))) * 8;
+      at = ((row0 + r) * 8 + (g ^ (r & 7))) * 8;
     } else {
       const uint32_t k = 8 * g + (r >> 2), h = pair_hash(k) % (ROWS / 16);
-#pragma unroll
-      for (int i = 0; i < NF; ++i) at[i] = k * ROWS + (((row0 >> 4) + i) ^ h) * 16 + (r & 3) * 4;
+      at = k * ROWS + ((row0 >> 4) ^ h) * 16 + (r & 3) * 4;
     }
   }
 
-  __device__ __forceinline__ frag<T> get(const T* lds, int i, int sub) const {
+  __device__ __forceinline__ frag<T> get(const T* lds, int half, int i) const {
     if constexpr (!COL) {
-      return *reinterpret_cast<const frag<T>*>(lds + at[sub] + i * 16 * kBK);
+      return *reinterpret_cast<const frag<T>*>(lds + (at ^ (half * 4 * 8)) + i * 16 * kBK);
     } else {
       typedef short s4 __attribute__((ext_vector_type(4)));
       using lp = __attribute__((address_space(3))) s4*;
-      const T* p = lds + at[i] + sub * 32 * ROWS;
+      const T* p = lds + (at ^ (i * 16)) + half * 32 * ROWS;
       const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)(p));
       const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)(p + 4 * ROWS));
       return __builtin_bit_cast(frag<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
+
+  // hides the place from the compiler, which would form all the others ahead of the loop and spill them
+  __device__ __forceinline__ void touch() { asm volatile("" : "+v"(at)); }
 };
 
 // ---------------------------------------------------------------- the product
@@ -227,7 +232,7 @@ template <class T, int EPI, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   constexpr int NT = 64 * WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
   constexpr bool AC = EPI == kHidden || EPI == kWeight, BC = EPI == kWeight;
-  __shared__ __attribute__((aligned(1024))) T la0[BM * kBK], la1[BM * kBK], lb0[BN * kBK], lb1[BN * kBK];
+  __shared__ __attribute__((aligned(1024))) T la[2][BM * kBK], lb[2][BN * kBK];
   // Workgroup ids go round the 8 XCDs: give each XCD a contiguous stretch of tiles, and walk the stretch in groups of 8
   // tile rows, so the tiles that run together on an XCD share operands in its L2.
   uint32_t id = blockIdx.x;
@@ -238,7 +243,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   const uint32_t group = id / (8 * a.nt), gm = min(8u, a.mt - group * 8), in = id - group * 8 * a.nt;
   const uint32_t m0 = (group * 8 + in % gm) * BM, n0 = in / gm * BN;
   const uint64_t kbegin = static_cast<uint64_t>(split) * a.ksplit;
-  uint32_t left = min(a.ksplit, static_cast<uint32_t>(a.k - kbegin));
+  const uint32_t left = min(a.ksplit, static_cast<uint32_t>(a.k - kbegin));
 
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const uint32_t wm = wave % WM, wn = wave / WM;
@@ -252,34 +257,103 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   fb.init(wn * (BN / WN));
   v4f acc[MF][NF] = {};
 
-  auto step = [&](T* ca, T* cb, T* na, T* nb) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    left = left > kBK ? left - kBK : 0;
-    if (left != 0) {
-      ta.load(na, left);
-      tb.load(nb, left);
+  // A step's 64 k are two halves.  The fragments of a half are read while the half before is multiplied: x[0], y[0] hold
+  // the first half of a step, x[1], y[1] the second.  Between them lies the step's one barrier: in front of it every wave
+  // has read its last from the step's buffer, into which the tile after the next may then be loaded, and has waited for
+  // its own pieces of the next tile.  Reads and loads are issued a few at a time between the matrix instructions: eight
+  // loads behind each other, from eight waves at once, held every wave's products for about 1000 of a step's 3600 clocks.
+  frag<T> x[2][MF], y[2][NF];
+  constexpr int kLoads = Tile<T, BM, NT, AC>::kPieces + Tile<T, BN, NT, BC>::kPieces;
+  static_assert(kLoads <= 2 * MF, "two loads a group at most");
+  const uint32_t steps = (left + kBK - 1) / kBK, full = left / kBK;
+  auto meet = [&]() {  // (the scheduler would move the products behind it)
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto fetch = [&](uint32_t t) {  // a whole tile at once
+    const uint32_t toa = ta.place(la[t & 1]), tob = tb.place(lb[t & 1]);
+    if (t < full) {
+#pragma unroll
+      for (int i = 0; i < Tile<T, BM, NT, AC>::kPieces; ++i) ta.load(i, toa);
+#pragma unroll
+      for (int i = 0; i < Tile<T, BN, NT, BC>::kPieces; ++i) tb.load(i, tob);
+    } else {
+      ta.load_end(toa, left - t * kBK);
+      tb.load_end(tob, left - t * kBK);
     }
+    ta.advance();
+    tb.advance();
+  };
+  // The products of one half, with the reads of the other from step t's buffer; with `loads` also the loads of step
+  // t + 1's tile.  (The reads end two groups early: the barrier behind waits for them.)
+  auto half = [&](int h, uint32_t t, bool loads) {
+    const T *ca = la[t & 1], *cb = lb[t & 1];
+    const uint32_t toa = ta.place(la[(t + 1) & 1]), tob = tb.place(lb[(t + 1) & 1]);
+    constexpr int kReads = MF + NF, kOver = MF - 2;
+    fa.touch();
+    fb.touch();
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      frag<T> x[MF], y[NF];
+    for (int i = 0; i < MF; ++i) {
 #pragma unroll
-      for (int i = 0; i < MF; ++i) x[i] = fa.get(ca, i, sub);
+      for (int j = 0; j < NF; ++j) acc[i][j] = mma(x[h][i], y[h][j], acc[i][j]);
+      if (loads) {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) y[j] = fb.get(cb, j, sub);
+        for (int l = i * kLoads / MF; l < (i + 1) * kLoads / MF; ++l) {
+          if (l < Tile<T, BM, NT, AC>::kPieces)
+            ta.load(l, toa);
+          else
+            tb.load(l - Tile<T, BM, NT, AC>::kPieces, tob);
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < MF; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) acc[i][j] = mma(x[i], y[j], acc[i][j]);
+      for (int r = i * kReads / kOver; r < (i + 1) * kReads / kOver && r < kReads; ++r) {
+        if (r < NF)
+          y[h ^ 1][r] = fb.get(cb, h ^ 1, r);
+        else
+          x[h ^ 1][r - NF] = fa.get(ca, h ^ 1, r - NF);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (loads) {
+      ta.advance();
+      tb.advance();
     }
   };
-  ta.load(la0, left);
-  tb.load(lb0, left);
-  while (true) {
-    step(la0, lb0, la1, lb1);
-    if (left == 0) break;
-    step(la1, lb1, la0, lb0);
-    if (left == 0) break;
+  fetch(0);
+  meet();
+  if (steps > 1) fetch(1);
+  uint32_t t = 0;
+  if (full > 2) {
+#pragma unroll
+    for (int j = 0; j < NF; ++j) y[0][j] = fb.get(lb[0], 0, j);
+#pragma unroll
+    for (int i = 0; i < MF; ++i) x[0][i] = fa.get(la[0], 0, i);
+    do {
+      half(0, t, false);
+      meet();
+      half(1, t + 1, true);
+    } while (++t + 2 < full);
+  }
+  // the last steps, whose tiles may be cut short: read and multiply in turn
+  for (; t < steps; ++t) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      fa.touch();
+      fb.touch();
+#pragma unroll
+      for (int j = 0; j < NF; ++j) y[0][j] = fb.get(lb[t & 1], h, j);
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        x[0][i] = fa.get(la[t & 1], h, i);
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = mma(x[0][i], y[0][j], acc[i][j]);
+      }
+    }
+    meet();
+    if (t + 2 < steps) fetch(t + 2);
   }
 
   // acc[i][j][r] = C[m + 16 i + r, n + 16 j]
