@@ -28,7 +28,7 @@ using namespace omr_elem;
 
 namespace {
 
-constexpr float kGScale = 4096.0f;
+constexpr float kGScale = 4096.0f, kLog2E = 1.44269504f;
 constexpr uint32_t kMaxStride = 1u << 22;  // elements: a tile's 32-bit byte offsets hold 256 rows of it
 
 // 16 zero bytes: what lanes past the end of a product's inner dimension load
@@ -367,13 +367,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
       const int at = target - static_cast<int>(a.v0 + m);  // the target's place among this lane's rows
       if constexpr (EPI == kStats) {
         float top = -INFINITY, z = 0.0f;
+        if (a.v0 + m0 + BM > a.vocab) {  // rows past the vocabulary do not count
+#pragma unroll
+          for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (a.v0 + m + 16 * i + r >= a.vocab) acc[i][j][r] = -INFINITY;
+        }
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if (a.v0 + m + 16 * i + r >= a.vocab) acc[i][j][r] = -INFINITY;
-            top = fmaxf(top, acc[i][j][r]);
-          }
+          for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float from = top == -INFINITY ? 0.0f : top;
@@ -399,19 +403,30 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
           *reinterpret_cast<float2*>(s) = make_float2(top, sum);
         }
       } else {
-        const float lse = target >= 0 ? a.lse[tok] : 0.0f;
+        // 2^12 exp(z - lse) as one power of two: 2^(z log2 e + shift); the argument's rounding, 2^-24 of some tens, is
+        // far below the result's
+        const float shift = target >= 0 ? 12.0f - a.lse[tok] * kLog2E : 0.0f;
         const bool here = target >= 0 && at >= 0 && at < 16 * MF && (at & 15) < 4;
-        const bool any = __ballot(here) != 0;
+        const bool any = __ballot(here) != 0, tail = a.v0 + m0 + BM > a.vocab;
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
+          float p[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2E, shift));
+          if (any) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (at == 16 * i + r) p[r] -= kGScale;
+          }
+          if (tail) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (a.v0 + m + 16 * i + r >= a.vocab) p[r] = 0.0f;
+          }
           vec_t<T, 4> o;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float p = __expf(acc[i][j][r] - lse);
-            if (any && at == 16 * i + r) p -= 1.0f;
-            if (target < 0 || a.v0 + m + 16 * i + r >= a.vocab) p = 0.0f;
-            o[r] = static_cast<T>(p * kGScale);
-          }
+          for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(p[r]);
+          if (target < 0) o = vec_t<T, 4>{};  // (whatever its hidden state holds)
           if (real) *reinterpret_cast<vec_t<T, 4>*>(a.g + static_cast<uint64_t>(tok) * a.ldg + m + 16 * i) = o;
         }
       }
