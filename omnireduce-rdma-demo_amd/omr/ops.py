@@ -294,22 +294,25 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class _Call:
-    """The device and stream of one call: every tensor must be on that device, which is made the current one."""
+    """The device and stream of one call: every tensor must be on that device, which `with` makes the current one.
+    (Short calls are bound by what is done here: a check costs a tenth of a microsecond or two, and is made once.)"""
 
-    __slots__ = ("device", "stream", "ptr", "_guard")
+    __slots__ = ("device", "index", "stream", "ptr", "_guard")
 
-    def __init__(self, device: torch.device, stream: Optional[torch.cuda.Stream]):
+    def __init__(self, t: torch.Tensor, stream: Optional[torch.cuda.Stream]):
+        device = t.device
         if device.type != "cuda":
             raise ValueError("expected a device (HIP) tensor")
-        self.device = device
-        if stream is not None and stream.device != device:
+        self.device, self.index, self.stream, self._guard = device, device.index, stream, None
+        if stream is None:
+            self.ptr = torch._C._cuda_getCurrentRawStream(self.index)
+        elif stream.device != device:
             raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-        self.stream = stream
-        self.ptr = (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
-        self._guard = None
+        else:
+            self.ptr = stream.cuda_stream
 
     def __enter__(self):
-        if torch.cuda.current_device() != self.device.index:
+        if torch._C._cuda_getDevice() != self.index:
             self._guard = torch.cuda.device(self.device)
             self._guard.__enter__()
         return self
@@ -326,49 +329,52 @@ class _Call:
             return torch.empty(shape, dtype=dtype, device=self.device)
 
     def on(self, t: torch.Tensor, name: str) -> int:
-        if t.device != self.device:
+        if not t.is_cuda or t.get_device() != self.index:
             raise ValueError(f"{name} is on {t.device}, expected {self.device}")
         return t.data_ptr()
 
     def rows(self, t: torch.Tensor, name: str, dim: Optional[int] = None, rows: Optional[int] = None,
              dtype: Optional[torch.dtype] = None, out: bool = False):
         """(pointer, rows, dim, row stride) of a tensor taken as rows of its last dimension."""
-        if t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
+        if t.dtype not in _DTYPES if dtype is None else t.dtype is not dtype:
             raise ValueError(f"{name}: element type {t.dtype}" + (f", expected {dtype}" if dtype is not None else ""))
         ptr = self.on(t, name)
         shape = t.shape
-        if t.dim() < 1 or shape[-1] == 0 or (dim is not None and shape[-1] != dim):
+        dims = len(shape)
+        if dims == 0 or shape[-1] == 0 or (dim is not None and shape[-1] != dim):
             raise ValueError(f"{name}: rows of {dim if dim is not None else 'at least one'} elements expected, got "
                              f"shape {tuple(shape)}")
         d = shape[-1]
-        n = t.numel() // d
+        n = shape[0] if dims == 2 else t.numel() // d
         if rows is not None and n != rows:
             raise ValueError(f"{name}: {rows} rows expected, got shape {tuple(shape)}")
-        if d > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{name}: the elements of a row must be consecutive (stride {t.stride()})")
-        if n <= 1 or t.dim() == 1:
+        strides = t.stride()
+        if d > 1 and strides[-1] != 1:
+            raise ValueError(f"{name}: the elements of a row must be consecutive (stride {strides})")
+        if n <= 1 or dims == 1:
             return ptr, n, d, d
-        if t.dim() == 2:
-            stride = t.stride(0)
+        if dims == 2:
+            stride = strides[0]
         elif t.is_contiguous():
             stride = d
         else:
-            raise ValueError(f"{name}: more than two dimensions must be contiguous (stride {t.stride()})")
+            raise ValueError(f"{name}: more than two dimensions must be contiguous (stride {strides})")
         if out and stride < d:
-            raise ValueError(f"{name}: an output's rows must not overlap (stride {t.stride()})")
+            raise ValueError(f"{name}: an output's rows must not overlap (stride {strides})")
         return ptr, n, d, stride
 
     def vector(self, t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype = torch.float32) -> Optional[int]:
         if t is None:
             return None
-        if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{name}: expected contiguous {dtype}[{n}], got {t.dtype}{tuple(t.shape)}")
         return self.on(t, name)
 
     def ids(self, t: torch.Tensor, name: str):
-        if t.dtype not in (torch.int32, torch.int64) or not t.is_contiguous():
+        wide = t.dtype is torch.int64
+        if not (wide or t.dtype is torch.int32) or not t.is_contiguous():
             raise ValueError(f"{name}: expected contiguous int32 or int64, got {t.dtype} (stride {t.stride()})")
-        return self.on(t, name), int(t.dtype == torch.int64), t.numel()
+        return self.on(t, name), int(wide), t.numel()
 
 
 class _Workspace:
@@ -393,7 +399,7 @@ def embed(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, out: Optio
           out_dtype: Optional[torch.dtype] = None, stream=None) -> torch.Tensor:
     """Embedding lookup: out[..., :] = scale * table[ids, :], rounded once to out's type (default: the table's).  An id
     outside [0, rows) names no row (padding): a row of zeros."""
-    with _Call(table.device, stream) as call:
+    with _Call(table, stream) as call:
         if table.dim() != 2:
             raise ValueError(f"table: expected [rows, dim], got shape {tuple(table.shape)}")
         tp, rows, dim, tstride = call.rows(table, "table")
@@ -417,7 +423,7 @@ class EmbedGradPlan:
             scale: float = 1.0, accumulate: bool = False, stream=None) -> torch.Tensor:
         """grad_table[v, :] = scale * (sum of grad_out's rows whose id is v, in token order), every row of it, or added
         to the rows that tokens name (accumulate).  Ids outside [0, rows) contribute nothing."""
-        with _Call(grad_out.device, stream) as call:
+        with _Call(grad_out, stream) as call:
             ip, ids64, n = call.ids(ids, "ids")
             if n > self.max_tokens:
                 raise ValueError(f"{n} tokens, the plan is for {self.max_tokens}")
@@ -458,7 +464,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5, out: Optional[torch.Tensor] = None, mean: Optional[torch.Tensor] = None,
                rstd: Optional[torch.Tensor] = None, stream=None) -> LayerNormResult:
     """Layer norm over the last dimension; out may be x.  mean and rstd (fp32, one a row) are what the gradient takes."""
-    with _Call(x.device, stream) as call:
+    with _Call(x, stream) as call:
         xp, n, dim, xstride = call.rows(x, "x")
         if weight is not None and bias is not None and weight.dtype != bias.dtype:
             raise ValueError("weight and bias must have one element type")
@@ -491,7 +497,7 @@ class LayerNormGradPlan:
             accumulate: bool = False, params: bool = True, stream=None) -> LayerNormGrads:
         """grad_x (may be grad_out or x), and the fp32 gradients of weight and bias, written or added to what is there
         (accumulate).  params=False: grad_x alone."""
-        with _Call(x.device, stream) as call:
+        with _Call(x, stream) as call:
             xp, n, dim, xstride = call.rows(x, "x", self.dim)
             if n > self.max_rows:
                 raise ValueError(f"{n} rows, the plan is for {self.max_rows}")
@@ -548,7 +554,7 @@ class VocabLossPlan:
     def forward(self, hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
                 loss: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, stream=None):
         """(loss, lse), fp32, one a token: loss = lse - logit of the target; 0 where the target names no row."""
-        with _Call(hidden.device, stream) as call:
+        with _Call(hidden, stream) as call:
             args, n = self._inputs(call, hidden, weight, targets)
             if loss is None:
                 loss = call.empty(targets.shape, torch.float32)
@@ -567,7 +573,7 @@ class VocabLossPlan:
         weight's type (default), written or added to (accumulate); need_hidden / need_weight=False leave one out."""
         if not self.grads:
             raise ValueError("the plan was made with grads=False")
-        with _Call(hidden.device, stream) as call:
+        with _Call(hidden, stream) as call:
             args, n = self._inputs(call, hidden, weight, targets)
             if grad_loss.dtype != torch.float32 or grad_loss.numel() not in (n, 1):
                 raise ValueError(f"grad_loss: fp32, {n} or one, got {grad_loss.dtype}{tuple(grad_loss.shape)}")
