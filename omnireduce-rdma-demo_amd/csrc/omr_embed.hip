@@ -358,6 +358,22 @@ constexpr uint64_t kMaxBlocks = (1u << 24) - 1;  // of 256 threads: a launch hol
 
 }  // namespace
 
+namespace omr_detail {
+int sort_ids(const void* ids, int ids64, uint32_t num_ids, uint32_t rows, uint32_t* start, uint32_t* perm,
+             hipStream_t stream) {
+  // rows per workgroup: one workgroup a CU where the table is small enough for that
+  const uint32_t range = std::min<uint32_t>(std::max<uint32_t>(static_cast<uint32_t>(ceil_div(rows, 256)), 16), kSortRange);
+  const unsigned blocks = static_cast<unsigned>(ceil_div(rows, range));
+  if (ids64)
+    k_embed_sort<int64_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int64_t*>(ids), num_ids, rows, range,
+                                                                 start, perm);
+  else
+    k_embed_sort<int32_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int32_t*>(ids), num_ids, rows, range,
+                                                                 start, perm);
+  return elaunch("sort by row");
+}
+}  // namespace omr_detail
+
 extern "C" {
 
 int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t dim, uint64_t row_stride,
@@ -442,19 +458,8 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   a.chunks = num_ids > kFew ? static_cast<uint32_t>(ceil_div(num_ids, kChunk)) : 0;
   a.scale = scale;
   a.accumulate = accumulate != 0;
-  const uint32_t tokens = static_cast<uint32_t>(num_ids);
-  // rows per sorting workgroup: one workgroup a CU where the table is small enough for that
-  uint64_t range = ceil_div(num_rows, 256);
-  if (range > kSortRange) range = kSortRange;
-  if (range < 16) range = 16;
-  const unsigned sorters = static_cast<unsigned>(ceil_div(num_rows, range));
-  if (ids64)
-    k_embed_sort<int64_t><<<sorters, 64 * kSortWaves, 0, S(stream)>>>(
-        static_cast<const int64_t*>(ids), tokens, a.rows, static_cast<uint32_t>(range), start, perm);
-  else
-    k_embed_sort<int32_t><<<sorters, 64 * kSortWaves, 0, S(stream)>>>(
-        static_cast<const int32_t*>(ids), tokens, a.rows, static_cast<uint32_t>(range), start, perm);
-  if (const int rc = elaunch("omr_embed_grad_f32 (sort)")) return rc;
+  if (const int rc = omr_detail::sort_ids(ids, ids64, static_cast<uint32_t>(num_ids), a.rows, start, perm, S(stream)))
+    return rc;
   return with_dtype(grad_dtype, [&](auto t) {
     using T = decltype(t);
     const bool wide = dim % 4 == 0 && grad_stride % 4 == 0 && table_stride % 4 == 0 &&

@@ -12,9 +12,10 @@
 // hidden states.
 //
 // Roundings to 16 bits, besides the outputs':
-//   - G, times 2^12 so that fp16 keeps the small probabilities normal (2^-26 and up).  grad_loss stays out of it: a mean's
-//     1 / tokens would shift every target's near -1 to the same place of a binade and bias the whole gradient by its one
-//     rounding error; near -1 itself the error is at most 2^-9 and random.
+//   - G, times 2^12 so that fp16 keeps the small probabilities normal (2^-26 and up).  The targets' entries, exp(..) - 1,
+//     outweigh the others together: what their rounding loses (`lost`, one value a token) is added to both products in
+//     fp32 (to a row of grad_weight only where it is at most kFewTargets tokens' target: more tokens' errors average out).
+//     Without that a few tokens' gradient was off by up to 2^-8 in bf16, twice what the output's own rounding is.
 //   - hidden[n] * (grad_loss[n] / max |grad_loss|) for grad_weight's sum over tokens: exact where grad_loss is the same
 //     for every token (the mean and the sum), else one rounding.
 // Sums are in fp32 throughout.
@@ -28,6 +29,7 @@ using namespace omr_elem;
 
 namespace {
 
+constexpr uint32_t kFewTargets = 8;
 constexpr float kGScale = 4096.0f, kLog2E = 1.44269504f;
 constexpr uint32_t kMaxStride = 1u << 22;  // elements: a tile's 32-bit byte offsets hold 256 rows of it
 
@@ -197,6 +199,9 @@ struct GemmArgs {
   int first, last;          // the sum over the pieces begins; is complete and goes to `out`
   const float* rowscale;    // [tokens]
   const float* amax;        // [1]
+  float* lost;              // [tokens] what the target's entry of G lost in rounding
+  Operand<T> w;             // kHidden: the whole weight
+  const uint32_t *start, *perm;  // kWeight: the tokens by target
   void* out;
   uint64_t ostride;
   int out_f32, accumulate, wide;  // wide: out takes 4 elements at a time
@@ -426,6 +431,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
           vec_t<T, 4> o;
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(p[r]);
+          if (any && here) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (at == 16 * i + r) a.lost[tok] = p[r] - static_cast<float>(o[r]);
+          }
           if (target < 0) o = vec_t<T, 4>{};  // (whatever its hidden state holds)
           if (real) *reinterpret_cast<vec_t<T, 4>*>(a.g + static_cast<uint64_t>(tok) * a.ldg + m + 16 * i) = o;
         }
@@ -437,6 +447,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
       const uint32_t tok = n + 16 * j;
       if (tok >= a.tokens) continue;
       const float scale = a.last ? a.rowscale[tok] : 0.0f;
+      const int target = a.last ? target_of(a, tok) : -1;
+      const float lost = target >= 0 ? a.lost[tok] : 0.0f;
+      auto target_row = [&](uint32_t c) {
+        float f[4] = {};
+        if (target >= 0) load_f32<T, 4>(a.w.p + target * a.w.ld + c, f);
+        return v4f{f[0], f[1], f[2], f[3]};
+      };
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         const uint32_t c = m + 16 * i;
@@ -450,6 +467,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
             if (static_cast<uint32_t>(r) < have) v[r] = sum[r] + v[r];
         }
         if (a.last) {
+          v += lost * target_row(c);
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = scale == 0.0f ? 0.0f : v[r] * scale;
           put4<T>(static_cast<T*>(a.out) + static_cast<uint64_t>(tok) * a.ostride + c, v, have, 0, a.wide);
@@ -465,6 +483,20 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
       const uint32_t row = n + 16 * j;
       if (a.v0 + row >= a.vocab) continue;
       const uint64_t o = static_cast<uint64_t>(a.v0 + row) * a.ostride;
+      const uint32_t t0 = a.start[a.v0 + row], t1 = a.start[a.v0 + row + 1];
+      if (t1 - t0 <= kFewTargets)
+        for (uint32_t t = t0; t < t1; ++t) {
+          const uint32_t tok = a.perm[t];
+          const float lost = a.lost[tok];
+#pragma unroll
+          for (int i = 0; i < MF; ++i)
+            if (m + 16 * i < a.dim) {
+              float f[4];
+              load_f32<T, 4>(a.a.p + tok * a.a.ld + m + 16 * i, f);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[i][j][r] += lost * f[r];
+            }
+        }
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         const uint32_t c = m + 16 * i;
@@ -570,6 +602,8 @@ __global__ __launch_bounds__(256) void k_join(GemmArgs<T> a) {
   const uint32_t tok = static_cast<uint32_t>(i / a.dim), c = static_cast<uint32_t>(i - static_cast<uint64_t>(tok) * a.dim);
   float v = 0.0f;
   for (uint32_t s = 0; s < a.splits; ++s) v += a.acc[s * all + i];
+  const int target = target_of(a, tok);
+  if (target >= 0) v += a.lost[tok] * static_cast<float>(a.w.p[target * a.w.ld + c]);
   const float scale = a.rowscale[tok];
   static_cast<T*>(a.out)[tok * a.ostride + c] = static_cast<T>(scale == 0.0f ? 0.0f : v * scale);
 }
@@ -638,7 +672,7 @@ Space layout(uint64_t tokens, uint64_t vocab, uint64_t dim, bool pack, bool grad
   s.h = s.w + (pack ? up(vocab * pdim * 2, 256) : 0);
   s.rest = s.h + (pack ? up(tokens * pdim * 2, 256) : 0);
   uint64_t fwd = up(tokens * 4, 256) + tokens * ceil_div(vocab, 64) * 8 + tokens * 32;
-  uint64_t bwd = 256 + up(tokens * 4, 256) + up(tokens * pdim * 2, 256) + up(piece_bytes_most(tokens, vocab), 256) +
+  uint64_t bwd = 256 + 3 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) + up(piece_bytes_most(tokens, vocab), 256) +
                  acc_bytes_most(tokens, dim);
   s.bytes = s.rest + (grads ? std::max(fwd, bwd) : fwd) + 256;
   return s;
@@ -791,6 +825,9 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     };
     float* amax = reinterpret_cast<float*>(take(4));
     float* rowscale = reinterpret_cast<float*>(take(tokens * 4));
+    float* lost = reinterpret_cast<float*>(take(tokens * 4));
+    uint32_t* perm = reinterpret_cast<uint32_t*>(take(tokens * 4));
+    uint32_t* start = reinterpret_cast<uint32_t*>(take(4 * vocab + 4));
     T* clean = reinterpret_cast<T*>(take(tokens * pdim * 2));
     T* g = reinterpret_cast<T*>(take(piece_bytes_most(tokens, vocab)));
     float* acc = reinterpret_cast<float*>(take(acc_bytes_most(tokens, dim)));
@@ -802,8 +839,10 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     a.dim = dim;
     k_scales<T><<<1, 1024, 0, S(stream)>>>(a, grad_loss, grad_loss_stride, amax, rowscale);
     if (const int rc = elaunch("omr_vocab_loss_grad (scales)")) return rc;
-    if (grad_weight != nullptr)
+    if (grad_weight != nullptr) {
       if (const int rc = pack_rows<T>(hidden, hidden_stride, tokens, dim, rowscale, amax, clean, S(stream))) return rc;
+      if (const int rc = omr_detail::sort_ids(targets, targets64, a.tokens, a.vocab, start, perm, S(stream))) return rc;
+    }
     const uint32_t piece = piece_rows(tokens, vocab);
     a.lse = lse;
     a.g = g;
@@ -811,6 +850,10 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     a.acc = acc;
     a.rowscale = rowscale;
     a.amax = amax;
+    a.lost = lost;
+    a.w = w;
+    a.start = start;
+    a.perm = perm;
     const uint32_t whole = static_cast<uint32_t>(std::min<uint64_t>(piece, vocab));
     const uint32_t ksplit = static_cast<uint32_t>(up(ceil_div(whole, hidden_splits(tokens, dim, piece)), kBK));
     const uint32_t splits = static_cast<uint32_t>(ceil_div(whole, ksplit));  // of a whole piece; the last may have fewer
