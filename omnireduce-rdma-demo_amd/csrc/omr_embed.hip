@@ -189,16 +189,14 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
 //
 // Bound by HBM: grad_out is read once and the table's gradient written once (65536 x 1024 fp32: 256 MiB), most of it
 // zeros.  Two kinds of workgroups of one launch share the rows:
-//   - row workgroups: a group of lanes takes four consecutive rows and stores the sums of those of at most kFew tokens,
-//     most of them zeros;
-//   - chunk workgroups: the sorted list in chunks of 64 positions, one a lane; the chunk's rows of more than kFew tokens
-//     are added up there.  A row that lies within its chunk is done; of one that goes on (a frequent word) the chunk's
-//     piece goes to `partial`, and k_embed_join adds its pieces up in order, a launch later.
-// So no wave adds up more than 64 rows behind each other.  (Rows of up to 128 tokens in the row workgroups held the
-// launch for 122 us at 8192 tokens of 65536 x 1024, whose bytes take 55.)
-constexpr uint32_t kChunk = 64, kFew = 8;
-constexpr int kRows = 4;  // consecutive rows of a lane group
-static_assert(kFew <= 8, "a lane group, 8 lanes at least, holds the tokens of a row of few");
+//   - chunk workgroups take the sorted list in chunks of 32 positions and add up the rows that lie there, 16 tokens'
+//     loads in flight whichever rows they belong to.  A row within its chunk is done; of one that goes on (a frequent
+//     word) the chunk's piece goes to `partial`, and k_embed_join adds its pieces up in order, a launch later;
+//   - fill workgroups store the zeros of the rows that no token names.
+// (Lane groups that summed or zeroed four rows each took 62 to 80 us at 8192 tokens of 65536 x 1024, every row with
+// tokens two dependent loads behind the stores around it; the zeros alone take 33.)
+constexpr uint32_t kChunk = 32;
+constexpr int kFlight = 16, kFillRows = 4;
 
 struct SumArgs {
   const void* grad_out;
@@ -228,84 +226,64 @@ __device__ __forceinline__ void put(const SumArgs& a, uint32_t row, uint32_t c, 
   store_f32<float, VEC>(o, v);
 }
 
-// acc += rows of grad_out, in order, at columns c + j * step: the tokens that lanes [l0, l0 + n) of this lane's group of
-// `width` lanes hold
-template <class T, int VEC, int NJ, int K>
-__device__ __forceinline__ void add_tokens(const SumArgs& a, uint32_t held, uint32_t l0, uint32_t n, uint32_t width,
-                                           uint32_t c, uint32_t step, float (&acc)[NJ][VEC]) {
-  const T* g = static_cast<const T*>(a.grad_out) + c;
-  for (uint32_t p = 0; p < n; p += K) {
-    float v[K][NJ][VEC];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t t = __shfl(held, static_cast<int>(l0 + (p + k < n ? p + k : n - 1)), static_cast<int>(width));
-      const T* r = g + static_cast<uint64_t>(t) * a.gstride;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        if (p + k < n && c + j * step < a.dim) load_f32<T, VEC>(r + j * step, v[k][j]);
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        if (p + k < n && c + j * step < a.dim)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[j][i] += v[k][j][i];
-  }
-}
-
-constexpr int kRowsNJ = 4;
-
-// blocks [0, chunks * tiles): chunks; behind them: rows, 2^lpr_log lanes a row
+// blocks [0, chunk_blocks): chunks, 256 VEC columns each; behind them: zeros, four rows a wave
 template <class T, class I, int VEC>
-__global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blocks, uint32_t lpr_log) {
+__global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blocks) {
+  const uint32_t lane = threadIdx.x & 63;
   if (blockIdx.x < chunk_blocks) {
     const uint32_t valid = a.start[a.rows];
-    const uint32_t k = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles, lane = threadIdx.x & 63;
+    const uint32_t k = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
     const uint32_t p0 = k * kChunk, p1 = min(p0 + kChunk, valid);
     if (p0 >= p1) return;
     const uint32_t c = (tile * 256 + threadIdx.x) * VEC;
-    // each lane: the token at its position and that token's row; a row's first position here speaks for it
-    const uint32_t held = a.perm[min(p0 + lane, p1 - 1)];
+    // lane l: the token at position p0 + l, its row, and whether the row's tokens here end with it
+    const uint32_t pos = min(p0 + lane % kChunk, p1 - 1);
+    const uint32_t held = a.perm[pos];
     const uint32_t row = static_cast<uint32_t>(static_cast<const I*>(a.ids)[held]);
     const uint32_t s = a.start[row], e = a.start[row + 1];
-    uint64_t todo = __ballot(p0 + lane < p1 && e - s > kFew && p0 + lane == max(s, p0));
-    while (todo != 0) {
-      const int l = __ffsll(static_cast<unsigned long long>(todo)) - 1;
-      todo &= todo - 1;
-      const uint32_t r = __shfl(row, l), rs = __shfl(s, l), re = __shfl(e, l);
-      float acc[1][VEC] = {};
-      add_tokens<T, VEC, 1, 8>(a, held, l, min(re, p1) - (p0 + l), 64, c, 0, acc);
-      if (c < a.dim) {
-        if (rs >= p0 && re <= p1)
-          put<VEC>(a, r, c, acc[0]);
-        else
-          store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k + (rs >= p0 ? 1 : 0)) * a.dim + c, acc[0]);
+    const uint64_t ends = __ballot(pos + 1 == min(e, p1));
+    const T* g = static_cast<const T*>(a.grad_out) + c;
+    float acc[VEC] = {};
+    const uint32_t here = p1 - p0;
+    for (uint32_t b = 0; b < here; b += kFlight) {
+      float v[kFlight][VEC];
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        const uint32_t t = __builtin_amdgcn_readlane(held, b + i);
+        if (b + i < here && c < a.dim) load_f32<T, VEC>(g + static_cast<uint64_t>(t) * a.gstride, v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        if (b + i < here) {
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) acc[x] += v[i][x];
+          if (ends >> (b + i) & 1) {
+            const uint32_t r = __builtin_amdgcn_readlane(row, b + i), rs = __builtin_amdgcn_readlane(s, b + i),
+                           re = __builtin_amdgcn_readlane(e, b + i);
+            if (c < a.dim) {
+              if (rs >= p0 && re <= p1)
+                put<VEC>(a, r, c, acc);
+              else
+                store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k + (rs >= p0 ? 1 : 0)) * a.dim + c, acc);
+            }
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) acc[x] = 0.0f;
+          }
+        }
       }
     }
     return;
   }
-  const uint32_t lpr = 1u << lpr_log, sub = threadIdx.x & (lpr - 1), step = lpr * VEC;
-  const uint64_t unit = (static_cast<uint64_t>(blockIdx.x - chunk_blocks) * 256 + threadIdx.x) >> lpr_log;
-  const uint32_t tiles = (a.dim + step * kRowsNJ - 1) / (step * kRowsNJ);
-  const uint64_t four = unit / tiles;
-  const uint32_t c = static_cast<uint32_t>(unit - four * tiles) * step * kRowsNJ + sub * VEC;
-  uint32_t at[kRows + 1];
+  const uint64_t first = (static_cast<uint64_t>(blockIdx.x - chunk_blocks) * 4 + (threadIdx.x >> 6)) * kFillRows;
+  uint32_t at[kFillRows + 1];
 #pragma unroll
-  for (int q = 0; q <= kRows; ++q) at[q] = a.start[min(four * kRows + q, static_cast<uint64_t>(a.rows))];
+  for (int q = 0; q <= kFillRows; ++q) at[q] = a.start[min(first + q, static_cast<uint64_t>(a.rows))];
+  const float zero[VEC] = {};
 #pragma unroll
-  for (int q = 0; q < kRows; ++q) {
-    const uint64_t row = four * kRows + q;
-    const uint32_t n = at[q + 1] - at[q];
-    if (row >= a.rows || n > kFew || (a.accumulate && n == 0)) continue;
-    float acc[kRowsNJ][VEC] = {};
-    if (n != 0) {
-      const uint32_t held = a.perm[at[q] + min(sub, n - 1)];
-      add_tokens<T, VEC, kRowsNJ, 4>(a, held, 0, n, lpr, c, step, acc);
-    }
-#pragma unroll
-    for (int j = 0; j < kRowsNJ; ++j)
-      if (c + j * step < a.dim) put<VEC>(a, static_cast<uint32_t>(row), c + j * step, acc[j]);
+  for (int q = 0; q < kFillRows; ++q) {
+    if (first + q >= a.rows || at[q] != at[q + 1]) continue;
+    float* o = a.out + (first + q) * a.ostride;
+    for (uint32_t c = lane * VEC; c < a.dim; c += 64 * VEC) store_f32<float, VEC>(o + c, zero);
   }
 }
 
@@ -320,7 +298,7 @@ __global__ __launch_bounds__(256) void k_embed_join(SumArgs a, uint32_t tiles) {
   if (p1 >= valid) return;  // nothing goes on behind the last chunk
   const uint32_t row = static_cast<uint32_t>(static_cast<const I*>(a.ids)[a.perm[p1 - 1]]);
   const uint32_t s = a.start[row], e = a.start[row + 1];
-  if (e - s <= kFew || s < p0 || e <= p1) return;
+  if (s < p0 || e <= p1) return;
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const uint32_t c = (tile * 64 + lane) * VEC;
   const uint32_t pieces = (e - 1) / kChunk - k + 1, quarter = (pieces + 3) / 4;
@@ -422,7 +400,7 @@ int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t di
 }
 
 size_t omr_embed_grad_workspace_bytes(uint64_t num_ids, uint64_t num_rows, uint32_t dim) {
-  const uint64_t chunks = num_ids > kFew ? ceil_div(num_ids, kChunk) : 0;
+  const uint64_t chunks = num_ids != 0 ? ceil_div(num_ids, kChunk) : 0;
   return round16(4 * (num_rows + 1)) + round16(4 * num_ids) + 2 * chunks * round16(4ull * dim);
 }
 
@@ -455,7 +433,7 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   a.ostride = table_stride;
   a.rows = static_cast<uint32_t>(num_rows);
   a.dim = dim;
-  a.chunks = num_ids > kFew ? static_cast<uint32_t>(ceil_div(num_ids, kChunk)) : 0;
+  a.chunks = num_ids != 0 ? static_cast<uint32_t>(ceil_div(num_ids, kChunk)) : 0;
   a.scale = scale;
   a.accumulate = accumulate != 0;
   if (const int rc = omr_detail::sort_ids(ids, ids64, static_cast<uint32_t>(num_ids), a.rows, start, perm, S(stream)))
@@ -468,14 +446,11 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
       using I = decltype(i);
       constexpr int VEC = decltype(vec)::value;
       a.tiles = static_cast<uint32_t>(ceil_div(dim, 256 * VEC));
-      uint32_t lpr_log = 6;  // the fewest lanes that hold a row, and its tokens
-      while (lpr_log > 3 && (1u << (lpr_log - 1)) * VEC * kRowsNJ >= dim) --lpr_log;
       const uint64_t first = static_cast<uint64_t>(a.chunks) * a.tiles;
-      const uint64_t units = ceil_div(num_rows, kRows) * ceil_div(dim, (static_cast<uint64_t>(VEC) << lpr_log) * kRowsNJ);
-      const uint64_t blocks = first + ceil_div(units, 256u >> lpr_log);
-      if (blocks > kMaxBlocks) return efail("embed_grad: the table is too large for one call");
-      k_embed_sum<T, I, VEC><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(a, static_cast<uint32_t>(first),
-                                                                                  lpr_log);
+      const uint64_t blocks = first + (accumulate ? 0 : ceil_div(num_rows, 4 * kFillRows));
+      if (blocks > kMaxBlocks) return efail("embed_grad: too many tokens or rows for one call");
+      if (blocks == 0) return 0;
+      k_embed_sum<T, I, VEC><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(a, static_cast<uint32_t>(first));
       if (const int rc = elaunch("omr_embed_grad_f32")) return rc;
       if (a.chunks <= 1) return 0;
       const uint32_t tiles = static_cast<uint32_t>(ceil_div(dim, 64 * VEC));
