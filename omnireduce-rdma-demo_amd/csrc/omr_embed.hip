@@ -74,20 +74,22 @@ __global__ __launch_bounds__(256) void k_embed(const T* table, uint32_t rows, ui
 //   scan    start[v] = ids below v; hist[w][.] = where wave w's first token of that row goes
 //   pass 2  the waves walk their lists (or, where a list is full, their tokens again) and place them: within 64 tokens
 //           the lanes of equal ids rank themselves by lane (match by ballots over the bits of the local id), so the
-//           order within a row is token order
+//           order within a row is token order; named[i], where it is wanted, is the row of the i-th of the sorted list
 // Every workgroup reads T ids: hidden in the L2 up to some 100 k tokens, where a radix sort would take three launches
 // for each of three digits.
 constexpr int kSortWaves = 16;
 constexpr int kSortRange = 1024;  // rows per workgroup at most: 64 KiB of histogram
 constexpr int kSortBits = 10;
+constexpr uint32_t kNoRow = ~0u;
 constexpr uint32_t kSortList = 512;  // tokens a wave notes: 32 KiB
 
 template <class I>
 __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, uint32_t tokens, uint32_t rows,
-                                                               uint32_t range, uint32_t* start, uint32_t* perm) {
+                                                               uint32_t range, uint32_t* start, uint32_t* perm,
+                                                               uint32_t* named) {
   __shared__ uint32_t hist[kSortWaves * kSortRange];
   __shared__ uint32_t list[kSortWaves][kSortList];  // (token - the wave's first) << 10 | local id
-  __shared__ uint32_t wsum[kSortWaves], below_w[kSortWaves];
+  __shared__ uint32_t wsum[kSortWaves], below_w[kSortWaves], valid;
   const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t lo = blockIdx.x * range, n = min(range, rows - lo);
   for (uint32_t i = tid; i < kSortWaves * range; i += 64 * kSortWaves) hist[i] = 0;
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
   }
   if (tid < n) {
     start[lo + tid] = at;
-    if (lo + tid == rows - 1) start[rows] = at + total;
+    if (lo + tid == rows - 1) start[rows] = valid = at + total;
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
       const uint32_t c = hist[w * range + tid];
@@ -181,8 +183,14 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
     uint32_t base = 0;
     if (in && lane == leader) base = atomicAdd(&mine[v], static_cast<uint32_t>(__popcll(same)));
     base = __shfl(base, static_cast<int>(leader));
-    if (in) perm[base + __popcll(same & ((1ull << lane) - 1))] = t;
+    if (in) {
+      const uint32_t to = base + __popcll(same & ((1ull << lane) - 1));
+      perm[to] = t;
+      if (named != nullptr) named[to] = lo + v;
+    }
   }
+  if (named != nullptr && lo + n == rows)  // behind the last
+    for (uint32_t i = valid + tid; i < tokens; i += 64 * kSortWaves) named[i] = kNoRow;
 }
 
 // ---------------------------------------------------------------- sums
@@ -201,9 +209,10 @@ constexpr int kFlight = 16, kFillRows = 4;
 struct SumArgs {
   const void* grad_out;
   uint64_t gstride;
-  const void* ids;
   const uint32_t* start;  // [rows + 1]
   const uint32_t* perm;   // the valid tokens by row
+  const uint32_t* named;  // their rows, kNoRow behind the last
+  uint32_t tokens;
   float* partial;         // [2 * chunks][dim]: the piece of the row that began before the chunk; of the one that goes on
   float* out;
   uint64_t ostride;
@@ -227,24 +236,25 @@ __device__ __forceinline__ void put(const SumArgs& a, uint32_t row, uint32_t c, 
 }
 
 // blocks [0, chunk_blocks): chunks, 256 VEC columns each; behind them: zeros, four rows a wave
-template <class T, class I, int VEC>
+template <class T, int VEC>
 __global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blocks) {
   const uint32_t lane = threadIdx.x & 63;
   if (blockIdx.x < chunk_blocks) {
-    const uint32_t valid = a.start[a.rows];
     const uint32_t k = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
-    const uint32_t p0 = k * kChunk, p1 = min(p0 + kChunk, valid);
-    if (p0 >= p1) return;
+    const uint32_t p0 = k * kChunk, p1 = min(p0 + kChunk, a.tokens);
     const uint32_t c = (tile * 256 + threadIdx.x) * VEC;
-    // lane l: the token at position p0 + l, its row, and whether the row's tokens here end with it
+    // lane l: the token at position p0 + l, its row and its neighbours', all at once: a load that waits for another one
+    // waits behind the zero fills' stores each time
     const uint32_t pos = min(p0 + lane % kChunk, p1 - 1);
-    const uint32_t held = a.perm[pos];
-    const uint32_t row = static_cast<uint32_t>(static_cast<const I*>(a.ids)[held]);
-    const uint32_t s = a.start[row], e = a.start[row + 1];
-    const uint64_t ends = __ballot(pos + 1 == min(e, p1));
+    const uint32_t held = a.perm[pos], row = a.named[pos];
+    const uint32_t next = pos + 1 < a.tokens ? a.named[pos + 1] : kNoRow;
+    const uint32_t before = p0 != 0 ? a.named[p0 - 1] : kNoRow;
+    const bool real = p0 + lane < p1 && row != kNoRow;
+    const uint32_t here = static_cast<uint32_t>(__popcll(__ballot(real)));
+    // its row's tokens here end with it, or go on behind the chunk
+    const uint64_t ends = __ballot(real && (row != next || pos + 1 == p1)), on = __ballot(real && row == next);
     const T* g = static_cast<const T*>(a.grad_out) + c;
     float acc[VEC] = {};
-    const uint32_t here = p1 - p0;
     for (uint32_t b = 0; b < here; b += kFlight) {
       float v[kFlight][VEC];
 #pragma unroll
@@ -258,13 +268,13 @@ __global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blo
 #pragma unroll
           for (int x = 0; x < VEC; ++x) acc[x] += v[i][x];
           if (ends >> (b + i) & 1) {
-            const uint32_t r = __builtin_amdgcn_readlane(row, b + i), rs = __builtin_amdgcn_readlane(s, b + i),
-                           re = __builtin_amdgcn_readlane(e, b + i);
+            const uint32_t r = __builtin_amdgcn_readlane(row, b + i);
+            const bool began = r == before, goes = on >> (b + i) & 1;
             if (c < a.dim) {
-              if (rs >= p0 && re <= p1)
+              if (!began && !goes)
                 put<VEC>(a, r, c, acc);
               else
-                store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k + (rs >= p0 ? 1 : 0)) * a.dim + c, acc);
+                store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k + (began ? 0 : 1)) * a.dim + c, acc);
             }
 #pragma unroll
             for (int x = 0; x < VEC; ++x) acc[x] = 0.0f;
@@ -289,16 +299,15 @@ __global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blo
 
 // The row that begins in chunk k and goes on behind it, 64 VEC columns; the four waves each take a quarter of its pieces
 // (in order), and wave 0 adds the quarters up.
-template <class I, int VEC>
+template <int VEC>
 __global__ __launch_bounds__(256) void k_embed_join(SumArgs a, uint32_t tiles) {
   __shared__ float sums[4][64 * VEC];
-  const uint32_t valid = a.start[a.rows];
   const uint32_t k = blockIdx.x / tiles, tile = blockIdx.x % tiles;
   const uint32_t p0 = k * kChunk, p1 = p0 + kChunk;
-  if (p1 >= valid) return;  // nothing goes on behind the last chunk
-  const uint32_t row = static_cast<uint32_t>(static_cast<const I*>(a.ids)[a.perm[p1 - 1]]);
-  const uint32_t s = a.start[row], e = a.start[row + 1];
-  if (s < p0 || e <= p1) return;
+  if (p1 >= a.tokens) return;  // nothing goes on behind the last chunk
+  const uint32_t row = a.named[p1 - 1];
+  if (row == kNoRow || a.named[p1] != row || (p0 != 0 && a.named[p0 - 1] == row)) return;
+  const uint32_t e = a.start[row + 1];
   const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const uint32_t c = (tile * 64 + lane) * VEC;
   const uint32_t pieces = (e - 1) / kChunk - k + 1, quarter = (pieces + 3) / 4;
@@ -338,16 +347,16 @@ constexpr uint64_t kMaxBlocks = (1u << 24) - 1;  // of 256 threads: a launch hol
 
 namespace omr_detail {
 int sort_ids(const void* ids, int ids64, uint32_t num_ids, uint32_t rows, uint32_t* start, uint32_t* perm,
-             hipStream_t stream) {
+             uint32_t* named, hipStream_t stream) {
   // rows per workgroup: one workgroup a CU where the table is small enough for that
   const uint32_t range = std::min<uint32_t>(std::max<uint32_t>(static_cast<uint32_t>(ceil_div(rows, 256)), 16), kSortRange);
   const unsigned blocks = static_cast<unsigned>(ceil_div(rows, range));
   if (ids64)
     k_embed_sort<int64_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int64_t*>(ids), num_ids, rows, range,
-                                                                 start, perm);
+                                                                 start, perm, named);
   else
     k_embed_sort<int32_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int32_t*>(ids), num_ids, rows, range,
-                                                                 start, perm);
+                                                                 start, perm, named);
   return elaunch("sort by row");
 }
 }  // namespace omr_detail
@@ -401,7 +410,7 @@ int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t di
 
 size_t omr_embed_grad_workspace_bytes(uint64_t num_ids, uint64_t num_rows, uint32_t dim) {
   const uint64_t chunks = num_ids != 0 ? ceil_div(num_ids, kChunk) : 0;
-  return round16(4 * (num_rows + 1)) + round16(4 * num_ids) + 2 * chunks * round16(4ull * dim);
+  return round16(4 * (num_rows + 1)) + 2 * round16(4 * num_ids) + 2 * chunks * round16(4ull * dim);
 }
 
 int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_stride, const void* ids, int ids64,
@@ -423,12 +432,14 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   char* ws = static_cast<char*>(workspace);
   a.grad_out = grad_out;
   a.gstride = grad_stride;
-  a.ids = ids;
   uint32_t* start = reinterpret_cast<uint32_t*>(ws);
   uint32_t* perm = reinterpret_cast<uint32_t*>(ws + round16(4 * (num_rows + 1)));
   a.start = start;
   a.perm = perm;
-  a.partial = reinterpret_cast<float*>(ws + round16(4 * (num_rows + 1)) + round16(4 * num_ids));
+  uint32_t* named = perm + round16(4 * num_ids) / 4;
+  a.named = named;
+  a.tokens = static_cast<uint32_t>(num_ids);
+  a.partial = reinterpret_cast<float*>(ws + round16(4 * (num_rows + 1)) + 2 * round16(4 * num_ids));
   a.out = grad_table;
   a.ostride = table_stride;
   a.rows = static_cast<uint32_t>(num_rows);
@@ -436,31 +447,28 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   a.chunks = num_ids != 0 ? static_cast<uint32_t>(ceil_div(num_ids, kChunk)) : 0;
   a.scale = scale;
   a.accumulate = accumulate != 0;
-  if (const int rc = omr_detail::sort_ids(ids, ids64, static_cast<uint32_t>(num_ids), a.rows, start, perm, S(stream)))
+  if (const int rc = omr_detail::sort_ids(ids, ids64, a.tokens, a.rows, start, perm, named, S(stream)))
     return rc;
   return with_dtype(grad_dtype, [&](auto t) {
     using T = decltype(t);
     const bool wide = dim % 4 == 0 && grad_stride % 4 == 0 && table_stride % 4 == 0 &&
                       aligned(grad_out, 4 * sizeof(T)) && aligned(grad_table, 16);
-    auto go = [&](auto i, auto vec) {
-      using I = decltype(i);
+    auto go = [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       a.tiles = static_cast<uint32_t>(ceil_div(dim, 256 * VEC));
       const uint64_t first = static_cast<uint64_t>(a.chunks) * a.tiles;
       const uint64_t blocks = first + (accumulate ? 0 : ceil_div(num_rows, 4 * kFillRows));
       if (blocks > kMaxBlocks) return efail("embed_grad: too many tokens or rows for one call");
       if (blocks == 0) return 0;
-      k_embed_sum<T, I, VEC><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(a, static_cast<uint32_t>(first));
+      k_embed_sum<T, VEC><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(a, static_cast<uint32_t>(first));
       if (const int rc = elaunch("omr_embed_grad_f32")) return rc;
       if (a.chunks <= 1) return 0;
       const uint32_t tiles = static_cast<uint32_t>(ceil_div(dim, 64 * VEC));
       if (static_cast<uint64_t>(a.chunks) * tiles > kMaxBlocks) return efail("embed_grad: too many tokens for one call");
-      k_embed_join<I, VEC><<<a.chunks * tiles, 256, 0, S(stream)>>>(a, tiles);
+      k_embed_join<VEC><<<a.chunks * tiles, 256, 0, S(stream)>>>(a, tiles);
       return elaunch("omr_embed_grad_f32 (join)");
     };
-    if (wide)
-      return ids64 ? go(int64_t{}, std::integral_constant<int, 4>{}) : go(int32_t{}, std::integral_constant<int, 4>{});
-    return ids64 ? go(int64_t{}, std::integral_constant<int, 1>{}) : go(int32_t{}, std::integral_constant<int, 1>{});
+    return wide ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 1>{});
   });
 }
 

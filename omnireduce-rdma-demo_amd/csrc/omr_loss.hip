@@ -841,7 +841,8 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     if (const int rc = elaunch("omr_vocab_loss_grad (scales)")) return rc;
     if (grad_weight != nullptr) {
       if (const int rc = pack_rows<T>(hidden, hidden_stride, tokens, dim, rowscale, amax, clean, S(stream))) return rc;
-      if (const int rc = omr_detail::sort_ids(targets, targets64, a.tokens, a.vocab, start, perm, S(stream))) return rc;
+      if (const int rc = omr_detail::sort_ids(targets, targets64, a.tokens, a.vocab, start, perm, nullptr, S(stream)))
+        return rc;
     }
     const uint32_t piece = piece_rows(tokens, vocab);
     a.lse = lse;
