@@ -469,7 +469,7 @@ int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t di
 /* Its gradient: grad_table[v, :] = scale * (sum over the t with ids[t] == v, in order of t, of grad_out[t, :]), fp32;
  * every row of grad_table is written (zeros where no token names it), or, with accumulate != 0, the sums are added to
  * the rows that tokens name and the others are left as they are.  Tokens whose id names no row are skipped, whatever
- * their row of grad_out holds.  (A row of many tokens is summed in chunks of at most 32, which
+ * their row of grad_out holds.  (A row of many tokens is summed in chunks of at most 16, which
  * are then added up.) */
 size_t omr_embed_grad_workspace_bytes(uint64_t num_ids, uint64_t num_rows, uint32_t dim);
 int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_stride, const void* ids, int ids64,

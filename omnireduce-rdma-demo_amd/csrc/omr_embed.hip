@@ -197,14 +197,16 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
 //
 // Bound by HBM: grad_out is read once and the table's gradient written once (65536 x 1024 fp32: 256 MiB), most of it
 // zeros.  Two kinds of workgroups of one launch share the rows:
-//   - chunk workgroups take the sorted list in chunks of 32 positions and add up the rows that lie there, 16 tokens'
-//     loads in flight whichever rows they belong to.  A row within its chunk is done; of one that goes on (a frequent
+//   - chunk workgroups take the sorted list in chunks of 16 positions and add up the rows that lie there, all their
+//     loads in flight at once.  A row within its chunk is done; of one that goes on (a frequent
 //     word) the chunk's piece goes to `partial`, and k_embed_join adds its pieces up in order, a launch later;
 //   - fill workgroups store the zeros of the rows that no token names.
-// (Lane groups that summed or zeroed four rows each took 62 to 80 us at 8192 tokens of 65536 x 1024, every row with
-// tokens two dependent loads behind the stores around it; the zeros alone take 33.)
-constexpr uint32_t kChunk = 32;
-constexpr int kFlight = 16, kFillRows = 4;
+// 8192 tokens of 65536 x 1024 take 55 us with the sort and the join, 290 MB at 5.3 TB/s; the zeros alone, with the sort,
+// 41.  (Chunks of 32 in two flights of 16: 63.  Lane groups that summed or zeroed four rows each: 92, every row with
+// tokens two dependent loads behind the stores around it.  The chunks in a launch of their own in front of the zeros,
+// at 32: 64, and 94 against 88 at 32768 tokens.)
+constexpr uint32_t kChunk = 16;
+constexpr int kFillRows = 4;
 
 struct SumArgs {
   const void* grad_out;
@@ -255,30 +257,28 @@ __global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blo
     const uint64_t ends = __ballot(real && (row != next || pos + 1 == p1)), on = __ballot(real && row == next);
     const T* g = static_cast<const T*>(a.grad_out) + c;
     float acc[VEC] = {};
-    for (uint32_t b = 0; b < here; b += kFlight) {
-      float v[kFlight][VEC];
+    float v[kChunk][VEC];
 #pragma unroll
-      for (int i = 0; i < kFlight; ++i) {
-        const uint32_t t = __builtin_amdgcn_readlane(held, b + i);
-        if (b + i < here && c < a.dim) load_f32<T, VEC>(g + static_cast<uint64_t>(t) * a.gstride, v[i]);
-      }
+    for (uint32_t i = 0; i < kChunk; ++i) {
+      const uint32_t t = __builtin_amdgcn_readlane(held, i);
+      if (i < here && c < a.dim) load_f32<T, VEC>(g + static_cast<uint64_t>(t) * a.gstride, v[i]);
+    }
 #pragma unroll
-      for (int i = 0; i < kFlight; ++i) {
-        if (b + i < here) {
+    for (uint32_t i = 0; i < kChunk; ++i) {
+      if (i < here) {
 #pragma unroll
-          for (int x = 0; x < VEC; ++x) acc[x] += v[i][x];
-          if (ends >> (b + i) & 1) {
-            const uint32_t r = __builtin_amdgcn_readlane(row, b + i);
-            const bool began = r == before, goes = on >> (b + i) & 1;
-            if (c < a.dim) {
-              if (!began && !goes)
-                put<VEC>(a, r, c, acc);
-              else
-                store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k + (began ? 0 : 1)) * a.dim + c, acc);
-            }
-#pragma unroll
-            for (int x = 0; x < VEC; ++x) acc[x] = 0.0f;
+        for (int x = 0; x < VEC; ++x) acc[x] += v[i][x];
+        if (ends >> i & 1) {
+          const uint32_t r = __builtin_amdgcn_readlane(row, i);
+          const bool began = r == before, goes = on >> i & 1;
+          if (c < a.dim) {
+            if (!began && !goes)
+              put<VEC>(a, r, c, acc);
+            else
+              store_f32<float, VEC>(a.partial + static_cast<uint64_t>(2 * k + (began ? 0 : 1)) * a.dim + c, acc);
           }
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) acc[x] = 0.0f;
         }
       }
     }
@@ -288,12 +288,18 @@ __global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blo
   uint32_t at[kFillRows + 1];
 #pragma unroll
   for (int q = 0; q <= kFillRows; ++q) at[q] = a.start[min(first + q, static_cast<uint64_t>(a.rows))];
-  const float zero[VEC] = {};
 #pragma unroll
   for (int q = 0; q < kFillRows; ++q) {
     if (first + q >= a.rows || at[q] != at[q + 1]) continue;
     float* o = a.out + (first + q) * a.ostride;
-    for (uint32_t c = lane * VEC; c < a.dim; c += 64 * VEC) store_f32<float, VEC>(o + c, zero);
+    if constexpr (VEC == 4) {
+      // written through (sc0 sc1): no dirty lines are left in the L2s to be flushed behind the last wave (2 us)
+      typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+      const auto to = __builtin_amdgcn_make_buffer_rsrc(o, 0, static_cast<int>(a.dim * 4), 0x00020000);
+      for (uint32_t c = lane * 4; c < a.dim; c += 256) __builtin_amdgcn_raw_buffer_store_b128(v4u{}, to, c * 4, 0, 17);
+    } else {
+      for (uint32_t c = lane; c < a.dim; c += 64) o[c] = 0.0f;
+    }
   }
 }
 
