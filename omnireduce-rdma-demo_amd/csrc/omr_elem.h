@@ -92,6 +92,19 @@ __device__ __forceinline__ void store_f32(T* p, const float (&v)[N]) {
   }
 }
 
+// store_f32 of rows that are written once and not read here again: whole 16-byte pieces go out non-temporally
+template <class T, int N>
+__device__ __forceinline__ void stream_f32(T* p, const float (&v)[N]) {
+  if constexpr (N * sizeof(T) == 16) {
+    vec_t<T, N> x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = static_cast<T>(v[i]);
+    __builtin_nontemporal_store(__builtin_bit_cast(v4f, x), reinterpret_cast<v4f*>(p));
+  } else {
+    store_f32<T, N>(p, v);
+  }
+}
+
 // Sum over the 64 lanes of a wave, in every lane (fixed order: the same bits every run).
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
