@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void k_embed(const T* table, uint32_t rows, ui
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[j][i] *= scale;
     }
-    store_f32<O, VEC>(out + static_cast<uint64_t>(tok[j]) * ostride + col[j], v[j]);
+    stream_f32<O, VEC>(out + static_cast<uint64_t>(tok[j]) * ostride + col[j], v[j]);
   }
 }
 

@@ -213,6 +213,12 @@ __device__ __forceinline__ int target_of(const GemmArgs<T>& a, uint32_t n) {
   return t >= 0 && t < a.vocab ? static_cast<int>(t) : -1;
 }
 
+// (maximum, sum of exp(. - maximum)) of two parts together; a part of nothing is (-inf, 0)
+__device__ __forceinline__ float2 join(float2 p, float2 q) {
+  const float top = fmaxf(p.x, q.x), from = top == -INFINITY ? 0.0f : top;
+  return make_float2(top, p.y * expf(p.x - from) + q.y * expf(q.x - from));
+}
+
 // out[0..3] (+)= v, of which the first `n` exist
 template <class O>
 __device__ __forceinline__ void put4(O* out, v4f v, uint32_t n, int accumulate, int wide) {
@@ -511,30 +517,136 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   }
 }
 
+// ---------------------------------------------------------------- few tokens
+//
+// The forward of up to 32 tokens is bound by reading the weight.  The tiles above keep one step of it in flight a CU
+// (16 KiB, 17 us for 16 tokens x 32000 x 1024 bf16); here each wave streams 16 rows of the vocabulary through a ring of
+// its own in LDS, kRing steps of 64 columns (2 KiB) deep, and waits for nobody: 80 KiB in flight a CU.  The hidden
+// states lie in LDS, 1024 / NF columns of them at a time.  (Rows loaded straight into the matrix instructions' registers
+// come in halves of a cache line: 19 us.)
+constexpr uint32_t kFewTokens = 32;
+constexpr int kRing = 5;
+
+template <class T, int NF>
+__global__ __launch_bounds__(256) void k_few(GemmArgs<T> a) {
+  constexpr uint32_t KC = 1024 / NF, kSteps = KC / kBK;  // columns of the hidden states in LDS; steps of them
+  __shared__ __attribute__((aligned(1024))) T ring[4][kRing][16 * kBK];
+  __shared__ __attribute__((aligned(1024))) T hid[kSteps][16 * NF * kBK];
+  __shared__ float2 part[4][16 * NF];
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4,
+                 r16 = lane & 15;
+  const uint32_t row0 = blockIdx.x * 64 + wave * 16;
+  // a load instruction's lane: row lane / 8 of eight, piece lane % 8 of its step's line, permuted as in Tile
+  const uint32_t lr = lane >> 3, lc = (lane & 7) ^ lr;
+  const char* w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = reinterpret_cast<const char*>(a.a.p + min(row0 + 8 * i + lr, a.vocab - 1) * a.a.ld + lc * 8);
+  auto load = [&](const char* src, const T* lds) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) T*)(lds))));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(src) : "memory");
+  };
+  const uint32_t steps = (a.k + kBK - 1) / kBK;
+  auto fetch = [&](uint32_t t) {  // step t into its place in the ring; past the end zeros, which nothing multiplies
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      load(t * kBK + lc * 8 < a.k ? w[i] + static_cast<uint64_t>(t) * kBK * sizeof(T)
+                                  : reinterpret_cast<const char*>(g_zero),
+           ring[wave][t % kRing] + 8 * i * kBK);
+  };
+  v4f acc[NF] = {};
+  for (uint32_t t = 0; t < kRing; ++t) fetch(t);
+  for (uint32_t t0 = 0; t0 < steps; t0 += kSteps) {
+    __syncthreads();  // (every wave is done with the columns before)
+    for (uint32_t q = wave; q < kSteps * 2 * NF; q += 4) {  // eight rows of a step each
+      const uint32_t t = t0 + q / (2 * NF), row = q % (2 * NF) * 8 + lr, k = t * kBK + lc * 8;
+      if (t >= steps) break;
+      load(k < a.k ? reinterpret_cast<const char*>(a.b.p + min(row, a.tokens - 1) * a.b.ld + k)
+                   : reinterpret_cast<const char*>(g_zero),
+           hid[q / (2 * NF)] + q % (2 * NF) * 8 * kBK);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (uint32_t t = t0; t < min(t0 + kSteps, steps); ++t) {
+      // two loads a step, kRing steps: this one's are there when those of the kRing - 1 behind it are all that is out
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * (kRing - 1)) : "memory");
+      const T* x = ring[wave][t % kRing];
+      const T* y = hid[t - t0];
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const uint32_t at = (r16 * 8 + ((sub * 4 + g) ^ (r16 & 7))) * 8;
+        const frag<T> f = *reinterpret_cast<const frag<T>*>(x + at);
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+          acc[j] = mma(f, *reinterpret_cast<const frag<T>*>(y + j * 16 * kBK + at), acc[j]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the step is read: its place may be loaded into
+      fetch(t + kRing);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < NF; ++j) {
+    const uint32_t tok = 16 * j + r16;
+    const int target = tok < a.tokens ? target_of(a, tok) : -1;
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t v = row0 + 4 * g + r;
+      if (v >= a.vocab) acc[j][r] = -INFINITY;
+      if (target >= 0 && static_cast<uint32_t>(target) == v) a.ztarget[tok] = acc[j][r];
+      top = fmaxf(top, acc[j][r]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float from = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum += __expf(acc[j][r] - from);
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (g == 0) part[wave][tok] = make_float2(top, sum);
+  }
+  __syncthreads();
+  if (threadIdx.x >= 16 * NF || threadIdx.x >= a.tokens) return;
+  float2 all = part[0][threadIdx.x];
+#pragma unroll
+  for (int v = 1; v < 4; ++v) all = join(all, part[v][threadIdx.x]);
+  reinterpret_cast<float2*>(a.stats)[static_cast<uint64_t>(threadIdx.x) * a.pieces + blockIdx.x] = all;
+}
+
 // ---------------------------------------------------------------- the small kernels around it
 
-// A wave a token: joins the pieces' maxima and sums.
-template <class T>
+// Joins the pieces' maxima and sums: WAVES waves a token, four pieces a lane in flight.
+template <class T, int WAVES>
 __global__ __launch_bounds__(256) void k_merge(GemmArgs<T> a, float* loss, float* lse) {
-  const uint32_t tok = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (tok >= a.tokens) return;
-  const float2* s = reinterpret_cast<const float2*>(a.stats) + static_cast<uint64_t>(tok) * a.pieces;
-  float top = -INFINITY, sum = 0.0f;
-  for (uint32_t p = lane; p < a.pieces; p += 64) {
-    const float2 v = s[p];
-    const float up = fmaxf(top, v.x), from = up == -INFINITY ? 0.0f : up;
-    sum = sum * expf(top - from) + v.y * expf(v.x - from);
-    top = up;
+  __shared__ float2 part[4];
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t tok = blockIdx.x * (4 / WAVES) + wave / WAVES;
+  float2 all = make_float2(-INFINITY, 0.0f);
+  if (tok < a.tokens) {
+    const float2* s = reinterpret_cast<const float2*>(a.stats) + static_cast<uint64_t>(tok) * a.pieces;
+    for (uint32_t p = (wave % WAVES) * 64 + lane; p < a.pieces; p += 4 * 64 * WAVES) {
+      float2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = p + i * 64 * WAVES < a.pieces ? s[p + i * 64 * WAVES] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) all = join(all, v[i]);
+    }
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float ot = __shfl_xor(top, d), os = __shfl_xor(sum, d);
-    const float up = fmaxf(top, ot), from = up == -INFINITY ? 0.0f : up;
-    sum = sum * expf(top - from) + os * expf(ot - from);
-    top = up;
+  for (int d = 32; d; d >>= 1) all = join(all, make_float2(__shfl_xor(all.x, d), __shfl_xor(all.y, d)));
+  if constexpr (WAVES > 1) {
+    if (lane == 0) part[wave] = all;
+    __syncthreads();
+    if (wave % WAVES != 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) all = join(all, part[wave + w]);
   }
-  if (lane != 0) return;
-  const float l = top + logf(sum);
+  if (lane != 0 || tok >= a.tokens) return;
+  const float l = all.x + logf(all.y);
   lse[tok] = l;
   loss[tok] = target_of(a, tok) >= 0 ? l - a.ztarget[tok] : 0.0f;
 }
@@ -771,9 +883,24 @@ int omr_vocab_loss(const void* hidden, uint64_t hidden_stride, const void* weigh
     a.tokens = static_cast<uint32_t>(tokens);
     a.ztarget = reinterpret_cast<float*>(ws + sp.rest);
     a.stats = reinterpret_cast<float*>(ws + sp.rest + up(tokens * 4, 256));
-    a.pieces = static_cast<uint32_t>(big ? ceil_div(vocab, 256) * 2 : ceil_div(vocab, 128) * 2);
-    if (const int rc = launch<T, kStats>(a, a.vocab, a.tokens, big, S(stream))) return rc;
-    k_merge<T><<<static_cast<unsigned>(ceil_div(tokens, 4)), 256, 0, S(stream)>>>(a, loss, lse);
+    if (tokens <= kFewTokens) {
+      a.pieces = static_cast<uint32_t>(ceil_div(vocab, 64));
+      const unsigned grid = a.pieces;
+      if (grid > (1u << 24) - 1) return efail("vocab_loss: too many tiles for one call");
+      if (tokens <= 16)
+        k_few<T, 1><<<grid, 256, 0, S(stream)>>>(a);
+      else
+        k_few<T, 2><<<grid, 256, 0, S(stream)>>>(a);
+      if (const int rc = elaunch("omr_vocab_loss")) return rc;
+    } else {
+      a.pieces = static_cast<uint32_t>(big ? ceil_div(vocab, 256) * 2 : ceil_div(vocab, 128) * 2);
+      if (const int rc = launch<T, kStats>(a, a.vocab, a.tokens, big, S(stream))) return rc;
+    }
+    // four waves a token where there are not enough tokens to fill the CUs
+    if (tokens <= 1024)
+      k_merge<T, 4><<<static_cast<unsigned>(tokens), 256, 0, S(stream)>>>(a, loss, lse);
+    else
+      k_merge<T, 1><<<static_cast<unsigned>(ceil_div(tokens, 4)), 256, 0, S(stream)>>>(a, loss, lse);
     return elaunch("omr_vocab_loss");
   };
   return dtype == OMR_BF16 ? go(__bf16{}) : go(_Float16{});

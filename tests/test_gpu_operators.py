@@ -369,7 +369,7 @@ def loss_ref(h, w, t, off):
     return z, lse, loss, tol
 
 
-LOSS_SIZES = [(1, 1, 8), (1, 7, 1), (3, 300, 72), (17, 129, 264), (64, 1000, 128), (130, 257, 61), (257, 2000, 200),
+LOSS_SIZES = [(1, 1, 8), (1, 7, 1), (3, 300, 72), (16, 70, 2120), (17, 129, 264), (32, 200, 1000), (33, 200, 64), (64, 1000, 128), (130, 257, 61), (257, 2000, 200),
               (300, 5003, 520), (1025, 700, 96), (16, 40000, 64), (700, 70000, 64), (2048, 8192, 256), (5, 256, 4096)]
 
 
