@@ -61,17 +61,19 @@ inline auto with_dtype(int dtype, F&& fn) {
 template <class T, int N>
 using vec_t = T __attribute__((ext_vector_type(N)));
 
-// N consecutive elements as fp32 (exact for every element type), and back with one round-to-nearest-even.  The caller
-// guarantees alignment to N * sizeof(T), at most 16 bytes.
+// N consecutive elements as fp32 (exact for every element type), and back with one round-to-nearest-even.  Rows may
+// begin at any element: whole vectors are loaded and stored at any alignment (one instruction up to 16 bytes, as fast as
+// an aligned one where the address happens to be).
+template <class T, int N>
+using any_vec = vec_t<T, N> __attribute__((aligned(sizeof(T)), may_alias));
+
 template <class T, int N>
 __device__ __forceinline__ void load_f32(const T* p, float (&v)[N]) {
-  if constexpr (N == 1) {
-    v[0] = static_cast<float>(p[0]);
-  } else if constexpr (N * sizeof(T) > 16) {
+  if constexpr (N * sizeof(T) > 16) {
     load_f32<T, N / 2>(p, reinterpret_cast<float(&)[N / 2]>(v[0]));
     load_f32<T, N / 2>(p + N / 2, reinterpret_cast<float(&)[N / 2]>(v[N / 2]));
   } else {
-    const vec_t<T, N> x = *reinterpret_cast<const vec_t<T, N>*>(p);
+    const vec_t<T, N> x = *reinterpret_cast<const any_vec<T, N>*>(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = static_cast<float>(x[i]);
   }
@@ -79,30 +81,59 @@ __device__ __forceinline__ void load_f32(const T* p, float (&v)[N]) {
 
 template <class T, int N>
 __device__ __forceinline__ void store_f32(T* p, const float (&v)[N]) {
-  if constexpr (N == 1) {
-    p[0] = static_cast<T>(v[0]);
-  } else if constexpr (N * sizeof(T) > 16) {
+  if constexpr (N * sizeof(T) > 16) {
     store_f32<T, N / 2>(p, reinterpret_cast<const float(&)[N / 2]>(v[0]));
     store_f32<T, N / 2>(p + N / 2, reinterpret_cast<const float(&)[N / 2]>(v[N / 2]));
   } else {
     vec_t<T, N> x;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = static_cast<T>(v[i]);
-    *reinterpret_cast<vec_t<T, N>*>(p) = x;
+    *reinterpret_cast<any_vec<T, N>*>(p) = x;
   }
 }
 
 // store_f32 of rows that are written once and not read here again: whole 16-byte pieces go out non-temporally
 template <class T, int N>
 __device__ __forceinline__ void stream_f32(T* p, const float (&v)[N]) {
-  if constexpr (N * sizeof(T) == 16) {
+  if constexpr (N * sizeof(T) > 16) {
+    stream_f32<T, N / 2>(p, reinterpret_cast<const float(&)[N / 2]>(v[0]));
+    stream_f32<T, N / 2>(p + N / 2, reinterpret_cast<const float(&)[N / 2]>(v[N / 2]));
+  } else {
     vec_t<T, N> x;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = static_cast<T>(v[i]);
-    __builtin_nontemporal_store(__builtin_bit_cast(v4f, x), reinterpret_cast<v4f*>(p));
-  } else {
-    store_f32<T, N>(p, v);
+    __builtin_nontemporal_store(x, reinterpret_cast<any_vec<T, N>*>(p));
   }
+}
+
+// The same for a piece at the end of a row, of which the first `n` elements exist (the others are read as 0)
+template <class T, int N>
+__device__ __forceinline__ void load_some(const T* p, uint32_t n, float (&v)[N]) {
+  if (n >= N) {
+    load_f32<T, N>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = static_cast<uint32_t>(i) < n ? static_cast<float>(p[i]) : 0.0f;
+  }
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store_some(T* p, uint32_t n, const float (&v)[N]) {
+  if (n >= N) {
+    store_f32<T, N>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (static_cast<uint32_t>(i) < n) p[i] = static_cast<T>(v[i]);
+  }
+}
+
+template <class T, int N>
+__device__ __forceinline__ void stream_some(T* p, uint32_t n, const float (&v)[N]) {
+  if (n >= N)
+    stream_f32<T, N>(p, v);
+  else
+    store_some<T, N>(p, n, v);
 }
 
 // Sum over the 64 lanes of a wave, in every lane (fixed order: the same bits every run).

@@ -204,7 +204,7 @@ struct GemmArgs {
   const uint32_t *start, *perm;  // kWeight: the tokens by target
   void* out;
   uint64_t ostride;
-  int out_f32, accumulate, wide;  // wide: out takes 4 elements at a time
+  int out_f32, accumulate;
 };
 
 template <class T>
@@ -221,22 +221,12 @@ __device__ __forceinline__ float2 join(float2 p, float2 q) {
 
 // out[0..3] (+)= v, of which the first `n` exist
 template <class O>
-__device__ __forceinline__ void put4(O* out, v4f v, uint32_t n, int accumulate, int wide) {
-  if (wide && n >= 4) {
-    float f[4];
-    if (accumulate) {
-      load_f32<O, 4>(out, f);
+__device__ __forceinline__ void put4(O* out, v4f v, uint32_t n, int accumulate) {
+  float f[4] = {};
+  if (accumulate) load_some<O, 4>(out, n, f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = f[i] + v[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = v[i];
-    store_f32<O, 4>(out, f);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (static_cast<uint32_t>(i) < n) out[i] = static_cast<O>(accumulate ? static_cast<float>(out[i]) + v[i] : v[i]);
+  for (int i = 0; i < 4; ++i) f[i] = accumulate ? f[i] + v[i] : v[i];
+  store_some<O, 4>(out, n, f);
 }
 
 template <class T, int EPI, int BM, int BN, int WM, int WN>
@@ -476,9 +466,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
           v += lost * target_row(c);
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = scale == 0.0f ? 0.0f : v[r] * scale;
-          put4<T>(static_cast<T*>(a.out) + static_cast<uint64_t>(tok) * a.ostride + c, v, have, 0, a.wide);
+          put4<T>(static_cast<T*>(a.out) + static_cast<uint64_t>(tok) * a.ostride + c, v, have, 0);
         } else {
-          put4<float>(sum, v, have, 0, a.dim % 4 == 0);
+          put4<float>(sum, v, have, 0);
         }
       }
     }
@@ -509,9 +499,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
         if (c >= a.dim) continue;
         const v4f v = acc[i][j] * scale;
         if (a.out_f32)
-          put4<float>(static_cast<float*>(a.out) + o + c, v, a.dim - c, a.accumulate, a.wide);
+          put4<float>(static_cast<float*>(a.out) + o + c, v, a.dim - c, a.accumulate);
         else
-          put4<T>(static_cast<T*>(a.out) + o + c, v, a.dim - c, a.accumulate, a.wide);
+          put4<T>(static_cast<T*>(a.out) + o + c, v, a.dim - c, a.accumulate);
       }
     }
   }
@@ -676,34 +666,24 @@ __global__ __launch_bounds__(1024) void k_scales(GemmArgs<T> a, const float* gra
   *amax = m;
 }
 
-// Rows copied into whole 16-byte pieces [rows][pdim], zeros behind dim.  With rowscale: each row times its share of the
-// largest grad_loss, and zeros for tokens without a target, whatever they hold.
+// Rows copied into whole 16-byte pieces [rows][pdim], zeros behind dim; 2^lpr_log lanes a row.  With rowscale: each row
+// times its share of the largest grad_loss, and zeros for tokens without a target, whatever they hold.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const T* src, uint64_t stride, uint32_t rows, uint32_t dim, uint32_t pdim,
-                                              const float* rowscale, const float* amax, T* dst, int wide) {
-  const uint32_t per = pdim / 8;
-  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const uint64_t row = i / per;
+                                              uint32_t lpr_log, const float* rowscale, const float* amax, T* dst) {
+  const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x) >> lpr_log;
   if (row >= rows) return;
-  const uint32_t c = static_cast<uint32_t>(i - row * per) * 8;
-  const T* s = src + row * stride + c;
-  float v[8];
   float by = 1.0f;
   if (rowscale != nullptr) by = rowscale[row] == 0.0f ? 0.0f : rowscale[row] * kGScale / *amax;
-  if (by == 0.0f) {
+  for (uint32_t c = (threadIdx.x & ((1u << lpr_log) - 1)) * 8; c < pdim; c += 8u << lpr_log) {
+    float v[8] = {};
+    if (by != 0.0f) {
+      load_some<T, 8>(src + row * stride + c, dim - c, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-  } else {
-    if (wide) {
-      load_f32<T, 8>(s, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = c + k < dim ? static_cast<float>(s[k]) : 0.0f;
+      for (int k = 0; k < 8; ++k) v[k] *= by;
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= by;
+    store_f32<T, 8>(dst + row * pdim + c, v);
   }
-  store_f32<T, 8>(dst + row * pdim + c, v);
 }
 
 // grad_hidden = factor * (the parts' sums, in order)
@@ -804,12 +784,13 @@ template <class T>
 int pack_rows(const void* src, uint64_t stride, uint64_t rows, uint32_t dim, const float* rowscale, const float* amax,
               T* dst, hipStream_t stream) {
   const uint32_t pdim = static_cast<uint32_t>(up(dim, 8));
-  const uint64_t blocks = ceil_div(rows * (pdim / 8), 256);
-  if (blocks >= (1u << 24)) return efail("vocab_loss: too many elements to lay out in one call");
-  const int wide = dim % 8 == 0 && stride % 8 == 0 && aligned(src, 16);
+  uint32_t lpr_log = 0;
+  while (lpr_log < 6 && (8u << lpr_log) < pdim) ++lpr_log;
+  const uint64_t blocks = ceil_div(rows, 256u >> lpr_log);
+  if (blocks >= (1u << 24)) return efail("vocab_loss: too many rows to lay out in one call");
   k_pack<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T*>(src), stride,
-                                                               static_cast<uint32_t>(rows), dim, pdim, rowscale, amax,
-                                                               dst, wide);
+                                                               static_cast<uint32_t>(rows), dim, pdim, lpr_log, rowscale,
+                                                               amax, dst);
   return elaunch("omr_vocab_loss (layout)");
 }
 
@@ -1008,7 +989,6 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
         x.last = done && splits == 1;
         x.out = grad_hidden;
         x.ostride = grad_hidden_stride;
-        x.wide = grad_hidden_stride % 4 == 0 && aligned(grad_hidden, 8);
         if (const int rc = launch<T, kHidden>(x, dim, x.tokens, use_big(dim, tokens), S(stream))) return rc;
         if (done && splits > 1) {
           x.splits = splits;
@@ -1028,7 +1008,6 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
         y.ostride = grad_weight_stride;
         y.out_f32 = grad_weight_dtype == OMR_F32;
         y.accumulate = accumulate != 0;
-        y.wide = grad_weight_stride % 4 == 0 && aligned(grad_weight, y.out_f32 ? 16 : 8);
         if (const int rc = launch<T, kWeight>(y, dim, cols, use_big(dim, cols), S(stream))) return rc;
       }
     }

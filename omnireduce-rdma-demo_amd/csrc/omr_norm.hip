@@ -54,53 +54,46 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
   return v;
 }
 
-// A lane's columns: VEC consecutive ones of every piece j
-template <int WPR, int VEC>
-__device__ __forceinline__ uint32_t col_of(int j) {
-  const uint32_t t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
-  return (static_cast<uint32_t>(j) * 64 * WPR + t) * VEC;
-}
-
-// VEC elements as they lie in memory
+// VEC elements as they lie in memory, at any alignment; of a row's last piece the first n
 template <class T, int VEC>
-struct alignas(VEC * sizeof(T)) Piece {
-  T v[VEC];
-};
+struct Piece {
+  vec_t<T, VEC> v;
 
-template <class T, int WPR, int VEC>
-__device__ __forceinline__ void load_row(const T* p, uint32_t dim, float (&v)[kCols / VEC][VEC], float other) {
-#pragma unroll
-  for (int j = 0; j < kCols / VEC; ++j) {
-    const uint32_t c = col_of<WPR, VEC>(j);
-    if (c < dim) {
-      load_f32<T, VEC>(p + c, v[j]);
+  __device__ __forceinline__ void load(const T* p, uint32_t n) {
+    if (n >= VEC) {
+      v = *reinterpret_cast<const any_vec<T, VEC>*>(p);
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = other;
+      for (int i = 0; i < VEC; ++i) v[i] = static_cast<uint32_t>(i) < n ? p[i] : static_cast<T>(0.0f);
     }
   }
+};
+
+// Columns there are from c on: all VEC of them where rows are whole pieces (END false), known when compiling
+template <int VEC, bool END>
+__device__ __forceinline__ uint32_t have(uint32_t dim, uint32_t c) {
+  return END ? dim - c : VEC;
 }
 
-template <class T, class P, int VEC, int WPR>
+template <class T, class P, int WPR, bool END>
 __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) {
-  constexpr int NV = kCols / VEC, RPB = WPR == 1 ? 4 : 1;
+  constexpr int VEC = 16 / sizeof(T), NV = kCols / VEC, RPB = WPR == 1 ? 4 : 1;
   __shared__ float lds[2][WPR];
+  // a lane's columns: VEC consecutive ones of every piece j
+  const uint32_t t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  auto col = [&](int j) { return (static_cast<uint32_t>(j) * 64 * WPR + t) * VEC; };
   float w[NV][VEC], b[NV][VEC];
-  if (a.w != nullptr) {
-    load_row<P, WPR, VEC>(static_cast<const P*>(a.w), a.dim, w, 0.0f);
-  } else {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) w[j][i] = 1.0f;
-  }
-  if (a.b != nullptr) {
-    load_row<P, WPR, VEC>(static_cast<const P*>(a.b), a.dim, b, 0.0f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) b[j][i] = 0.0f;
+    for (int i = 0; i < VEC; ++i) {
+      w[j][i] = 1.0f;
+      b[j][i] = 0.0f;
+    }
+    if (col(j) >= a.dim) continue;
+    const uint32_t n = have<VEC, END>(a.dim, col(j));
+    if (a.w != nullptr) load_some<P, VEC>(static_cast<const P*>(a.w) + col(j), n, w[j]);
+    if (a.b != nullptr) load_some<P, VEC>(static_cast<const P*>(a.b) + col(j), n, b[j]);
   }
   // the next row is on its way while this one is worked on
   Piece<T, VEC> ahead[NV];
@@ -108,8 +101,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
     const T* p = static_cast<const T*>(a.x) + row * a.xstride;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const uint32_t c = col_of<WPR, VEC>(j);
-      if (c < a.dim) ahead[j] = *reinterpret_cast<const Piece<T, VEC>*>(p + c);
+      if (col(j) < a.dim) ahead[j].load(p + col(j), have<VEC, END>(a.dim, col(j)));
     }
   };
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * RPB;
@@ -120,7 +112,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = col_of<WPR, VEC>(j) < a.dim ? static_cast<float>(ahead[j].v[i]) : 0.0f;
+      for (int i = 0; i < VEC; ++i) v[j][i] = col(j) < a.dim ? static_cast<float>(ahead[j].v[i]) : 0.0f;
     if (row + step < a.rows) fetch(row + step);
     float s = 0.0f;
 #pragma unroll
@@ -131,10 +123,10 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
     float q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (col_of<WPR, VEC>(j) < a.dim) {
+      if (col(j) < a.dim) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          v[j][i] -= mean;
+          v[j][i] = !END || col(j) + i < a.dim ? v[j][i] - mean : 0.0f;
           q += v[j][i] * v[j][i];
         }
       }
@@ -143,11 +135,10 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
     T* out = static_cast<T*>(a.out) + row * a.ostride;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const uint32_t c = col_of<WPR, VEC>(j);
-      if (c < a.dim) {
+      if (col(j) < a.dim) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * rstd * w[j][i] + b[j][i];
-        stream_f32<T, VEC>(out + c, v[j]);
+        stream_some<T, VEC>(out + col(j), have<VEC, END>(a.dim, col(j)), v[j]);
       }
     }
     if (WPR == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) {
@@ -159,36 +150,31 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
 
 // A workgroup of 8 waves holds 8 / WPR rows at a time (WPR 16: one row of 16 waves), in lockstep where a row is more
 // than a wave.
-template <class T, class P, int VEC, int WPR>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void k_norm_grad(NormArgs a) {
-  constexpr int NV = kCols / VEC, RPB = WPR == 16 ? 1 : 8 / WPR, WAVES = RPB * WPR, NT = 64 * WAVES;
+template <class T, class P, int WPR, bool END>
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 512, 4) void k_norm_grad(NormArgs a) {
+  constexpr int VEC = 16 / sizeof(T), NV = kCols / VEC, RPB = WPR == 16 ? 1 : 8 / WPR, WAVES = RPB * WPR, NT = 64 * WAVES;
   __shared__ float lds[2][2][WAVES];
   __shared__ float sum[RPB > 1 ? WAVES * 64 * kCols : 1];
   const uint32_t wave = threadIdx.x >> 6, slot = wave / WPR, t = threadIdx.x - slot * 64 * WPR;
   auto col = [&](int j) { return (static_cast<uint32_t>(j) * 64 * WPR + t) * VEC; };
   float dw[NV][VEC] = {}, db[NV][VEC] = {};
-  // Rows of 16-bit elements in whole pieces: the next row is on its way while this one is worked on, and the weight waits
-  // in LDS (a lane's columns together), since with both in registers a CU holds half the waves (58 us against 49 at
-  // 16384 x 2048).  Else (fp32 has no registers for a row ahead) the weight is held in registers.
-  constexpr bool kAhead = VEC * sizeof(T) == 16 && sizeof(T) == 2 && WPR <= 8;
-  __shared__ __attribute__((aligned(16))) float wl[kAhead ? 64 * WPR * kCols : 4];
-  float wr[kAhead ? 1 : NV][VEC];
-  if (!kAhead || slot == 0) {
+  // Rows of 16-bit elements: the next row is on its way while this one is worked on (fp32 has no registers for that).
+  // The weight waits in LDS (a lane's columns together): with it in registers a CU holds half the waves (58 us against 49
+  // at 16384 x 2048 bf16).
+  constexpr bool kAhead = sizeof(T) == 2 && WPR <= 8;
+  __shared__ __attribute__((aligned(16))) float w[64 * WPR * kCols];
+  if (slot == 0) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float f[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) f[i] = 1.0f;
-      if (a.w != nullptr && col(j) < a.dim) load_f32<P, VEC>(static_cast<const P*>(a.w) + col(j), f);
-      if constexpr (kAhead) {
-        store_f32<float, VEC>(&wl[(j * 64 * WPR + t) * VEC], f);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) wr[j][i] = f[i];
-      }
+      if (a.w != nullptr && col(j) < a.dim)
+        load_some<P, VEC>(static_cast<const P*>(a.w) + col(j), have<VEC, END>(a.dim, col(j)), f);
+      store_f32<float, VEC>(&w[(j * 64 * WPR + t) * VEC], f);
     }
   }
-  if constexpr (kAhead) __syncthreads();
+  __syncthreads();
   Piece<T, VEC> xa[NV], da[NV];
   auto fetch = [&](uint64_t row) {
     if (row >= a.rows) return;
@@ -197,8 +183,8 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void k_norm_grad(NormArgs a
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (col(j) < a.dim) {
-        xa[j] = *reinterpret_cast<const Piece<T, VEC>*>(x + col(j));
-        da[j] = *reinterpret_cast<const Piece<T, VEC>*>(dy + col(j));
+        xa[j].load(x + col(j), have<VEC, END>(a.dim, col(j)));
+        da[j].load(dy + col(j), have<VEC, END>(a.dim, col(j)));  // (zeros behind a row's end add nothing below)
       }
   };
   int flip = 0;
@@ -225,12 +211,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void k_norm_grad(NormArgs a
       for (int j = 0; j < NV; ++j) {
         if (col(j) < a.dim) {
           float wj[VEC];
-          if constexpr (kAhead) {
-            load_f32<float, VEC>(&wl[(j * 64 * WPR + t) * VEC], wj);
-          } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) wj[i] = wr[j][i];
-          }
+          load_f32<float, VEC>(&w[(j * 64 * WPR + t) * VEC], wj);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             const float xh = (v[j][i] - mean) * rstd;
@@ -271,7 +252,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void k_norm_grad(NormArgs a
       if (col(j) < a.dim) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) g[j][i] = (g[j][i] - s1 - v[j][i] * s2) * rstd;
-        stream_f32<T, VEC>(out + col(j), g[j]);
+        stream_some<T, VEC>(out + col(j), have<VEC, END>(a.dim, col(j)), g[j]);
       }
     }
   }
@@ -300,7 +281,8 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512) void k_norm_grad(NormArgs a
       for (int j = 0; j < NV; ++j)
         if (col(j) < a.dim)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) part[which * a.dim + col(j) + i] = mine[j][i];
+          for (int i = 0; i < VEC; ++i)
+            if (!END || col(j) + i < a.dim) part[which * a.dim + col(j) + i] = mine[j][i];
     }
   }
 }
@@ -429,18 +411,16 @@ uint32_t grad_blocks(uint64_t rows, uint32_t dim) {
   return static_cast<uint32_t>(want < kGradBlocks ? want : kGradBlocks);
 }
 
-// fn(VEC, WPR) as integral constants
-template <int W, class F>
-int with_shape(bool wide, int wpr, F&& fn) {
-  auto vec = [&](auto p) {
-    return wide ? fn(std::integral_constant<int, W>{}, p) : fn(std::integral_constant<int, 1>{}, p);
-  };
+// fn(WPR, whether rows end inside a piece) as integral constants
+template <class F>
+int with_shape(bool end, int wpr, F&& fn) {
+  auto ends = [&](auto p) { return end ? fn(p, std::true_type{}) : fn(p, std::false_type{}); };
   switch (wpr) {
-    case 1: return vec(std::integral_constant<int, 1>{});
-    case 2: return vec(std::integral_constant<int, 2>{});
-    case 4: return vec(std::integral_constant<int, 4>{});
-    case 8: return vec(std::integral_constant<int, 8>{});
-    default: return vec(std::integral_constant<int, 16>{});
+    case 1: return ends(std::integral_constant<int, 1>{});
+    case 2: return ends(std::integral_constant<int, 2>{});
+    case 4: return ends(std::integral_constant<int, 4>{});
+    case 8: return ends(std::integral_constant<int, 8>{});
+    default: return ends(std::integral_constant<int, 16>{});
   }
 }
 
@@ -487,15 +467,11 @@ int omr_layer_norm(const void* x, int dtype, uint64_t rows, uint32_t dim, uint64
         k_norm_any<T, P><<<grid, 64 * kAnyWaves, 0, S(stream)>>>(a);
         return elaunch("omr_layer_norm");
       }
-      constexpr int W = 16 / sizeof(T);
-      const bool wide = dim % W == 0 && x_stride % W == 0 && out_stride % W == 0 && aligned(x, 16) &&
-                        aligned(out, 16) && aligned(weight, W * sizeof(P) < 16 ? W * sizeof(P) : 16) &&
-                        aligned(bias, W * sizeof(P) < 16 ? W * sizeof(P) : 16);
-      return with_shape<W>(wide, wpr, [&](auto vec, auto waves) {
-        constexpr int VEC = decltype(vec)::value, WPR = decltype(waves)::value;
+      return with_shape(dim % (16 / sizeof(T)) != 0, wpr, [&](auto waves, auto end) {
+        constexpr int WPR = decltype(waves)::value;
         const uint64_t want = WPR == 1 ? ceil_div(rows, 4) : rows;
         const uint64_t most = WPR <= 4 ? 1024 : 4096 / WPR;
-        k_norm<T, P, VEC, WPR><<<static_cast<unsigned>(want < most ? want : most), WPR == 1 ? 256 : 64 * WPR, 0,
+        k_norm<T, P, WPR, decltype(end)::value><<<static_cast<unsigned>(want < most ? want : most), WPR == 1 ? 256 : 64 * WPR, 0,
                                  S(stream)>>>(a);
         return elaunch("omr_layer_norm");
       });
@@ -556,13 +532,9 @@ int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* 
         k_norm_dx_any<T, P><<<static_cast<unsigned>(rows < 2048 ? rows : 2048), 64 * kAnyWaves, 0, S(stream)>>>(a);
         return elaunch("omr_layer_norm_grad");
       }
-      constexpr int W = 16 / sizeof(T);
-      const bool wide = dim % W == 0 && x_stride % W == 0 && grad_stride % W == 0 && grad_x_stride % W == 0 &&
-                        aligned(x, 16) && aligned(grad_out, 16) && aligned(grad_x, 16) &&
-                        aligned(weight, W * sizeof(P) < 16 ? W * sizeof(P) : 16);
-      return with_shape<W>(wide, wpr, [&](auto vec, auto waves) {
-        constexpr int VEC = decltype(vec)::value, WPR = decltype(waves)::value;
-        k_norm_grad<T, P, VEC, WPR><<<blocks, WPR == 16 ? 1024 : 512, 0, S(stream)>>>(a);
+      return with_shape(dim % (16 / sizeof(T)) != 0, wpr, [&](auto waves, auto end) {
+        constexpr int WPR = decltype(waves)::value;
+        k_norm_grad<T, P, WPR, decltype(end)::value><<<blocks, WPR == 16 ? 1024 : 512, 0, S(stream)>>>(a);
         return elaunch("omr_layer_norm_grad");
       });
     };
