@@ -229,11 +229,49 @@ __device__ __forceinline__ void put4(O* out, v4f v, uint32_t n, int accumulate) 
   store_some<O, 4>(out, n, f);
 }
 
+// A wave's MW x NW results as 16-bit elements, stored in whole 16-byte pieces by way of its own part of LDS: the matrix
+// instruction leaves a lane four consecutive m of one n, and stores of those are segments of 32 bytes.  quad(i, j): the
+// four at m = 16 i + 4 (lane / 16), n = 16 j + lane % 16; row(n, m, piece): eight consecutive m of an n.  (The pieces of a
+// row of LDS are permuted by its number, for the banks.)
+template <class T, int MW, int NW, class Q, class R>
+__device__ __forceinline__ void put_tile(T* stage, Q&& quad, R&& row) {
+  constexpr int CH = MW / 8;
+  const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < NW / 16; ++j)
+#pragma unroll
+    for (int i = 0; i < MW / 16; ++i) {
+      const uint32_t n = 16 * j + (lane & 15), c = (2 * i + (g >> 1)) ^ (n & (CH - 1));
+      *reinterpret_cast<vec_t<T, 4>*>(stage + (n * CH + c) * 8 + (g & 1) * 4) = quad(i, j);
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 4
+  for (int q = 0; q < NW * CH / 64; ++q) {
+    const uint32_t n = (q * 64 + lane) / CH, c = lane % CH;
+    row(n, c * 8, *reinterpret_cast<const vec_t<T, 8>*>(stage + (n * CH + (c ^ (n & (CH - 1)))) * 8));
+  }
+}
+
+// eight elements of which the first n exist; they are not read here again
+template <class T>
+__device__ __forceinline__ void stream8(T* p, uint32_t n, const vec_t<T, 8>& v) {
+  if (n >= 8) {
+    __builtin_nontemporal_store(v, reinterpret_cast<any_vec<T, 8>*>(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (static_cast<uint32_t>(i) < n) p[i] = v[i];
+  }
+}
+
 template <class T, int EPI, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   constexpr int NT = 64 * WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
   constexpr bool AC = EPI == kHidden || EPI == kWeight, BC = EPI == kWeight;
-  __shared__ __attribute__((aligned(1024))) T la[2][BM * kBK], lb[2][BN * kBK];
+  __shared__ __attribute__((aligned(1024))) T lds[2 * (BM + BN) * kBK];
+  auto la = [&](uint32_t t) { return lds + (t & 1) * (BM * kBK); };  // step t's buffers
+  auto lb = [&](uint32_t t) { return lds + 2 * BM * kBK + (t & 1) * (BN * kBK); };
+  static_assert(BM * BN <= 2 * (BM + BN) * kBK, "the results pass through LDS as 16-bit elements");
   // Workgroup ids go round the 8 XCDs: give each XCD a contiguous stretch of tiles, and walk the stretch in groups of 8
   // tile rows, so the tiles that run together on an XCD share operands in its L2.
   uint32_t id = blockIdx.x;
@@ -275,7 +313,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
     __builtin_amdgcn_sched_barrier(0);
   };
   auto fetch = [&](uint32_t t) {  // a whole tile at once
-    const uint32_t toa = ta.place(la[t & 1]), tob = tb.place(lb[t & 1]);
+    const uint32_t toa = ta.place(la(t)), tob = tb.place(lb(t));
     if (t < full) {
 #pragma unroll
       for (int i = 0; i < Tile<T, BM, NT, AC>::kPieces; ++i) ta.load(i, toa);
@@ -291,8 +329,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   // The products of one half, with the reads of the other from step t's buffer; with `loads` also the loads of step
   // t + 1's tile.  (The reads end two groups early: the barrier behind waits for them.)
   auto half = [&](int h, uint32_t t, bool loads) {
-    const T *ca = la[t & 1], *cb = lb[t & 1];
-    const uint32_t toa = ta.place(la[(t + 1) & 1]), tob = tb.place(lb[(t + 1) & 1]);
+    const T *ca = la(t), *cb = lb(t);
+    const uint32_t toa = ta.place(la(t + 1)), tob = tb.place(lb(t + 1));
     constexpr int kReads = MF + NF, kOver = MF - 2;
     fa.touch();
     fb.touch();
@@ -329,9 +367,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   uint32_t t = 0;
   if (full > 2) {
 #pragma unroll
-    for (int j = 0; j < NF; ++j) y[0][j] = fb.get(lb[0], 0, j);
+    for (int j = 0; j < NF; ++j) y[0][j] = fb.get(lb(0), 0, j);
 #pragma unroll
-    for (int i = 0; i < MF; ++i) x[0][i] = fa.get(la[0], 0, i);
+    for (int i = 0; i < MF; ++i) x[0][i] = fa.get(la(0), 0, i);
     do {
       half(0, t, false);
       meet();
@@ -345,10 +383,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
       fa.touch();
       fb.touch();
 #pragma unroll
-      for (int j = 0; j < NF; ++j) y[0][j] = fb.get(lb[t & 1], h, j);
+      for (int j = 0; j < NF; ++j) y[0][j] = fb.get(lb(t), h, j);
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
-        x[0][i] = fa.get(la[t & 1], h, i);
+        x[0][i] = fa.get(la(t), h, i);
 #pragma unroll
         for (int j = 0; j < NF; ++j) acc[i][j] = mma(x[0][i], y[0][j], acc[i][j]);
       }
@@ -358,66 +396,80 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   }
 
   // acc[i][j][r] = C[m + 16 i + r, n + 16 j]
-  const uint32_t m = m0 + wm * (BM / WM) + 4 * (lane >> 4), n = n0 + wn * (BN / WN) + (lane & 15);
-  if constexpr (EPI == kStats || EPI == kGrad) {
+  constexpr int MW = BM / WM, NW = BN / WN;
+  const uint32_t mw = m0 + wm * MW, nw = n0 + wn * NW;
+  const uint32_t m = mw + 4 * (lane >> 4), n = nw + (lane & 15);
+  T* const stage = lds + wave * (MW * NW);
+  if constexpr (EPI == kStats) {
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
       const uint32_t tok = n + 16 * j;
-      const bool real = tok < a.tokens;
-      const int target = real ? target_of(a, tok) : -1;
-      const int at = target - static_cast<int>(a.v0 + m);  // the target's place among this lane's rows
-      if constexpr (EPI == kStats) {
-        float top = -INFINITY, z = 0.0f;
-        if (a.v0 + m0 + BM > a.vocab) {  // rows past the vocabulary do not count
-#pragma unroll
-          for (int i = 0; i < MF; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (a.v0 + m + 16 * i + r >= a.vocab) acc[i][j][r] = -INFINITY;
-        }
+      const int target = tok < a.tokens ? target_of(a, tok) : -1;
+      const int at = target - static_cast<int>(m);  // the target's place among this lane's rows
+      if (m0 + BM > a.vocab) {  // rows past the vocabulary do not count
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float from = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f;
+          for (int r = 0; r < 4; ++r)
+            if (m + 16 * i + r >= a.vocab) acc[i][j][r] = -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += __expf(acc[i][j][r] - from);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      const bool here = target >= 0 && at >= 0 && at < 16 * MF && (at & 15) < 4;
+      if (__ballot(here)) {
+        float z = 0.0f;
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sum += __expf(acc[i][j][r] - from);
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        const bool here = target >= 0 && at >= 0 && at < 16 * MF && (at & 15) < 4;
-        if (__ballot(here)) {
+          for (int r = 0; r < 4; ++r)
+            if (at == 16 * i + r) z = acc[i][j][r];
+        if (here) a.ztarget[tok] = z;
+      }
+      if (tok < a.tokens && lane < 16) {
+        float* s = a.stats + (static_cast<uint64_t>(tok) * a.pieces + mw / MW) * 2;
+        *reinterpret_cast<float2*>(s) = make_float2(top, sum);
+      }
+    }
+  } else if constexpr (EPI == kGrad) {
+    const bool tail = a.v0 + m0 + BM > a.vocab;
+    int at[NF];
+    float shift[NF];
+    bool keep[NF], here[NF], any[NF];
 #pragma unroll
-          for (int i = 0; i < MF; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (at == 16 * i + r) z = acc[i][j][r];
-          if (here) a.ztarget[tok] = z;
-        }
-        if (real && lane < 16) {
-          const uint32_t piece = m0 / (BM / WM) + wm;
-          float* s = a.stats + (static_cast<uint64_t>(tok) * a.pieces + piece) * 2;
-          *reinterpret_cast<float2*>(s) = make_float2(top, sum);
-        }
-      } else {
-        // 2^12 exp(z - lse) as one power of two: 2^(z log2 e + shift); the argument's rounding, 2^-24 of some tens, is
-        // far below the result's
-        const float shift = target >= 0 ? 12.0f - a.lse[tok] * kLog2E : 0.0f;
-        const bool here = target >= 0 && at >= 0 && at < 16 * MF && (at & 15) < 4;
-        const bool any = __ballot(here) != 0, tail = a.v0 + m0 + BM > a.vocab;
-#pragma unroll
-        for (int i = 0; i < MF; ++i) {
+    for (int j = 0; j < NF; ++j) {
+      const uint32_t tok = n + 16 * j;
+      const int target = tok < a.tokens ? target_of(a, tok) : -1;
+      keep[j] = target >= 0;
+      at[j] = target - static_cast<int>(a.v0 + m);
+      // 2^12 exp(z - lse) as one power of two: 2^(z log2 e + shift); the argument's rounding, 2^-24 of some tens, is far
+      // below the result's
+      shift[j] = keep[j] ? 12.0f - a.lse[tok] * kLog2E : 0.0f;
+      here[j] = keep[j] && at[j] >= 0 && at[j] < 16 * MF && (at[j] & 15) < 4;
+      any[j] = __ballot(here[j]) != 0;
+    }
+    put_tile<T, MW, NW>(
+        stage,
+        [&](int i, int j) {
           float p[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2E, shift));
-          if (any) {
+          for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2E, shift[j]));
+          if (any[j]) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (at == 16 * i + r) p[r] -= kGScale;
+              if (at[j] == 16 * i + r) p[r] -= kGScale;
           }
           if (tail) {
 #pragma unroll
@@ -427,53 +479,67 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
           vec_t<T, 4> o;
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(p[r]);
-          if (any && here) {
+          if (any[j] && here[j]) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (at == 16 * i + r) a.lost[tok] = p[r] - static_cast<float>(o[r]);
+              if (at[j] == 16 * i + r) a.lost[n + 16 * j] = p[r] - static_cast<float>(o[r]);
           }
-          if (target < 0) o = vec_t<T, 4>{};  // (whatever its hidden state holds)
-          if (real) *reinterpret_cast<vec_t<T, 4>*>(a.g + static_cast<uint64_t>(tok) * a.ldg + m + 16 * i) = o;
-        }
-      }
-    }
+          return keep[j] ? o : vec_t<T, 4>{};  // (zeros without a target, whatever its hidden state holds)
+        },
+        [&](uint32_t row, uint32_t c, const vec_t<T, 8>& v) {
+          if (nw + row < a.tokens)
+            *reinterpret_cast<vec_t<T, 8>*>(a.g + static_cast<uint64_t>(nw + row) * a.ldg + mw + c) = v;
+        });
   } else if constexpr (EPI == kHidden) {
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
       const uint32_t tok = n + 16 * j;
-      if (tok >= a.tokens) continue;
-      const float scale = a.last ? a.rowscale[tok] : 0.0f;
-      const int target = a.last ? target_of(a, tok) : -1;
+      const bool real = tok < a.tokens;
+      const float scale = real && a.last ? a.rowscale[tok] : 0.0f;
+      const int target = real && a.last ? target_of(a, tok) : -1;
       const float lost = target >= 0 ? a.lost[tok] : 0.0f;
-      auto target_row = [&](uint32_t c) {
-        float f[4] = {};
-        if (target >= 0) load_f32<T, 4>(a.w.p + target * a.w.ld + c, f);
-        return v4f{f[0], f[1], f[2], f[3]};
-      };
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         const uint32_t c = m + 16 * i;
-        if (c >= a.dim) continue;
+        if (!real || c >= a.dim) continue;
         float* sum = a.acc + (static_cast<uint64_t>(split) * a.tokens + tok) * a.dim + c;
-        v4f v = acc[i][j];
         const uint32_t have = a.dim - c;
         if (!a.first) {
+          float f[4];
+          load_some<float, 4>(sum, have, f);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (static_cast<uint32_t>(r) < have) v[r] = sum[r] + v[r];
+          for (int r = 0; r < 4; ++r) acc[i][j][r] += f[r];
         }
-        if (a.last) {
-          v += lost * target_row(c);
+        if (!a.last) {
+          put4<float>(sum, acc[i][j], have, 0);
+          continue;
+        }
+        if (target >= 0) {
+          float f[4];
+          load_f32<T, 4>(a.w.p + target * a.w.ld + c, f);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = scale == 0.0f ? 0.0f : v[r] * scale;
-          put4<T>(static_cast<T*>(a.out) + static_cast<uint64_t>(tok) * a.ostride + c, v, have, 0);
-        } else {
-          put4<float>(sum, v, have, 0);
+          for (int r = 0; r < 4; ++r) acc[i][j][r] += lost * f[r];
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = scale == 0.0f ? 0.0f : acc[i][j][r] * scale;
       }
     }
+    if (a.last)
+      put_tile<T, MW, NW>(
+          stage,
+          [&](int i, int j) {
+            vec_t<T, 4> o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(acc[i][j][r]);
+            return o;
+          },
+          [&](uint32_t row, uint32_t c, const vec_t<T, 8>& v) {
+            if (nw + row < a.tokens && mw + c < a.dim)
+              stream8<T>(static_cast<T*>(a.out) + static_cast<uint64_t>(nw + row) * a.ostride + mw + c, a.dim - mw - c, v);
+          });
   } else {
     const float scale = *a.amax / kGScale;
+    const bool direct = a.out_f32 || a.accumulate;  // (a sum with what is there is rounded once, behind the addition)
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
       const uint32_t row = n + 16 * j;
@@ -493,6 +559,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
               for (int r = 0; r < 4; ++r) acc[i][j][r] += lost * f[r];
             }
         }
+      if (!direct) continue;
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         const uint32_t c = m + 16 * i;
@@ -504,6 +571,20 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
           put4<T>(static_cast<T*>(a.out) + o + c, v, a.dim - c, a.accumulate);
       }
     }
+    if (!direct)
+      put_tile<T, MW, NW>(
+          stage,
+          [&](int i, int j) {
+            vec_t<T, 4> o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(acc[i][j][r] * scale);
+            return o;
+          },
+          [&](uint32_t row, uint32_t c, const vec_t<T, 8>& v) {
+            if (a.v0 + nw + row < a.vocab && mw + c < a.dim)
+              stream8<T>(static_cast<T*>(a.out) + static_cast<uint64_t>(a.v0 + nw + row) * a.ostride + mw + c,
+                         a.dim - mw - c, v);
+          });
   }
 }
 
