@@ -173,8 +173,8 @@ struct Frags {
 
 // ---------------------------------------------------------------- the product
 //
-// The workgroup's tile is BM x BN, WM x WN waves of (BM / WM) x (BN / WN); two LDS buffers, one barrier a step of 64:
-// behind it the next step's tile starts on its way into the buffer that the step before has done with.
+// The workgroup's tile is BM x BN, WM x WN waves of (BM / WM) x (BN / WN); a ring of R LDS buffers, one barrier a step of
+// 64: behind it the tile R steps on starts on its way into the buffer that the step has done with.
 enum { kStats, kGrad, kHidden, kWeight };
 
 template <class T>
@@ -264,14 +264,15 @@ __device__ __forceinline__ void stream8(T* p, uint32_t n, const vec_t<T, 8>& v) 
   }
 }
 
-template <class T, int EPI, int BM, int BN, int WM, int WN>
+template <class T, int EPI, int BM, int BN, int WM, int WN, int R>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   constexpr int NT = 64 * WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
   constexpr bool AC = EPI == kHidden || EPI == kWeight, BC = EPI == kWeight;
-  __shared__ __attribute__((aligned(1024))) T lds[2 * (BM + BN) * kBK];
-  auto la = [&](uint32_t t) { return lds + (t & 1) * (BM * kBK); };  // step t's buffers
-  auto lb = [&](uint32_t t) { return lds + 2 * BM * kBK + (t & 1) * (BN * kBK); };
-  static_assert(BM * BN <= 2 * (BM + BN) * kBK, "the results pass through LDS as 16-bit elements");
+  __shared__ __attribute__((aligned(1024))) T lds[R * (BM + BN) * kBK];
+  static_assert((R & (R - 1)) == 0, "step t's buffers are those at t mod R");
+  auto la = [&](uint32_t t) { return lds + (t & (R - 1)) * (BM * kBK); };
+  auto lb = [&](uint32_t t) { return lds + R * BM * kBK + (t & (R - 1)) * (BN * kBK); };
+  static_assert(BM * BN <= R * (BM + BN) * kBK, "the results pass through LDS as 16-bit elements");
   // Workgroup ids go round the 8 XCDs: give each XCD a contiguous stretch of tiles, and walk the stretch in groups of 8
   // tile rows, so the tiles that run together on an XCD share operands in its L2.
   uint32_t id = blockIdx.x;
@@ -298,8 +299,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
 
   // A step's 64 k are two halves.  The fragments of a half are read while the half before is multiplied: x[0], y[0] hold
   // the first half of a step, x[1], y[1] the second.  Between them lies the step's one barrier: in front of it every wave
-  // has read its last from the step's buffer, into which the tile after the next may then be loaded, and has waited for
-  // its own pieces of the next tile.  Reads and loads are issued a few at a time between the matrix instructions: eight
+  // has read its last from the step's buffer, into which the tile R steps on may then be loaded, and has waited for its
+  // own pieces of the next tile.  Reads and loads are issued a few at a time between the matrix instructions: eight
   // loads behind each other, from eight waves at once, held every wave's products for about 1000 of a step's 3600 clocks.
   frag<T> x[2][MF], y[2][NF];
   constexpr int kLoads = Tile<T, BM, NT, AC>::kPieces + Tile<T, BN, NT, BC>::kPieces;
@@ -307,12 +308,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   const uint32_t steps = (left + kBK - 1) / kBK, full = left / kBK;
   auto meet = [&]() {  // (the scheduler would move the products behind it)
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // (the tiles behind the next one, R - 2 of them, may still be on their way)
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((R - 2) * kLoads) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto fetch = [&](uint32_t t) {  // a whole tile at once
+  // A whole tile at once.  Past the last step (R > 2) these are loads of zeros that nothing reads, so that the wait above
+  // always has as many behind the one it is for.
+  auto fetch = [&](uint32_t t) {
     const uint32_t toa = ta.place(la(t)), tob = tb.place(lb(t));
     if (t < full) {
 #pragma unroll
@@ -320,18 +324,19 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
 #pragma unroll
       for (int i = 0; i < Tile<T, BN, NT, BC>::kPieces; ++i) tb.load(i, tob);
     } else {
-      ta.load_end(toa, left - t * kBK);
-      tb.load_end(tob, left - t * kBK);
+      const uint32_t n = t < steps ? left - t * kBK : 0;
+      ta.load_end(toa, n);
+      tb.load_end(tob, n);
     }
     ta.advance();
     tb.advance();
   };
   // The products of one half, with the reads of the other from step t's buffer; with `loads` also the loads of step
-  // t + 1's tile.  (The reads end two groups early: the barrier behind waits for them.)
+  // t + R - 1's tile.  (The reads end two groups early: the barrier behind waits for them.)
   auto half = [&](int h, uint32_t t, bool loads) {
     const T *ca = la(t), *cb = lb(t);
-    const uint32_t toa = ta.place(la(t + 1)), tob = tb.place(lb(t + 1));
-    constexpr int kReads = MF + NF, kOver = MF - 2;
+    const uint32_t toa = ta.place(la(t + R - 1)), tob = tb.place(lb(t + R - 1));
+    constexpr int kReads = MF + NF, kOver = MF > 2 ? MF - 2 : 1;
     fa.touch();
     fb.touch();
 #pragma unroll
@@ -361,11 +366,19 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
       tb.advance();
     }
   };
-  fetch(0);
-  meet();
-  if (steps > 1) fetch(1);
+  if constexpr (R == 2) {
+    fetch(0);
+    meet();
+    if (steps > 1) fetch(1);
+  } else {
+#pragma unroll
+    for (uint32_t t = 0; t < R; ++t) fetch(t);
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 1) * kLoads) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
   uint32_t t = 0;
-  if (full > 2) {
+  if (full > R) {
 #pragma unroll
     for (int j = 0; j < NF; ++j) y[0][j] = fb.get(lb(0), 0, j);
 #pragma unroll
@@ -374,7 +387,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
       half(0, t, false);
       meet();
       half(1, t + 1, true);
-    } while (++t + 2 < full);
+    } while (++t + R < full);
   }
   // the last steps, whose tiles may be cut short: read and multiply in turn
   for (; t < steps; ++t) {
@@ -392,7 +405,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
       }
     }
     meet();
-    if (t + 2 < steps) fetch(t + 2);
+    if (R > 2 || t + R < steps) fetch(t + R);
+  }
+  if constexpr (R > 2) {  // LDS is free when the zeros have come, too
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
   }
 
   // acc[i][j][r] = C[m + 16 i + r, n + 16 j]
@@ -791,25 +808,34 @@ __global__ __launch_bounds__(256) void k_zero(O* out, uint64_t rows, uint32_t di
 
 uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
-constexpr uint32_t kBig = 256, kSmall = 128;
+// Tile shapes: big ones do more work for each byte that goes through LDS, small ones fill the CUs with less.  Big from one
+// tile a CU on (8192 x 32768 x 2048: 871 us, small ones 1192); small ones two a CU while there are enough, else one with a
+// deeper ring; tiny ones where even those leave half the CUs idle (33 tokens x 5003 x 520: forward 10.7 us, small ones
+// 14.1; backward 35, 42).
+constexpr uint32_t kBig = 256, kSmall = 128, kTiny = 64;
+enum { kTileBig, kTileSmall, kTileSmallDeep, kTileTiny };
+int tile_of(uint64_t m, uint64_t n, uint64_t splits) {
+  auto tiles = [&](uint32_t t) { return ceil_div(m, t) * ceil_div(n, t) * splits; };
+  return tiles(kBig) >= 256 ? kTileBig : tiles(kSmall) > 256 ? kTileSmall : tiles(kSmall) > 128 ? kTileSmallDeep : kTileTiny;
+}
+uint32_t tile_rows(int tile) { return tile == kTileBig ? kBig : tile == kTileTiny ? kTiny : kSmall; }
 
 template <class T, int EPI>
-int launch(GemmArgs<T>& a, uint32_t m, uint32_t n, bool big, hipStream_t stream) {
-  const uint32_t t = big ? kBig : kSmall;
+int launch(GemmArgs<T>& a, uint32_t m, uint32_t n, int tile, hipStream_t stream) {
+  const uint32_t t = tile_rows(tile);
   a.mt = static_cast<uint32_t>(ceil_div(m, t));
   a.nt = static_cast<uint32_t>(ceil_div(n, t));
   const uint64_t grid = static_cast<uint64_t>(a.mt) * a.nt * a.splits;
   if (grid >= (1u << 22)) return efail("vocab_loss: too many tiles for one call");
-  if (big)
-    k_gemm<T, EPI, 256, 256, 2, 4><<<static_cast<unsigned>(grid), 512, 0, stream>>>(a);
-  else
-    k_gemm<T, EPI, 128, 128, 2, 2><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a);
+  const unsigned g = static_cast<unsigned>(grid);
+  switch (tile) {
+    case kTileBig: k_gemm<T, EPI, 256, 256, 2, 4, 2><<<g, 512, 0, stream>>>(a); break;
+    case kTileSmall: k_gemm<T, EPI, 128, 128, 2, 2, 2><<<g, 256, 0, stream>>>(a); break;
+    case kTileSmallDeep: k_gemm<T, EPI, 128, 128, 2, 2, 4><<<g, 256, 0, stream>>>(a); break;
+    default: k_gemm<T, EPI, 64, 64, 2, 2, 4><<<g, 256, 0, stream>>>(a); break;
+  }
   return elaunch("omr_vocab_loss");
 }
-
-// Big tiles do twice the work for each byte that goes through LDS, small ones fill the CUs with less: big from one tile a
-// CU on.
-bool use_big(uint64_t m, uint64_t n) { return ceil_div(m, kBig) * ceil_div(n, kBig) >= 256; }
 
 // The piece of the vocabulary whose G is held at a time: about 256 MiB of it (what the last-level cache holds), at least
 // 1024 rows, in equal pieces of whole tiles.
@@ -823,10 +849,10 @@ uint64_t piece_bytes_most(uint64_t tokens, uint64_t vocab) {
   return std::min(std::max(kPieceBytes, tokens * 1024 * 2), tokens * up(vocab, 256) * 2);
 }
 
-// Parts of grad_hidden's inner dimension (the vocabulary piece): enough to fill the CUs where its tiles do not, of no less
-// than 512 rows.
+// Parts of grad_hidden's inner dimension (the vocabulary piece): two small tiles a CU where its tiles do not fill them, of
+// no less than 512 rows each.
 uint32_t hidden_splits(uint64_t tokens, uint64_t dim, uint32_t piece) {
-  if (use_big(dim, tokens)) return 1;
+  if (tile_of(dim, tokens, 1) == kTileBig) return 1;
   const uint64_t tiles = ceil_div(dim, kSmall) * ceil_div(tokens, kSmall);
   return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(512 / std::min<uint64_t>(tiles, 512), piece / 512)));
 }
@@ -844,7 +870,7 @@ Space layout(uint64_t tokens, uint64_t vocab, uint64_t dim, bool pack, bool grad
   s.w = 0;
   s.h = s.w + (pack ? up(vocab * pdim * 2, 256) : 0);
   s.rest = s.h + (pack ? up(tokens * pdim * 2, 256) : 0);
-  uint64_t fwd = up(tokens * 4, 256) + tokens * ceil_div(vocab, 64) * 8 + tokens * 32;
+  uint64_t fwd = up(tokens * 4, 256) + tokens * (ceil_div(vocab, 32) + 4) * 8;  // (a piece is 32 rows at least)
   uint64_t bwd = 256 + 3 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) + up(piece_bytes_most(tokens, vocab), 256) +
                  acc_bytes_most(tokens, dim);
   s.bytes = s.rest + (grads ? std::max(fwd, bwd) : fwd) + 256;
@@ -935,7 +961,7 @@ int omr_vocab_loss(const void* hidden, uint64_t hidden_stride, const void* weigh
     if (const int rc = operands<T>(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, sp, ws, &a.b, &a.a,
                                    S(stream)))
       return rc;
-    const bool big = use_big(vocab, tokens);
+    const int tile = tile_of(vocab, tokens, 1);
     a.k = dim;
     a.splits = 1;
     a.ksplit = dim;
@@ -955,8 +981,8 @@ int omr_vocab_loss(const void* hidden, uint64_t hidden_stride, const void* weigh
         k_few<T, 2><<<grid, 256, 0, S(stream)>>>(a);
       if (const int rc = elaunch("omr_vocab_loss")) return rc;
     } else {
-      a.pieces = static_cast<uint32_t>(big ? ceil_div(vocab, 256) * 2 : ceil_div(vocab, 128) * 2);
-      if (const int rc = launch<T, kStats>(a, a.vocab, a.tokens, big, S(stream))) return rc;
+      a.pieces = static_cast<uint32_t>(ceil_div(vocab, tile_rows(tile)) * 2);  // two waves' parts a tile
+      if (const int rc = launch<T, kStats>(a, a.vocab, a.tokens, tile, S(stream))) return rc;
     }
     // four waves a token where there are not enough tokens to fill the CUs
     if (tokens <= 1024)
@@ -1057,7 +1083,7 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
       z.k = dim;
       z.ksplit = dim;
       z.splits = 1;
-      if (const int rc = launch<T, kGrad>(z, cols, z.tokens, use_big(cols, tokens), S(stream))) return rc;
+      if (const int rc = launch<T, kGrad>(z, cols, z.tokens, tile_of(cols, tokens, 1), S(stream))) return rc;
       if (grad_hidden != nullptr) {
         GemmArgs<T> x = a;
         x.a = {w.p + v0 * w.ld, w.ld, pdim};
@@ -1070,7 +1096,7 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
         x.last = done && splits == 1;
         x.out = grad_hidden;
         x.ostride = grad_hidden_stride;
-        if (const int rc = launch<T, kHidden>(x, dim, x.tokens, use_big(dim, tokens), S(stream))) return rc;
+        if (const int rc = launch<T, kHidden>(x, dim, x.tokens, tile_of(dim, tokens, x.splits), S(stream))) return rc;
         if (done && splits > 1) {
           x.splits = splits;
           const uint64_t blocks = ceil_div(tokens * dim, 256);
@@ -1089,7 +1115,7 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
         y.ostride = grad_weight_stride;
         y.out_f32 = grad_weight_dtype == OMR_F32;
         y.accumulate = accumulate != 0;
-        if (const int rc = launch<T, kWeight>(y, dim, cols, use_big(dim, cols), S(stream))) return rc;
+        if (const int rc = launch<T, kWeight>(y, dim, cols, tile_of(dim, cols, 1), S(stream))) return rc;
       }
     }
     return 0;
