@@ -15,6 +15,11 @@
 //       wire format of common.cc:399-443)    -T file  (with -M) write the last round's wire trace: per message
 //       a {src, dst, imm, len} record of four uint32 (workers 0..k-1, aggregator 100) then its payload, the
 //       (B*len + len)*4 bytes an ibv_post_send would carry (common.cc:424), slot by slot, round by round
+//   -E dim:tokens  the tensor is a gradient instead of the generator's: that of an embedding table of n / dim rows of dim
+//       floats, from one step of a small language model on each worker's own `tokens` tokens (lookup, layer norm, loss
+//       against an output layer, and back: omr_embed ... omr_embed_grad_f32).  Its non-zero blocks are the rows of the
+//       worker's tokens.  -c then expects the sum of every worker's gradient, made again worker by worker (the step's
+//       operators give the same bits each time)
 //
 // With an aggregator list agg[:port][,agg[:port]...] the worker connects to every ./omr_server in list order, as the
 // reference's sock_connect does (common.cc:71-97): each server gives it its ID (the position of its IP in the
@@ -28,7 +33,9 @@
 #include <getopt.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -55,6 +62,8 @@ struct Opts {
   bool host = false;  // -H: the tensor in pinned host memory, as the reference's registered res->buf
   int transport = omrnet::kRccl, local_id = -1;
   const char* trace = nullptr;
+  uint32_t dim = 0;  // -E: the embedding's row length (0: the generator's tensor), and a worker's tokens
+  uint64_t tokens = 0;
 };
 
 void usage(const char* argv0) {  // common.cc:1441-1457 (default port and -r text corrected: SURVEY.md §5)
@@ -71,6 +80,8 @@ void usage(const char* argv0) {  // common.cc:1441-1457 (default port and -r tex
   fprintf(stdout, " -M message mode: the round as the reference's wire messages; -T <file> trace them\n");
   fprintf(stdout, " -H the tensor in pinned host memory (the reference's registered buffer): each round reads it and\n"
                   "    returns its results into it (omr_sparse_buckets_f32, one bucket)\n");
+  fprintf(stdout, " -E <dim>:<tokens> the tensor is an embedding table's gradient (rows of dim floats) from a step on\n"
+                  "    tokens tokens\n");
   fprintf(stdout, " -X rccl|ipc transport to the servers (default rccl)  -C co-located aggregation  -l <k> local id\n");
   fprintf(stdout, " -h, --help show this help message\n");
 }
@@ -84,9 +95,94 @@ void usage(const char* argv0) {  // common.cc:1441-1457 (default port and -r tex
     }                                                                            \
   } while (0)
 
+#define OMROK(x)                                                                 \
+  do {                                                                           \
+    if (x) {                                                                     \
+      fprintf(stderr, "%s failed: %s\n", #x, omr_last_error());                  \
+      return 1;                                                                  \
+    }                                                                            \
+  } while (0)
+
+struct DeviceMem {  // freed with its scope
+  void* p = nullptr;
+  ~DeviceMem() { (void)hipFree(p); }
+  hipError_t get(size_t bytes) { return hipMalloc(&p, bytes ? bytes : 1); }
+};
+
+// -E: the gradient of the embedding table E of one training step on the worker's tokens t_0 .. t_T:
+//   h = sqrt(dim) E[t_i],  y = layer norm(h),  loss = mean cross entropy of y U^T against t_{i+1}
+// E: uniform [-1, 1); U = E / 16 in bf16 (the output layer, the same on every worker); tokens: low ids the more often.
+int make_step_gradient(uint32_t worker_id, const Opts& o, float* d_x, float* mean_loss) {
+  const uint64_t rows = o.n / o.dim, T = o.tokens;
+  std::vector<int64_t> ids(std::max<uint64_t>(rows, T + 1));
+  DeviceMem table, ones, U, d_ids, h, y, gy, stats, loss, gone, ws_loss, ws_norm, ws_embed;
+  // the table, by the generator's hashed fill of every block
+  std::vector<int32_t> all(o.n / o.block, 1);
+  HIPOK(ones.get(all.size() * sizeof(int32_t)));
+  HIPOK(hipMemcpy(ones.p, all.data(), all.size() * sizeof(int32_t), hipMemcpyHostToDevice));
+  HIPOK(table.get(o.n * sizeof(float)));
+  OMROK(omr_fill_blocks_f32(static_cast<int32_t*>(ones.p), all.size(), o.block, 1, 1, static_cast<float*>(table.p), nullptr));
+  // the output layer: every row looked up
+  HIPOK(d_ids.get(ids.size() * sizeof(int64_t)));
+  for (uint64_t i = 0; i < rows; ++i) ids[i] = static_cast<int64_t>(i);
+  HIPOK(hipMemcpy(d_ids.p, ids.data(), rows * sizeof(int64_t), hipMemcpyHostToDevice));
+  HIPOK(U.get(o.n * 2));
+  OMROK(omr_embed(table.p, OMR_F32, rows, o.dim, o.dim, d_ids.p, 1, rows, 0.0625f, U.p, OMR_BF16, o.dim, nullptr));
+  HIPOK(hipDeviceSynchronize());
+  uint64_t x = 0x9E3779B97F4A7C15ull * (worker_id + 1);
+  for (uint64_t i = 0; i <= T; ++i) {
+    x ^= x << 13;
+    x ^= x >> 7;
+    x ^= x << 17;
+    const double u = static_cast<double>(x >> 11) / 9007199254740992.0;
+    ids[i] = static_cast<int64_t>(u * u * u * static_cast<double>(rows));
+  }
+  HIPOK(hipMemcpy(d_ids.p, ids.data(), (T + 1) * sizeof(int64_t), hipMemcpyHostToDevice));
+  const int64_t* tok = static_cast<const int64_t*>(d_ids.p);
+  const uint64_t act = T * o.dim * 2;
+  HIPOK(h.get(act));
+  HIPOK(y.get(act));
+  HIPOK(gy.get(act));
+  HIPOK(stats.get(2 * T * sizeof(float)));
+  HIPOK(loss.get(2 * T * sizeof(float)));
+  HIPOK(gone.get(sizeof(float)));
+  float *mean = static_cast<float*>(stats.p), *rstd = mean + T, *ls = static_cast<float*>(loss.p), *lse = ls + T;
+  const float each = 1.0f / static_cast<float>(T), scale = std::sqrt(static_cast<float>(o.dim));
+  HIPOK(hipMemcpy(gone.p, &each, sizeof(each), hipMemcpyHostToDevice));
+  const size_t wl = omr_vocab_loss_workspace_bytes(T, rows, o.dim, 0, 1), wn = omr_layer_norm_grad_workspace_bytes(T, o.dim),
+               we = omr_embed_grad_workspace_bytes(T, rows, o.dim);
+  HIPOK(ws_loss.get(wl));
+  HIPOK(ws_norm.get(wn));
+  HIPOK(ws_embed.get(we));
+  OMROK(omr_embed(table.p, OMR_F32, rows, o.dim, o.dim, tok, 1, T, scale, h.p, OMR_BF16, o.dim, nullptr));
+  OMROK(omr_layer_norm(h.p, OMR_BF16, T, o.dim, o.dim, nullptr, nullptr, OMR_F32, 1e-5f, y.p, o.dim, mean, rstd, nullptr));
+  OMROK(omr_vocab_loss(y.p, o.dim, U.p, o.dim, OMR_BF16, T, rows, o.dim, tok + 1, 1, ls, lse, ws_loss.p, wl, nullptr));
+  OMROK(omr_vocab_loss_grad(y.p, o.dim, U.p, o.dim, OMR_BF16, T, rows, o.dim, tok + 1, 1, lse,
+                            static_cast<const float*>(gone.p), 0, gy.p, o.dim, nullptr, OMR_F32, o.dim, 0, ws_loss.p, wl,
+                            nullptr));
+  OMROK(omr_layer_norm_grad(gy.p, o.dim, h.p, OMR_BF16, T, o.dim, o.dim, mean, rstd, nullptr, OMR_F32, gy.p, o.dim, nullptr,
+                            nullptr, 0, nullptr, 0, nullptr));
+  OMROK(omr_embed_grad_f32(gy.p, OMR_BF16, o.dim, tok, 1, T, rows, o.dim, scale, d_x, o.dim, 0, ws_embed.p, we, nullptr));
+  std::vector<float> host(T);
+  HIPOK(hipMemcpy(host.data(), ls, T * sizeof(float), hipMemcpyDeviceToHost));
+  double sum = 0.0;
+  for (float v : host) sum += v;
+  if (mean_loss) *mean_loss = static_cast<float>(sum / static_cast<double>(T));
+  return 0;
+}
+
 // the worker's tensor: the reference generator (client.cc:396-421) on the device
 int make_input(uint32_t worker_id, const Opts& o, float* d_x, int32_t* d_bitmap) {
   const uint64_t nb = o.n / o.block;
+  if (o.dim) {
+    float mean_loss = 0.0f;
+    if (make_step_gradient(worker_id, o, d_x, &mean_loss)) return 1;
+    HIPOK(hipDeviceSynchronize());
+    if (worker_id == 0)
+      std::cout << "embedding gradient: " << o.n / o.dim << " rows of " << o.dim << ", " << o.tokens
+                << " tokens; loss: " << mean_loss << std::endl;
+    return 0;
+  }
   std::vector<int32_t> bm(nb);
   uint64_t nz = 0;
   if (omr_gen_bitmap(worker_id, o.density, nb, bm.data(), &nz)) return 1;
@@ -104,6 +200,23 @@ int make_input(uint32_t worker_id, const Opts& o, float* d_x, int32_t* d_bitmap)
 // Returns 0 (check OK), 1 (mismatch, the reference's "error: " line printed) or -1 (could not check).
 int host_check(const Opts& o, int workers, const float* d_result) {
   const uint64_t nb = o.n / o.block;
+  if (o.dim) {  // -E: every worker's gradient made again, and summed here in rank order
+    DeviceMem again;
+    if (again.get(o.n * sizeof(float)) != hipSuccess) return -1;
+    std::vector<float> sum(o.n, 0.0f), one(o.n);
+    for (int w = 0; w < workers; ++w) {
+      if (make_step_gradient(static_cast<uint32_t>(w), o, static_cast<float*>(again.p), nullptr)) return -1;
+      if (hipMemcpy(one.data(), again.p, o.n * sizeof(float), hipMemcpyDeviceToHost) != hipSuccess) return -1;
+      for (uint64_t i = 0; i < o.n; ++i) sum[i] = sum[i] + one[i];
+    }
+    if (hipMemcpy(one.data(), d_result, o.n * sizeof(float), hipMemcpyDefault) != hipSuccess) return -1;
+    for (uint64_t i = 0; i < o.n; ++i)
+      if (!(one[i] == sum[i])) {  // (by value: a block of zeros keeps their signs)
+        std::cout << "error: " << sum[i] << "<---->" << one[i] << std::endl;
+        return 1;
+      }
+    return 0;
+  }
   std::vector<uint8_t> cnt(nb, 0);
   std::vector<int32_t> bm(nb);
   for (int w = 0; w < workers; ++w) {
@@ -502,7 +615,7 @@ int main(int argc, char* argv[]) {
                               {"service-level", 1, nullptr, 's'}, {"density-ratio", 1, nullptr, 'r'},
                               {"help", 0, nullptr, 'h'},          {nullptr, 0, nullptr, 0}};
   while (true) {
-    int c = getopt_long(argc, argv, "p:d:i:g:s:r:n:b:W:R:G:L:T:X:l:cIMCHh", longopts, nullptr);
+    int c = getopt_long(argc, argv, "p:d:i:g:s:r:n:b:W:R:G:L:T:X:l:E:cIMCHh", longopts, nullptr);
     if (c == -1) break;
     switch (c) {
       case 'p': o.port = static_cast<int>(strtoul(optarg, nullptr, 0)); break;
@@ -535,12 +648,27 @@ int main(int argc, char* argv[]) {
       case 'l': o.local_id = atoi(optarg); break;
       case 'C': o.colocated = true; break;
       case 'H': o.host = true; break;
+      case 'E': {
+        char* end = nullptr;
+        o.dim = static_cast<uint32_t>(strtoul(optarg, &end, 0));
+        o.tokens = *end == ':' ? strtoull(end + 1, nullptr, 0) : 0;
+        if (o.dim == 0 || o.tokens == 0) {
+          fprintf(stderr, "-E needs <dim>:<tokens>\n");
+          usage(argv[0]);
+          return 1;
+        }
+        break;
+      }
       default: usage(argv[0]); return 1;
     }
   }
   if (o.host && o.messages) {  // (the message round runs on device tensors only)
     fprintf(stderr, "-H and -M cannot be combined\n");
     usage(argv[0]);
+    return 1;
+  }
+  if (o.dim != 0 && (o.dim % 8 != 0 || o.n % o.dim != 0 || o.tokens >= 1u << 30)) {
+    fprintf(stderr, "-E: dim must be a multiple of 8 that divides -n, and tokens below 2^30\n");
     return 1;
   }
   int ndev = 0;

@@ -4,12 +4,15 @@ vocabulary loss) against their formulas in 64 bits.
 Tolerances are worst-case rounding bounds: u = 2^-24 is half an fp32 step, a sum of n terms in any order is off by at
 most n u times the sum of their magnitudes, and a result rounded to type t adds finfo(t).eps / 2 of its magnitude (and
 half the smallest subnormal step, where fp16 underflows)."""
-import math
+import ctypes
+import os
+import subprocess
+import threading
 
 import pytest
 import torch
 
-from omr import ops
+from omr import Layout, cdist, ops
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -557,3 +560,150 @@ def test_operators_in_a_graph_and_on_streams(gpu):
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(want, captured.outputs()))
     assert all(torch.equal(p, q) for p, q in zip(want, other.outputs()))
+
+
+# ---------------------------------------------------------------------------------------------------- a training step
+
+class Model:
+    """A small language model whose output layer is its embedding table: lookup, layer norm, loss, and back into one
+    flat fp32 gradient [table | norm weight | norm bias | padding to the layout]."""
+
+    def __init__(self, V, D, T, L, dtype=BF16, seed=0):
+        g = gen(seed)
+        self.V, self.D, self.T, self.dtype = V, D, T, dtype
+        self.table = rand((V, D), dtype, g, std=0.05)
+        self.weight, self.bias = rand((D,), F32, g, std=0.1, mean=1.0), rand((D,), F32, g, std=0.1)
+        self.scale = D ** 0.5
+        self.loss_plan = ops.VocabLossPlan(T, V, D, dtype=dtype)
+        self.norm_plan, self.embed_plan = ops.LayerNormGradPlan(T, D), ops.EmbedGradPlan(T, V, D)
+        self.flat = torch.zeros(L.n, device="cuda")
+        n = V * D
+        self.g_table, self.g_weight, self.g_bias = self.flat[:n].view(V, D), self.flat[n:n + D], self.flat[n + D:n + 2 * D]
+
+    def step(self, ids, targets, factor):
+        """The losses; the gradient of factor * (their sum) is in `flat`."""
+        h = ops.embed(self.table, ids, scale=self.scale)
+        f = ops.layer_norm(h, self.weight, self.bias)
+        loss, lse = self.loss_plan.forward(f.out, self.table, targets)
+        gy, _ = self.loss_plan.backward(f.out, self.table, targets, lse, factor, grad_weight=self.g_table)
+        r = self.norm_plan.run(gy, h, f.mean, f.rstd, self.weight, grad_weight=self.g_weight, grad_bias=self.g_bias)
+        self.embed_plan.run(r.grad_x, ids, self.g_table, scale=self.scale, accumulate=True)
+        return loss
+
+    def reference(self, ids, targets, factor):
+        """The same step by differentiation in 64 bits."""
+        E = self.table.double().requires_grad_()
+        w, b = self.weight.double().requires_grad_(), self.bias.double().requires_grad_()
+        ok = (ids >= 0) & (ids < self.V)
+        h = torch.where(ok[:, None], E[ids.clamp(0, self.V - 1)] * self.scale, 0.0)
+        y = torch.nn.functional.layer_norm(h, (self.D,), w, b, 1e-5)
+        loss = torch.nn.functional.cross_entropy(y @ E.t(), targets, ignore_index=-100, reduction="none")
+        (loss.sum() * factor).backward()
+        return loss.detach(), E.grad, w.grad, b.grad
+
+
+def tokens(T, V, g):
+    ids = make_ids(T, V, g, "low")
+    ids[::17] = -1
+    targets = torch.roll(ids, -1)
+    targets[targets < 0] = -100
+    targets[-1] = -100
+    return ids, targets
+
+
+@pytest.mark.parametrize("V,D,T", [(1000, 128, 300), (777, 200, 129)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_training_step(gpu, V, D, T, dtype):
+    """All operators together against differentiation in 64 bits.  The activations are rounded to the type at four places
+    (the lookup, the norm and the two gradients that pass back), each off by half a step of its magnitude; where such an
+    error enters the softmax or the norm it passes on with a factor of the order of one (logits of order one).  So each
+    gradient is within ten such errors of its norm."""
+    L = Layout(n=8 * 16384 * -(-(V * D + 2 * D) // (8 * 16384)))
+    m = Model(V, D, T, L, dtype)
+    ids, targets = tokens(T, V, gen(1))
+    factor = torch.tensor(1.0 / T, device="cuda")
+    loss = m.step(ids, targets, factor)
+    want = m.reference(ids, targets, 1.0 / T)
+    for got, ref, what in zip((loss, m.g_table, m.g_weight, m.g_bias), want, ("loss", "table", "weight", "bias")):
+        off = (got.double() - ref).norm().item() / ref.norm().item()
+        assert off <= 10 * half(dtype), (what, off)
+    assert not m.flat[V * D + 2 * D:].any()
+    again = m.flat.clone()
+    assert torch.equal(m.step(ids, targets, factor), loss) and torch.equal(m.flat, again)
+
+
+@pytest.mark.parametrize("world", [2, 3])
+def test_step_gradients_summed_by_the_round(gpu, world):
+    """Each worker's step gradient through the sparse all-reduce: every worker holds the rank-order sum, bit for bit."""
+    V, D, T = 1000, 128, 200
+    L = Layout(n=8 * 16384 * 2)
+    models = [Model(V, D, T, L) for _ in range(world)]
+    for w, m in enumerate(models):
+        ids, targets = tokens(T, V, gen(50 + w))
+        m.step(ids, targets, torch.tensor(1.0 / T, device="cuda"))
+    want = torch.zeros_like(models[0].flat)
+    for m in models:
+        want = want + m.flat
+    torch.cuda.synchronize()
+    D_ = cdist.load()
+    board = D_.omr_local_board_create(world)
+    errs = []
+
+    def rank(r):
+        try:
+            torch.cuda.set_device(0)
+            d, plan = ctypes.c_void_p(), ctypes.c_void_p()
+            assert D_.omr_dist_create_local(board, r, ctypes.byref(d)) == 0
+            assert D_.omr_ar_plan_create(d, L.n, L.block_size, L.num_lanes, L.num_threads, ctypes.byref(plan)) == 0
+            st = torch.cuda.Stream()
+            x = models[r].flat
+            rc = D_.omr_sparse_round_f32(plan, x.data_ptr(), x.data_ptr(), None, None, None, 0, None, None, st.cuda_stream)
+            assert rc == 0, D_.omr_dist_last_error()
+            st.synchronize()
+            D_.omr_ar_plan_destroy(plan)
+            D_.omr_dist_destroy(d)
+        except BaseException as e:  # noqa: BLE001
+            errs.append(f"rank {r}: {e!r}")
+
+    th = [threading.Thread(target=rank, args=(r,)) for r in range(world)]
+    for t in th:
+        t.start()
+    for t in th:
+        t.join(timeout=100)
+    assert not any(t.is_alive() for t in th) and not errs, errs
+    D_.omr_local_board_destroy(board)
+    for m in models:
+        assert torch.equal(m.flat, want)
+
+
+def test_step_in_a_graph(gpu):
+    """The whole step captured: every replay, with eager steps of another model between, gives the eager bits."""
+    V, D, T = 640, 96, 150
+    L = Layout(n=8 * 16384)
+    eager, captured = Model(V, D, T, L), Model(V, D, T, L)
+    factor = torch.tensor(1.0 / T, device="cuda")
+    ids, targets = tokens(T, V, gen(0))
+    captured.step(ids, targets, factor)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = captured.step(ids, targets, factor)
+    for k in range(4):
+        i, t = tokens(T, V, gen(10 + k))
+        ids.copy_(i)
+        targets.copy_(t)
+        want = eager.step(ids, targets, factor)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want) and torch.equal(captured.flat, eager.flat), k
+
+
+@pytest.mark.parametrize("args", [["-L", "1"], ["-L", "3"], ["-L", "2", "-I"], ["-L", "2", "-H"], ["-L", "2", "-M"]])
+def test_client_embedding_gradient(gpu, args):
+    """./omr_client -E: the workers' tensors are embedding gradients of a training step, and -c checks their sum."""
+    exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "omnireduce-rdma-demo_amd", "bin",
+                       "omr_client")
+    p = subprocess.run([exe, *args, "-n", str(1 << 20), "-E", "256:500", "-W", "1", "-R", "3", "-c"], capture_output=True,
+                       text=True, timeout=100)
+    out = p.stdout + p.stderr
+    assert p.returncode == 0 and "check OK" in out and "embedding gradient: 4096 rows of 256, 500 tokens" in out, out

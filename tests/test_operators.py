@@ -1,0 +1,117 @@
+"""The operators that make the gradient, without a GPU: what they refuse (before anything is launched), and the sizes of
+their workspaces."""
+import ctypes
+
+import pytest
+import torch
+
+from omr import _lib, ops
+
+EINVAL = _lib.OMR_EINVAL
+A = 1 << 12  # an address that is only checked
+
+
+def refused(rc, text):
+    assert rc == EINVAL
+    assert text in _lib.load().omr_last_error().decode(), _lib.load().omr_last_error()
+
+
+def embed(**k):
+    a = dict(table=A, td=1, rows=10, dim=8, stride=8, ids=A, ids64=1, n=4, scale=1.0, out=A, od=1, ostride=8)
+    a.update(k)
+    return _lib.load().omr_embed(*a.values(), None)
+
+
+def embed_grad(**k):
+    a = dict(grad=A, gd=1, gstride=8, ids=A, ids64=1, n=4, rows=10, dim=8, scale=1.0, out=A, ostride=8, acc=0, ws=A,
+             bytes=1 << 30)
+    a.update(k)
+    return _lib.load().omr_embed_grad_f32(*a.values(), None)
+
+
+def norm(**k):
+    a = dict(x=A, dt=1, rows=4, dim=8, stride=8, w=A, b=A, pdt=0, eps=1e-5, out=A, ostride=8, mean=A, rstd=A)
+    a.update(k)
+    return _lib.load().omr_layer_norm(*a.values(), None)
+
+
+def norm_grad(**k):
+    a = dict(dy=A, dystride=8, x=A, dt=1, rows=4, dim=8, stride=8, mean=A, rstd=A, w=A, pdt=0, dx=A, dxstride=8, dw=A, db=A,
+             acc=0, ws=A, bytes=1 << 30)
+    a.update(k)
+    return _lib.load().omr_layer_norm_grad(*a.values(), None)
+
+
+def loss(**k):
+    a = dict(h=A, hs=8, w=A, wstride=8, dt=1, n=4, vocab=10, dim=8, t=A, t64=1, loss=A, lse=A, ws=A, bytes=1 << 40)
+    a.update(k)
+    return _lib.load().omr_vocab_loss(*a.values(), None)
+
+
+def loss_grad(**k):
+    a = dict(h=A, hs=8, w=A, wstride=8, dt=1, n=4, vocab=10, dim=8, t=A, t64=1, lse=A, g=A, gs=1, gh=A, ghs=8, gw=A, gwd=0,
+             gws=8, acc=0, ws=A, bytes=1 << 40)
+    a.update(k)
+    return _lib.load().omr_vocab_loss_grad(*a.values(), None)
+
+
+@pytest.mark.parametrize("call,arg,text", [
+    (embed, dict(td=3), "element type"), (embed, dict(od=-1), "element type"), (embed, dict(dim=0), "dim"),
+    (embed, dict(dim=(1 << 24) + 1, ostride=1 << 25), "dim"), (embed, dict(rows=1 << 31), "2^31"),
+    (embed, dict(n=1 << 31), "2^31"), (embed, dict(ostride=7), "stride"), (embed, dict(out=None), "NULL"),
+    (embed, dict(ids=None), "NULL"), (embed, dict(table=None), "NULL"),
+    (embed, dict(n=(1 << 31) - 1, dim=1 << 16, ostride=1 << 16), "too many"),
+    (embed_grad, dict(gd=5), "element type"), (embed_grad, dict(dim=0), "dim"), (embed_grad, dict(rows=1 << 31), "2^31"),
+    (embed_grad, dict(n=1 << 31), "2^31"), (embed_grad, dict(ostride=4), "stride"), (embed_grad, dict(out=None), "NULL"),
+    (embed_grad, dict(ws=None), "NULL"), (embed_grad, dict(ids=None), "NULL"), (embed_grad, dict(ws=A + 8), "aligned"),
+    (embed_grad, dict(bytes=16), "workspace of 16 bytes"),
+    (norm, dict(dt=4), "elements"), (norm, dict(pdt=2), "parameters"), (norm, dict(dim=0), "dim"),
+    (norm, dict(ostride=7), "stride"), (norm, dict(eps=-1.0), "eps"), (norm, dict(eps=float("nan")), "eps"),
+    (norm, dict(mean=None), "NULL"), (norm, dict(x=None), "NULL"),
+    (norm_grad, dict(dt=7), "elements"), (norm_grad, dict(pdt=2), "parameters"), (norm_grad, dict(dxstride=1), "stride"),
+    (norm_grad, dict(dx=None), "NULL"), (norm_grad, dict(rstd=None), "NULL"), (norm_grad, dict(ws=None), "workspace"),
+    (norm_grad, dict(ws=A + 4), "aligned"), (norm_grad, dict(bytes=0), "workspace of 0 bytes"),
+    (loss, dict(dt=0), "bf16 or fp16"), (loss, dict(dim=0), "dim"), (loss, dict(dim=(1 << 20) + 1), "dim"),
+    (loss, dict(vocab=0), "vocab"), (loss, dict(vocab=1 << 31), "vocab"), (loss, dict(n=1 << 31), "tokens"),
+    (loss, dict(t=None), "NULL"), (loss, dict(lse=None), "NULL"), (loss, dict(ws=None), "workspace"),
+    (loss, dict(bytes=100), "workspace of 100 bytes"), (loss, dict(wstride=9, bytes=700), "pack"),
+    (loss, dict(w=A + 2, bytes=700), "pack"),
+    (loss_grad, dict(dt=0), "bf16 or fp16"), (loss_grad, dict(gwd=2), "grad_weight"), (loss_grad, dict(ghs=7), "stride"),
+    (loss_grad, dict(gws=7), "stride"), (loss_grad, dict(g=None), "NULL"), (loss_grad, dict(lse=None), "NULL"),
+    (loss_grad, dict(bytes=1000), "workspace of 1000 bytes"),
+])
+def test_refusals(call, arg, text):
+    refused(call(**arg), text)
+
+
+def test_empty_calls_launch_nothing():
+    assert embed(n=0, ids=None, out=None) == 0
+    assert embed_grad(rows=0, out=None, ws=None) == 0
+    assert norm(rows=0, x=None, out=None) == 0
+    assert loss(n=0, h=None, ws=None) == 0
+    assert loss_grad(n=0, gw=None) == 0
+    assert loss_grad(n=0, acc=1) == 0
+
+
+def test_workspaces_grow_with_the_call():
+    """A plan for so many tokens holds any smaller call."""
+    lib = _lib.load()
+    for size in (lambda n: lib.omr_embed_grad_workspace_bytes(n, 5000, 300),
+                 lambda n: lib.omr_layer_norm_grad_workspace_bytes(n, 300),
+                 lambda n: lib.omr_vocab_loss_workspace_bytes(n, 50001, 300, 1, 1),
+                 lambda n: lib.omr_vocab_loss_workspace_bytes(n, 50001, 300, 0, 0),
+                 lambda n: lib.omr_vocab_loss_workspace_bytes(n, 1 << 30, 64, 0, 1)):
+        at = [size(n) for n in (0, 1, 2, 15, 16, 17, 31, 33, 100, 257, 1000, 2048, 4095, 5000, 20000, 100000)]
+        assert at == sorted(at) and at[-1] < 1 << 50
+
+
+def test_the_front_end_refuses():
+    t = torch.zeros(4, 8)
+    with pytest.raises(ValueError, match="device"):
+        ops.embed(t, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="device"):
+        ops.layer_norm(t)
+    with pytest.raises(ValueError, match="dtype"):
+        ops.VocabLossPlan(4, 10, 8, dtype=torch.float32)
+    with pytest.raises(ValueError, match="sizes"):
+        ops.VocabLossPlan(4, 0, 8)
