@@ -745,12 +745,19 @@ __global__ __launch_bounds__(1024) void k_scales(GemmArgs<T> a, const float* gra
                                                  float* rowscale) {
   __shared__ float top[16];
   float m = 0.0f;
-  for (uint32_t n = threadIdx.x; n < a.tokens; n += 1024) {
-    const bool keep = target_of(a, n) >= 0;
-    const float g = keep ? grad_loss[n * stride] : 0.0f;
-    rowscale[n] = g / kGScale;
-    // (a NaN is kept: the gradient shall have it)
-    m = m != m || fabsf(g) <= m ? m : fabsf(g);
+  for (uint64_t n0 = threadIdx.x; n0 < a.tokens; n0 += 8 * 1024) {  // eight tokens in flight
+    float g[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t n = n0 + i * 1024;
+      g[i] = n < a.tokens && target_of(a, static_cast<uint32_t>(n)) >= 0 ? grad_loss[n * stride] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (n0 + i * 1024 < a.tokens) rowscale[n0 + i * 1024] = g[i] / kGScale;
+      // (a NaN is kept: the gradient shall have it)
+      m = m != m || fabsf(g[i]) <= m ? m : fabsf(g[i]);
+    }
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
@@ -861,6 +868,13 @@ uint64_t acc_bytes_most(uint64_t tokens, uint64_t dim) {
   return std::max<uint64_t>(tokens * dim * 4, 512ull * kSmall * kSmall * 4);
 }
 
+// The forward's pieces: two of each token a tile. Tiles of 64 rows are taken up to 2^21 logits, of 128 up to 2^24, and of 64
+// by k_few; else of 256.
+uint64_t stats_bytes_most(uint64_t tokens, uint64_t vocab) {
+  return tokens * (ceil_div(vocab, 128) + 4) * 8 + std::min<uint64_t>(tokens, kFewTokens) * (ceil_div(vocab, 64) + 1) * 8 +
+         (4ull << 20);
+}
+
 struct Space {
   uint64_t w, h, rest, bytes;  // packed weight, packed hidden states, then the pass's own
 };
@@ -870,9 +884,9 @@ Space layout(uint64_t tokens, uint64_t vocab, uint64_t dim, bool pack, bool grad
   s.w = 0;
   s.h = s.w + (pack ? up(vocab * pdim * 2, 256) : 0);
   s.rest = s.h + (pack ? up(tokens * pdim * 2, 256) : 0);
-  uint64_t fwd = up(tokens * 4, 256) + tokens * (ceil_div(vocab, 32) + 4) * 8;  // (a piece is 32 rows at least)
-  uint64_t bwd = 256 + 3 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) + up(piece_bytes_most(tokens, vocab), 256) +
-                 acc_bytes_most(tokens, dim);
+  uint64_t fwd = up(tokens * 4, 256) + stats_bytes_most(tokens, vocab);
+  uint64_t bwd = 256 + 3 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) +
+                 up(piece_bytes_most(tokens, vocab), 256) + acc_bytes_most(tokens, dim);
   s.bytes = s.rest + (grads ? std::max(fwd, bwd) : fwd) + 256;
   return s;
 }

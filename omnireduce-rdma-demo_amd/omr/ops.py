@@ -291,6 +291,9 @@ def block_sum(inputs: Sequence[torch.Tensor], block_list: torch.Tensor, num: int
 # plan and its tensors for as long as it is replayed.
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# (torch.cuda.current_stream(i).cuda_stream and torch.cuda.current_device(), without the objects they make)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 class _Call:
@@ -305,14 +308,14 @@ class _Call:
             raise ValueError("expected a device (HIP) tensor")
         self.device, self.index, self.stream, self._guard = device, device.index, stream, None
         if stream is None:
-            self.ptr = torch._C._cuda_getCurrentRawStream(self.index)
+            self.ptr = _raw_stream(self.index)
         elif stream.device != device:
             raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
         else:
             self.ptr = stream.cuda_stream
 
     def __enter__(self):
-        if torch._C._cuda_getDevice() != self.index:
+        if _current_device() != self.index:
             self._guard = torch.cuda.device(self.device)
             self._guard.__enter__()
         return self

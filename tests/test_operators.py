@@ -74,8 +74,8 @@ def loss_grad(**k):
     (loss, dict(dt=0), "bf16 or fp16"), (loss, dict(dim=0), "dim"), (loss, dict(dim=(1 << 20) + 1), "dim"),
     (loss, dict(vocab=0), "vocab"), (loss, dict(vocab=1 << 31), "vocab"), (loss, dict(n=1 << 31), "tokens"),
     (loss, dict(t=None), "NULL"), (loss, dict(lse=None), "NULL"), (loss, dict(ws=None), "workspace"),
-    (loss, dict(bytes=100), "workspace of 100 bytes"), (loss, dict(wstride=9, bytes=700), "pack"),
-    (loss, dict(w=A + 2, bytes=700), "pack"),
+    (loss, dict(bytes=100), "workspace of 100 bytes"), (loss, dict(wstride=9, bytes=(4 << 20) + 1100), "pack"),
+    (loss, dict(w=A + 2, bytes=(4 << 20) + 1100), "pack"),
     (loss_grad, dict(dt=0), "bf16 or fp16"), (loss_grad, dict(gwd=2), "grad_weight"), (loss_grad, dict(ghs=7), "stride"),
     (loss_grad, dict(gws=7), "stride"), (loss_grad, dict(g=None), "NULL"), (loss_grad, dict(lse=None), "NULL"),
     (loss_grad, dict(bytes=1000), "workspace of 1000 bytes"),
