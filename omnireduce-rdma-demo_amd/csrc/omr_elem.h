@@ -14,11 +14,6 @@
 
 namespace omr_detail {
 int set_error(int code, const char* msg);
-// (omr_embed.hip) the positions of the ids that name a row, by row and in order within it: those of row v at
-// perm[start[v] .. start[v + 1]); start: rows + 1, perm: one an id.  named (one an id, or null): the rows of perm's
-// positions, ~0 behind the last.  An error code, or 0.
-int sort_ids(const void* ids, int ids64, uint32_t num_ids, uint32_t rows, uint32_t* start, uint32_t* perm,
-             uint32_t* named, hipStream_t stream);
 }  // namespace omr_detail
 
 namespace omr_elem {

@@ -9,7 +9,7 @@
 //
 // Every sum has a fixed order, so the same inputs give the same bits: tokens are grouped by a stable sort instead of
 // meeting in floating-point atomics.
-#include "omr_elem.h"
+#include "omr_sort.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -17,11 +17,6 @@
 using namespace omr_elem;
 
 namespace {
-
-template <class I>
-__device__ __forceinline__ bool id_ok(I id, uint32_t rows) {
-  return id >= 0 && static_cast<uint64_t>(id) < rows;
-}
 
 // ---------------------------------------------------------------- lookup
 //
@@ -66,133 +61,12 @@ __global__ __launch_bounds__(256) void k_embed(const T* table, uint32_t rows, ui
   }
 }
 
-// ---------------------------------------------------------------- sort
-//
-// Groups the tokens by row in ONE launch without any exchange between workgroups: workgroup p owns the rows
-// [p R, p R + R) and reads ALL ids itself (they sit in the L2s: 64 KiB for 8192 int64 ids), counting its own and how
-// many are below its range, which is where its piece of the sorted list begins.
-//   pass 1  wave w counts the ids of its contiguous sixteenth of the tokens in hist[w][id - lo], and notes the tokens it
-//           counted, in order, in a list of its own
-//   scan    start[v] = ids below v; hist[w][.] = where wave w's first token of that row goes
-//   pass 2  the waves walk their lists (or, where a list is full, their tokens again) and place them: within 64 tokens
-//           the lanes of equal ids rank themselves by lane (match by ballots over the bits of the local id), so the
-//           order within a row is token order; named[i], where it is wanted, is the row of the i-th of the sorted list
-// Every workgroup reads T ids: hidden in the L2 up to some 100 k tokens, where a radix sort would take three launches
-// for each of three digits.
-constexpr int kSortWaves = 16;
-constexpr int kSortRange = 1024;  // rows per workgroup at most: 64 KiB of histogram
-constexpr int kSortBits = 10;
-constexpr uint32_t kNoRow = ~0u;
-constexpr uint32_t kSortList = 512;  // tokens a wave notes: 32 KiB
-
 template <class I>
 __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, uint32_t tokens, uint32_t rows,
                                                                uint32_t range, uint32_t* start, uint32_t* perm,
                                                                uint32_t* named) {
-  __shared__ uint32_t hist[kSortWaves * kSortRange];
-  __shared__ uint32_t list[kSortWaves][kSortList];  // (token - the wave's first) << 10 | local id
-  __shared__ uint32_t wsum[kSortWaves], below_w[kSortWaves], valid;
-  const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const uint32_t lo = blockIdx.x * range, n = min(range, rows - lo);
-  for (uint32_t i = tid; i < kSortWaves * range; i += 64 * kSortWaves) hist[i] = 0;
-  const uint32_t span = (tokens + 64 * kSortWaves - 1) / (64 * kSortWaves) * 64;  // tokens of a wave
-  const uint32_t t0 = min(wave * span, tokens), t1 = min(t0 + span, tokens);
-  uint32_t* mine = hist + wave * range;
-  uint32_t below = 0, noted = 0;
-  __syncthreads();
-  constexpr int K = 8;  // loads in flight
-  for (uint32_t t = t0; t < t1; t += 64 * K) {
-    I id[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t at = t + 64 * k + lane;
-      id[k] = at < t1 ? ids[at] : static_cast<I>(-1);
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t v = id_ok(id[k], rows) ? static_cast<uint32_t>(id[k]) : ~0u;
-      below += v < lo;
-      const bool in = v - lo < n;
-      const uint64_t who = __ballot(in);
-      if (who == 0) continue;
-      const uint32_t at = noted + __popcll(who & ((1ull << lane) - 1));
-      if (in) {
-        atomicAdd(&mine[v - lo], 1u);
-        if (at < kSortList) list[wave][at] = (t + 64 * k + lane - t0) << kSortBits | (v - lo);
-      }
-      noted += static_cast<uint32_t>(__popcll(who));
-    }
-  }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) below += __shfl_xor(below, d);
-  if (lane == 0) below_w[wave] = below;
-  __syncthreads();
-  // exclusive scan over the range's rows of their totals, then over the waves within a row
-  uint32_t total = 0;
-  if (tid < n) {
-#pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) total += hist[w * range + tid];
-  }
-  uint32_t incl = total;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t up = __shfl_up(incl, d);
-    if (lane >= static_cast<uint32_t>(d)) incl += up;
-  }
-  if (lane == 63) wsum[wave] = incl;
-  __syncthreads();
-  uint32_t at = incl - total;
-#pragma unroll
-  for (uint32_t w = 0; w < kSortWaves; ++w) {
-    at += below_w[w];
-    if (w < wave) at += wsum[w];
-  }
-  if (tid < n) {
-    start[lo + tid] = at;
-    if (lo + tid == rows - 1) start[rows] = valid = at + total;
-#pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = hist[w * range + tid];
-      hist[w * range + tid] = at;
-      at += c;
-    }
-  }
-  __syncthreads();
-  // (a list holds token distances of 22 bits)
-  const bool listed = noted <= kSortList && span <= 1u << (32 - kSortBits);
-  const uint32_t steps = listed ? noted : t1 - t0;
-  for (uint32_t i = 0; i < steps; i += 64) {
-    uint32_t v = ~0u, t = t0 + i + lane;
-    if (i + lane < steps) {
-      if (listed) {
-        const uint32_t e = list[wave][i + lane];
-        v = e & (kSortRange - 1);
-        t = t0 + (e >> kSortBits);
-      } else if (id_ok(ids[t], rows)) {
-        v = static_cast<uint32_t>(ids[t]) - lo;
-      }
-    }
-    const bool in = v < n;
-    uint64_t same = __ballot(in);
-    if (same == 0) continue;
-#pragma unroll
-    for (int b = 0; b < kSortBits; ++b) {
-      const bool bit = (v >> b) & 1;
-      const uint64_t m = __ballot(bit);
-      same &= bit ? m : ~m;
-    }
-    const uint32_t leader = in ? static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(same))) - 1 : lane;
-    uint32_t base = 0;
-    if (in && lane == leader) base = atomicAdd(&mine[v], static_cast<uint32_t>(__popcll(same)));
-    base = __shfl(base, static_cast<int>(leader));
-    if (in) {
-      const uint32_t to = base + __popcll(same & ((1ull << lane) - 1));
-      perm[to] = t;
-      if (named != nullptr) named[to] = lo + v;
-    }
-  }
-  if (named != nullptr && lo + n == rows)  // behind the last
-    for (uint32_t i = valid + tid; i < tokens; i += 64 * kSortWaves) named[i] = kNoRow;
+  __shared__ SortSpace space;
+  sort_by_row<I>(space, blockIdx.x, ids, tokens, rows, range, start, perm, named);
 }
 
 // ---------------------------------------------------------------- sums
@@ -356,22 +230,6 @@ constexpr uint64_t kMaxBlocks = (1u << 24) - 1;  // of 256 threads: a launch hol
 
 }  // namespace
 
-namespace omr_detail {
-int sort_ids(const void* ids, int ids64, uint32_t num_ids, uint32_t rows, uint32_t* start, uint32_t* perm,
-             uint32_t* named, hipStream_t stream) {
-  // rows per workgroup: one workgroup a CU where the table is small enough for that
-  const uint32_t range = std::min<uint32_t>(std::max<uint32_t>(static_cast<uint32_t>(ceil_div(rows, 256)), 16), kSortRange);
-  const unsigned blocks = static_cast<unsigned>(ceil_div(rows, range));
-  if (ids64)
-    k_embed_sort<int64_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int64_t*>(ids), num_ids, rows, range,
-                                                                 start, perm, named);
-  else
-    k_embed_sort<int32_t><<<blocks, 64 * kSortWaves, 0, stream>>>(static_cast<const int32_t*>(ids), num_ids, rows, range,
-                                                                 start, perm, named);
-  return elaunch("sort by row");
-}
-}  // namespace omr_detail
-
 extern "C" {
 
 int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t dim, uint64_t row_stride,
@@ -450,8 +308,15 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   a.chunks = num_ids != 0 ? static_cast<uint32_t>(ceil_div(num_ids, kChunk)) : 0;
   a.scale = scale;
   a.accumulate = accumulate != 0;
-  if (const int rc = omr_detail::sort_ids(ids, ids64, a.tokens, a.rows, start, perm, named, S(stream)))
-    return rc;
+  const uint32_t range = sort_range(a.rows);
+  const unsigned sorters = static_cast<unsigned>(ceil_div(a.rows, range));
+  if (ids64)
+    k_embed_sort<int64_t><<<sorters, 64 * kSortWaves, 0, S(stream)>>>(static_cast<const int64_t*>(ids), a.tokens, a.rows,
+                                                                     range, start, perm, named);
+  else
+    k_embed_sort<int32_t><<<sorters, 64 * kSortWaves, 0, S(stream)>>>(static_cast<const int32_t*>(ids), a.tokens, a.rows,
+                                                                     range, start, perm, named);
+  if (const int rc = elaunch("omr_embed_grad_f32 (sort)")) return rc;
   return with_dtype(grad_dtype, [&](auto t) {
     using T = decltype(t);
     a.wide = dim % VEC == 0 && table_stride % VEC == 0 && aligned(grad_table, 16);

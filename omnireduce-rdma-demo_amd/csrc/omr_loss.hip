@@ -19,7 +19,7 @@
 //   - hidden[n] * (grad_loss[n] / max |grad_loss|) for grad_weight's sum over tokens: exact where grad_loss is the same
 //     for every token (the mean and the sum), else one rounding.
 // Sums are in fp32 throughout.
-#include "omr_elem.h"
+#include "omr_sort.h"
 
 #include <algorithm>
 #include <cmath>
@@ -197,8 +197,9 @@ struct GemmArgs {
   uint32_t dim;
   float* acc;               // [splits][tokens][dim]
   int first, last;          // the sum over the pieces begins; is complete and goes to `out`
-  const float* rowscale;    // [tokens]
-  const float* amax;        // [1]
+  const float* up;          // grad_loss, upstride apart
+  uint64_t upstride;
+  const float* amax;        // [1] the largest |grad_loss| of the tokens with a target
   float* lost;              // [tokens] what the target's entry of G lost in rounding
   Operand<T> w;             // kHidden: the whole weight
   const uint32_t *start, *perm;  // kWeight: the tokens by target
@@ -211,6 +212,12 @@ template <class T>
 __device__ __forceinline__ int target_of(const GemmArgs<T>& a, uint32_t n) {
   const int64_t t = a.targets64 ? static_cast<const int64_t*>(a.targets)[n] : static_cast<const int32_t*>(a.targets)[n];
   return t >= 0 && t < a.vocab ? static_cast<int>(t) : -1;
+}
+
+// a token's factor: its grad_loss, 0 without a target (whatever grad_loss holds)
+template <class T>
+__device__ __forceinline__ float factor_of(const GemmArgs<T>& a, uint32_t n) {
+  return target_of(a, n) >= 0 ? a.up[n * a.upstride] : 0.0f;
 }
 
 // (maximum, sum of exp(. - maximum)) of two parts together; a part of nothing is (-inf, 0)
@@ -512,7 +519,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
     for (int j = 0; j < NF; ++j) {
       const uint32_t tok = n + 16 * j;
       const bool real = tok < a.tokens;
-      const float scale = real && a.last ? a.rowscale[tok] : 0.0f;
+      const float scale = real && a.last ? factor_of(a, tok) * (1.0f / kGScale) : 0.0f;
       const int target = real && a.last ? target_of(a, tok) : -1;
       const float lost = target >= 0 ? a.lost[tok] : 0.0f;
 #pragma unroll
@@ -739,51 +746,84 @@ __global__ __launch_bounds__(256) void k_merge(GemmArgs<T> a, float* loss, float
   loss[tok] = target_of(a, tok) >= 0 ? l - a.ztarget[tok] : 0.0f;
 }
 
-// The largest |grad_loss| of the tokens with a target (one workgroup), and each token's factor of grad_hidden.
+// The largest |grad_loss| of the tokens with a target, in every thread of a workgroup of 1024.  (A NaN counts as the
+// largest: the gradient shall have it.)
 template <class T>
-__global__ __launch_bounds__(1024) void k_scales(GemmArgs<T> a, const float* grad_loss, uint64_t stride, float* amax,
-                                                 float* rowscale) {
-  __shared__ float top[16];
+__device__ __forceinline__ float largest(const GemmArgs<T>& a, float* lds) {
   float m = 0.0f;
-  for (uint64_t n0 = threadIdx.x; n0 < a.tokens; n0 += 8 * 1024) {  // eight tokens in flight
-    float g[8];
+  auto more = [&](float g) { m = m != m || g <= m ? m : g; };
+  for (uint64_t n0 = threadIdx.x; n0 < a.tokens; n0 += 4 * 1024) {  // four tokens in flight
+    float g[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const uint64_t n = n0 + i * 1024;
-      g[i] = n < a.tokens && target_of(a, static_cast<uint32_t>(n)) >= 0 ? grad_loss[n * stride] : 0.0f;
+      g[i] = n < a.tokens ? fabsf(factor_of(a, static_cast<uint32_t>(n))) : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (n0 + i * 1024 < a.tokens) rowscale[n0 + i * 1024] = g[i] / kGScale;
-      // (a NaN is kept: the gradient shall have it)
-      m = m != m || fabsf(g[i]) <= m ? m : fabsf(g[i]);
-    }
+    for (int i = 0; i < 4; ++i) more(g[i]);
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float o = __shfl_xor(m, d);
-    m = m != m || o <= m ? m : o;
-  }
-  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+  for (int d = 32; d; d >>= 1) more(__shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int w = 1; w < 16; ++w) m = m != m || top[w] <= m ? m : top[w];
-  *amax = m;
+  m = lds[0];
+  for (int w = 1; w < 16; ++w) more(lds[w]);
+  return m;
 }
 
-// Rows copied into whole 16-byte pieces [rows][pdim], zeros behind dim; 2^lpr_log lanes a row.  With rowscale: each row
-// times its share of the largest grad_loss, and zeros for tokens without a target, whatever they hold.
+template <class T>
+__global__ __launch_bounds__(1024) void k_largest(GemmArgs<T> a, float* amax) {
+  __shared__ float lds[16];
+  const float m = largest(a, lds);
+  if (threadIdx.x == 0) *amax = m;
+}
+
+// Rows copied into whole 16-byte pieces [rows][pdim], zeros behind dim; 2^lpr_log lanes a row.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const T* src, uint64_t stride, uint32_t rows, uint32_t dim, uint32_t pdim,
-                                              uint32_t lpr_log, const float* rowscale, const float* amax, T* dst) {
+                                              uint32_t lpr_log, T* dst) {
   const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x) >> lpr_log;
   if (row >= rows) return;
-  float by = 1.0f;
-  if (rowscale != nullptr) by = rowscale[row] == 0.0f ? 0.0f : rowscale[row] * kGScale / *amax;
+  for (uint32_t c = (threadIdx.x & ((1u << lpr_log) - 1)) * 8; c < pdim; c += 8u << lpr_log) {
+    float v[8];
+    load_some<T, 8>(src + row * stride + c, dim - c, v);
+    store_f32<T, 8>(dst + row * pdim + c, v);
+  }
+}
+
+// What grad_weight's product needs, in one launch: blocks [0, sorters) sort the tokens by target; the others copy the
+// hidden states into whole pieces as k_pack does, each row times its share of the largest grad_loss, and zeros for tokens
+// without a target, whatever they hold.  Up to kFindHere tokens each of these finds the largest itself: a launch less,
+// 3 to 4 us of a backward pass up to 2048 tokens, nothing at 6000 to 8192, and 12 us lost at 16384, where every block
+// would read that many.
+constexpr uint32_t kFindHere = 4096;
+
+template <class T, class I>
+__global__ __launch_bounds__(64 * kSortWaves) void k_prepare(GemmArgs<T> a, uint32_t sorters, uint32_t range,
+                                                             uint32_t* start, uint32_t* perm, const T* src,
+                                                             uint64_t stride, uint32_t pdim, uint32_t lpr_log,
+                                                             float* amax, T* dst) {
+  static_assert(kSortWaves == 16, "largest() takes 1024 threads");
+  __shared__ SortSpace space;
+  if (blockIdx.x < sorters) {
+    sort_by_row<I>(space, blockIdx.x, static_cast<const I*>(a.targets), a.tokens, a.vocab, range, start, perm, nullptr);
+    return;
+  }
+  const uint32_t block = blockIdx.x - sorters;
+  float most;
+  if (a.tokens <= kFindHere) {
+    most = largest(a, reinterpret_cast<float*>(space.wsum));
+    if (block == 0 && threadIdx.x == 0) *amax = most;
+  } else {
+    most = *amax;
+  }
+  const uint64_t row = (static_cast<uint64_t>(block) * 1024 + threadIdx.x) >> lpr_log;
+  if (row >= a.tokens) return;
+  const float g = factor_of(a, static_cast<uint32_t>(row)), by = g == 0.0f ? 0.0f : g / most;
   for (uint32_t c = (threadIdx.x & ((1u << lpr_log) - 1)) * 8; c < pdim; c += 8u << lpr_log) {
     float v[8] = {};
     if (by != 0.0f) {
-      load_some<T, 8>(src + row * stride + c, dim - c, v);
+      load_some<T, 8>(src + row * stride + c, a.dim - c, v);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] *= by;
     }
@@ -801,7 +841,7 @@ __global__ __launch_bounds__(256) void k_join(GemmArgs<T> a) {
   for (uint32_t s = 0; s < a.splits; ++s) v += a.acc[s * all + i];
   const int target = target_of(a, tok);
   if (target >= 0) v += a.lost[tok] * static_cast<float>(a.w.p[target * a.w.ld + c]);
-  const float scale = a.rowscale[tok];
+  const float scale = factor_of(a, tok) * (1.0f / kGScale);
   static_cast<T*>(a.out)[tok * a.ostride + c] = static_cast<T>(scale == 0.0f ? 0.0f : v * scale);
 }
 
@@ -885,7 +925,7 @@ Space layout(uint64_t tokens, uint64_t vocab, uint64_t dim, bool pack, bool grad
   s.h = s.w + (pack ? up(vocab * pdim * 2, 256) : 0);
   s.rest = s.h + (pack ? up(tokens * pdim * 2, 256) : 0);
   uint64_t fwd = up(tokens * 4, 256) + stats_bytes_most(tokens, vocab);
-  uint64_t bwd = 256 + 3 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) +
+  uint64_t bwd = 256 + 2 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) +
                  up(piece_bytes_most(tokens, vocab), 256) + acc_bytes_most(tokens, dim);
   s.bytes = s.rest + (grads ? std::max(fwd, bwd) : fwd) + 256;
   return s;
@@ -901,17 +941,19 @@ int check(const char* what, int dtype, uint64_t tokens, uint64_t vocab, uint32_t
   return 0;
 }
 
+uint32_t lanes_log(uint32_t pdim) {  // lanes that a row of pdim elements fills, a power of two up to a wave
+  uint32_t l = 0;
+  while (l < 6 && (8u << l) < pdim) ++l;
+  return l;
+}
+
 template <class T>
-int pack_rows(const void* src, uint64_t stride, uint64_t rows, uint32_t dim, const float* rowscale, const float* amax,
-              T* dst, hipStream_t stream) {
-  const uint32_t pdim = static_cast<uint32_t>(up(dim, 8));
-  uint32_t lpr_log = 0;
-  while (lpr_log < 6 && (8u << lpr_log) < pdim) ++lpr_log;
+int pack_rows(const void* src, uint64_t stride, uint64_t rows, uint32_t dim, T* dst, hipStream_t stream) {
+  const uint32_t pdim = static_cast<uint32_t>(up(dim, 8)), lpr_log = lanes_log(pdim);
   const uint64_t blocks = ceil_div(rows, 256u >> lpr_log);
   if (blocks >= (1u << 24)) return efail("vocab_loss: too many rows to lay out in one call");
   k_pack<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T*>(src), stride,
-                                                               static_cast<uint32_t>(rows), dim, pdim, lpr_log, rowscale,
-                                                               amax, dst);
+                                                               static_cast<uint32_t>(rows), dim, pdim, lpr_log, dst);
   return elaunch("omr_vocab_loss (layout)");
 }
 
@@ -924,13 +966,13 @@ int operands(const void* hidden, uint64_t hstride, const void* weight, uint64_t 
   *w = {static_cast<const T*>(weight), wstride, static_cast<uint32_t>(vocab)};
   if (dim % 8 != 0 || !rows_ok(weight, wstride)) {
     T* to = reinterpret_cast<T*>(ws + sp.w);
-    if (const int rc = pack_rows<T>(weight, wstride, vocab, dim, nullptr, nullptr, to, stream)) return rc;
+    if (const int rc = pack_rows<T>(weight, wstride, vocab, dim, to, stream)) return rc;
     w->p = to;
     w->ld = pdim;
   }
   if (dim % 8 != 0 || !rows_ok(hidden, hstride)) {
     T* to = reinterpret_cast<T*>(ws + sp.h);
-    if (const int rc = pack_rows<T>(hidden, hstride, tokens, dim, nullptr, nullptr, to, stream)) return rc;
+    if (const int rc = pack_rows<T>(hidden, hstride, tokens, dim, to, stream)) return rc;
     h->p = to;
     h->ld = pdim;
   }
@@ -1053,7 +1095,6 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
       return p;
     };
     float* amax = reinterpret_cast<float*>(take(4));
-    float* rowscale = reinterpret_cast<float*>(take(tokens * 4));
     float* lost = reinterpret_cast<float*>(take(tokens * 4));
     uint32_t* perm = reinterpret_cast<uint32_t*>(take(tokens * 4));
     uint32_t* start = reinterpret_cast<uint32_t*>(take(4 * vocab + 4));
@@ -1066,20 +1107,30 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     a.vocab = static_cast<uint32_t>(vocab);
     a.tokens = static_cast<uint32_t>(tokens);
     a.dim = dim;
-    k_scales<T><<<1, 1024, 0, S(stream)>>>(a, grad_loss, grad_loss_stride, amax, rowscale);
-    if (const int rc = elaunch("omr_vocab_loss_grad (scales)")) return rc;
+    a.up = grad_loss;
+    a.upstride = grad_loss_stride;
+    a.amax = amax;
     if (grad_weight != nullptr) {
-      if (const int rc = pack_rows<T>(hidden, hidden_stride, tokens, dim, rowscale, amax, clean, S(stream))) return rc;
-      if (const int rc = omr_detail::sort_ids(targets, targets64, a.tokens, a.vocab, start, perm, nullptr, S(stream)))
-        return rc;
+      if (tokens > kFindHere) {
+        k_largest<T><<<1, 1024, 0, S(stream)>>>(a, amax);
+        if (const int rc = elaunch("omr_vocab_loss_grad (largest)")) return rc;
+      }
+      const uint32_t range = sort_range(a.vocab), lpr_log = lanes_log(pdim);
+      const uint64_t sorters = ceil_div(vocab, range), blocks = sorters + ceil_div(tokens, 1024u >> lpr_log);
+      if (blocks >= (1u << 22)) return efail("vocab_loss_grad: too many tokens or rows for one call");
+      auto prepare = [&](auto i) {
+        k_prepare<T, decltype(i)><<<static_cast<unsigned>(blocks), 64 * kSortWaves, 0, S(stream)>>>(
+            a, static_cast<uint32_t>(sorters), range, start, perm, static_cast<const T*>(hidden), hidden_stride, pdim,
+            lpr_log, amax, clean);
+        return elaunch("omr_vocab_loss_grad (prepare)");
+      };
+      if (const int rc = targets64 ? prepare(int64_t{}) : prepare(int32_t{})) return rc;
     }
     const uint32_t piece = piece_rows(tokens, vocab);
     a.lse = lse;
     a.g = g;
     a.ldg = piece;
     a.acc = acc;
-    a.rowscale = rowscale;
-    a.amax = amax;
     a.lost = lost;
     a.w = w;
     a.start = start;

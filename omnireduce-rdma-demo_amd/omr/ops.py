@@ -332,7 +332,7 @@ class _Call:
             return torch.empty(shape, dtype=dtype, device=self.device)
 
     def on(self, t: torch.Tensor, name: str) -> int:
-        if not t.is_cuda or t.get_device() != self.index:
+        if t.get_device() != self.index:  # (-1: not on a device)
             raise ValueError(f"{name} is on {t.device}, expected {self.device}")
         return t.data_ptr()
 
