@@ -469,8 +469,8 @@ int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t di
 /* Its gradient: grad_table[v, :] = scale * (sum over the t with ids[t] == v, in order of t, of grad_out[t, :]), fp32;
  * every row of grad_table is written (zeros where no token names it), or, with accumulate != 0, the sums are added to
  * the rows that tokens name and the others are left as they are.  Tokens whose id names no row are skipped, whatever
- * their row of grad_out holds.  (A row of many tokens is summed in chunks of at most 16, which
- * are then added up.) */
+ * their row of grad_out holds.  (A row of many tokens is summed in chunks of at most 16, which are
+ * then added up.) */
 size_t omr_embed_grad_workspace_bytes(uint64_t num_ids, uint64_t num_rows, uint32_t dim);
 int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_stride, const void* ids, int ids64,
                        uint64_t num_ids, uint64_t num_rows, uint32_t dim, float scale, float* grad_table,
@@ -496,7 +496,7 @@ int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* 
 
 /* Softmax cross entropy over a large vocabulary, without keeping the logits z = hidden weight^T:
  *   lse[n] = log(sum over v of exp(z[n, v])),  loss[n] = lse[n] - z[n, targets[n]]     (fp32, both required)
- * hidden [tokens, dim] and weight [vocab, dim]: bf16 or fp16 (`dtype`), dim <= 2^20.  targets: int32, or int64 with
+ * hidden [tokens, dim] and weight [vocab, dim]: bf16 or fp16 (`dtype`), dim <= 2^20, tokens < 2^26, vocab < 2^31 - 256.  targets: int32, or int64 with
  * targets64 != 0; a target outside [0, vocab) is none: its loss is 0 (its lse is still that of its row).
  * Rows of hidden and weight that are whole 16-byte pieces (dim, strides and addresses; strides below 2^22) are read as
  * they are; others are laid out again in the workspace by each call, which then has to be asked for with pack != 0 (a

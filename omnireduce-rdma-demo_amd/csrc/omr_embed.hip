@@ -308,6 +308,12 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   a.chunks = num_ids != 0 ? static_cast<uint32_t>(ceil_div(num_ids, kChunk)) : 0;
   a.scale = scale;
   a.accumulate = accumulate != 0;
+  a.wide = dim % VEC == 0 && table_stride % VEC == 0 && aligned(grad_table, 16);
+  a.tiles = static_cast<uint32_t>(ceil_div(dim, 256 * VEC));
+  const uint64_t chunk_blocks = static_cast<uint64_t>(a.chunks) * a.tiles, join_tiles = ceil_div(dim, 64 * VEC),
+                 blocks = chunk_blocks + (accumulate ? 0 : ceil_div(num_rows, 4 * kFillRows));
+  if (blocks > kMaxBlocks || a.chunks * join_tiles > kMaxBlocks)
+    return efail("embed_grad: too many tokens or rows for one call");
   const uint32_t range = sort_range(a.rows);
   const unsigned sorters = static_cast<unsigned>(ceil_div(a.rows, range));
   if (ids64)
@@ -319,18 +325,12 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   if (const int rc = elaunch("omr_embed_grad_f32 (sort)")) return rc;
   return with_dtype(grad_dtype, [&](auto t) {
     using T = decltype(t);
-    a.wide = dim % VEC == 0 && table_stride % VEC == 0 && aligned(grad_table, 16);
-    a.tiles = static_cast<uint32_t>(ceil_div(dim, 256 * VEC));
-    const uint64_t first = static_cast<uint64_t>(a.chunks) * a.tiles;
-    const uint64_t blocks = first + (accumulate ? 0 : ceil_div(num_rows, 4 * kFillRows));
-    if (blocks > kMaxBlocks) return efail("embed_grad: too many tokens or rows for one call");
     if (blocks == 0) return 0;
-    k_embed_sum<T><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(a, static_cast<uint32_t>(first));
+    k_embed_sum<T><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(a, static_cast<uint32_t>(chunk_blocks));
     if (const int rc = elaunch("omr_embed_grad_f32")) return rc;
     if (a.chunks <= 1) return 0;
-    const uint32_t tiles = static_cast<uint32_t>(ceil_div(dim, 64 * VEC));
-    if (static_cast<uint64_t>(a.chunks) * tiles > kMaxBlocks) return efail("embed_grad: too many tokens for one call");
-    k_embed_join<<<a.chunks * tiles, 256, 0, S(stream)>>>(a, tiles);
+    k_embed_join<<<static_cast<unsigned>(a.chunks * join_tiles), 256, 0, S(stream)>>>(
+        a, static_cast<uint32_t>(join_tiles));
     return elaunch("omr_embed_grad_f32 (join)");
   });
 }

@@ -847,8 +847,11 @@ __global__ __launch_bounds__(256) void k_join(GemmArgs<T> a) {
 
 template <class O>
 __global__ __launch_bounds__(256) void k_zero(O* out, uint64_t rows, uint32_t dim, uint64_t stride) {
-  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / dim;
-  if (row < rows) out[row * stride + (i - row * dim)] = static_cast<O>(0.0f);
+  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * dim;
+       i += static_cast<uint64_t>(gridDim.x) * 256) {
+    const uint64_t row = i / dim;
+    out[row * stride + (i - row * dim)] = static_cast<O>(0.0f);
+  }
 }
 
 // ---------------------------------------------------------------- launches
@@ -937,7 +940,7 @@ int check(const char* what, int dtype, uint64_t tokens, uint64_t vocab, uint32_t
   if (dtype != OMR_BF16 && dtype != OMR_F16) return efail("%s: hidden and weight are bf16 or fp16", what);
   if (dim == 0 || dim > (1u << 20)) return efail("%s: dim must be 1..%u", what, 1u << 20);
   if (vocab == 0 || vocab >= (1ull << 31) - 256) return efail("%s: vocab must be 1..2^31 - 257", what);
-  if (tokens >= (1ull << 31) - 256) return efail("%s: tokens must be below 2^31 - 256", what);
+  if (tokens >= (1ull << 26)) return efail("%s: tokens must be below 2^26", what);
   return 0;
 }
 
@@ -1066,8 +1069,7 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     return efail("vocab_loss_grad: NULL pointer");
   if (tokens == 0) {  // a sum over no tokens
     if (grad_weight == nullptr || accumulate) return 0;
-    const uint64_t blocks = ceil_div(vocab * dim, 256);
-    if (blocks >= (1u << 24)) return efail("vocab_loss_grad: the weight is too large for one call");
+    const uint64_t blocks = std::min<uint64_t>(ceil_div(vocab * dim, 256), 1u << 16);
     if (grad_weight_dtype == OMR_F32)
       k_zero<float><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(static_cast<float*>(grad_weight), vocab, dim,
                                                                           grad_weight_stride);

@@ -294,6 +294,13 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # (torch.cuda.current_stream(i).cuda_stream and torch.cuda.current_device(), without the objects they make)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_MAX_DIM = 1 << 24  # OMR_MAX_DIM
+
+
+def _sizes(count: int, rows: int, dim: int, least: int = 0):
+    """A plan's sizes are in range (the C calls take unsigned integers)."""
+    if not (0 <= count < 1 << 40 and least <= rows < 1 << 31 and 0 < dim <= _MAX_DIM):
+        raise ValueError(f"no such sizes: {count} tokens (rows), a table of {rows}, rows of {dim}")
 
 
 class _Call:
@@ -344,8 +351,8 @@ class _Call:
         ptr = self.on(t, name)
         shape = t.shape
         dims = len(shape)
-        if dims == 0 or shape[-1] == 0 or (dim is not None and shape[-1] != dim):
-            raise ValueError(f"{name}: rows of {dim if dim is not None else 'at least one'} elements expected, got "
+        if dims == 0 or not 0 < shape[-1] <= _MAX_DIM or (dim is not None and shape[-1] != dim):
+            raise ValueError(f"{name}: rows of {dim if dim is not None else f'1 to {_MAX_DIM}'} elements expected, got "
                              f"shape {tuple(shape)}")
         d = shape[-1]
         n = shape[0] if dims == 2 else t.numel() // d
@@ -407,6 +414,8 @@ def embed(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, out: Optio
             raise ValueError(f"table: expected [rows, dim], got shape {tuple(table.shape)}")
         tp, rows, dim, tstride = call.rows(table, "table")
         ip, ids64, n = call.ids(ids, "ids")
+        if out_dtype is not None and out_dtype not in _DTYPES:
+            raise ValueError(f"out_dtype: element type {out_dtype}")
         if out is None:
             out = call.empty((*ids.shape, dim), out_dtype if out_dtype is not None else table.dtype)
         op, _, _, ostride = call.rows(out, "out", dim, n, out_dtype, out=True)
@@ -419,6 +428,7 @@ class EmbedGradPlan:
     """The embedding table's fp32 gradient by sorted tokens, for at most max_tokens tokens a call."""
 
     def __init__(self, max_tokens: int, num_rows: int, dim: int, device="cuda"):
+        _sizes(max_tokens, num_rows, dim)
         self.max_tokens, self.num_rows, self.dim = max_tokens, num_rows, dim
         self.workspace = _Workspace(_lib.load().omr_embed_grad_workspace_bytes(max_tokens, num_rows, dim), device)
 
@@ -491,6 +501,7 @@ class LayerNormGradPlan:
     rows a call."""
 
     def __init__(self, max_rows: int, dim: int, device="cuda"):
+        _sizes(max_rows, 0, dim)
         self.max_rows, self.dim = max_rows, dim
         self.workspace = _Workspace(_lib.load().omr_layer_norm_grad_workspace_bytes(max_rows, dim), device)
 
@@ -538,8 +549,7 @@ class VocabLossPlan:
                  grads: bool = True, pack: bool = False):
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"dtype: bfloat16 or float16, got {dtype}")
-        if min(max_tokens, vocab, dim) < 0 or vocab == 0 or dim == 0:
-            raise ValueError(f"no such sizes: {max_tokens} tokens, vocab {vocab}, dim {dim}")
+        _sizes(max_tokens, vocab, dim, least=1)
         self.max_tokens, self.vocab, self.dim, self.dtype, self.grads = max_tokens, vocab, dim, dtype, grads
         self.workspace = _Workspace(_lib.load().omr_vocab_loss_workspace_bytes(max_tokens, vocab, dim, int(pack),
                                                                                int(grads)), device)

@@ -117,6 +117,8 @@ def test_embed_strides_shape_and_untouched_memory(gpu, dim, pad, offset, dtype):
 def test_embed_empty_and_far(gpu):
     table = torch.ones(4, 8, device="cuda")
     assert ops.embed(table, torch.empty(0, dtype=torch.int64, device="cuda")).shape == (0, 8)
+    with pytest.raises(ValueError, match="out_dtype"):
+        ops.embed(table, torch.tensor([1], device="cuda"), out_dtype=torch.int32)
     none = torch.empty(0, 8, device="cuda")
     assert not ops.embed(none, torch.tensor([0, 1], device="cuda")).any()
     # offsets past 2^32 elements: a table of 2^21 + 3 rows of 2050 in bf16 (8 GiB)
@@ -425,6 +427,46 @@ def test_vocab_loss(gpu, T, V, D, dtype):
         assert none is None and torch.equal(gh2, gh)
         again = plan.backward(hn, w, t, ll, upn)
         assert torch.equal(again[0], gh) and torch.equal(again[1], gw)  # the same bits
+
+
+@pytest.mark.parametrize("T,V,D", [(5, 300, 64), (150, 700, 200)])
+def test_vocab_loss_grad_is_the_slope(gpu, T, V, D):
+    """The forward's own differences against the gradient: for two points of the type a and b, loss(b) - loss(a) is the
+    mean of both ends' gradients along b - a, but for a third derivative.  Along a line of logits z + s dz that of
+    log sum exp is a third central moment of dz under the softmax: at most R^3 / (6 sqrt 3) for values in a range of R;
+    the trapezoid is off by a twelfth of it."""
+    g = gen(T)
+    h, w, t, off = loss_inputs(T, V, D, BF16, g, none=0.0)
+    plan = ops.VocabLossPlan(T, V, D)
+    one = torch.ones(T, device="cuda")
+    h2 = (h.float() + 0.05 * rand((T, D), F32, g)).to(BF16)
+    w2 = (w.float() + 0.05 * D ** -0.5 * rand((V, D), F32, g)).to(BF16)
+    tols = [loss_ref(a, b, t, off)[3].sum() for a, b in ((h, w), (h2, w), (h, w2))]
+    la, lse_a = plan.forward(h, w, t)
+    for which, (hb, wb) in enumerate(((h2, w), (h, w2))):
+        lb, lse_b = plan.forward(hb, wb, t)
+        ga = plan.backward(h, w, t, lse_a, one, grad_weight=torch.empty(V, D, device="cuda"))[which].double()
+        gb = plan.backward(hb, wb, t, lse_b, one, grad_weight=torch.empty(V, D, device="cuda"))[which].double()
+        d = (hb.double() - h.double()) if which == 0 else (wb.double() - w.double())
+        along = ((ga + gb) / 2 * d).sum()
+        dz = (d @ w.double().t()) if which == 0 else h.double() @ d.t()
+        R = dz.amax(1) - dz.amin(1)
+        # the gradients' own error: every entry of G rounded to bf16 (sum |G| <= 2 a token), and grad_hidden's rounding
+        most = dz.abs().amax(1)
+        err = (2 * most * (half(BF16) * 1.1 + (V + T + 8) * U)).sum() + (half(BF16) * ((ga.abs() + gb.abs()) / 2 * d.abs()).sum())
+        tol = (R ** 3).sum() / (12 * 6 * 3 ** 0.5) + err + tols[0] + tols[1 + which]
+        diff = (lb.double() - la.double()).sum()
+        assert (diff - along).abs() <= tol, (which, diff.item(), along.item(), tol.item())
+        assert tol < 0.2 * d.norm() * ga.norm()  # (the bound says something)
+
+
+def test_vocab_loss_grad_of_no_tokens_and_a_large_weight(gpu):
+    """Zeros into more than 2^32 elements."""
+    plan = ops.VocabLossPlan(0, 65537, 65536)
+    out = torch.ones(65537, 65536, dtype=BF16, device="cuda")
+    plan.backward(out[:0], out, torch.empty(0, dtype=torch.int64, device="cuda"), torch.empty(0, device="cuda"),
+                  torch.empty(0, device="cuda"), grad_weight=out)
+    assert not any(out[i:i + 8192].any() for i in range(0, 65537, 8192))
 
 
 def test_vocab_loss_no_targets_no_tokens_and_one_factor(gpu):

@@ -73,6 +73,8 @@ def loss_grad(**k):
     (norm_grad, dict(ws=A + 4), "aligned"), (norm_grad, dict(bytes=0), "workspace of 0 bytes"),
     (loss, dict(dt=0), "bf16 or fp16"), (loss, dict(dim=0), "dim"), (loss, dict(dim=(1 << 20) + 1), "dim"),
     (loss, dict(vocab=0), "vocab"), (loss, dict(vocab=1 << 31), "vocab"), (loss, dict(n=1 << 31), "tokens"),
+    (loss, dict(n=1 << 26), "2^26"), (loss_grad, dict(n=1 << 26), "2^26"),
+    (embed_grad, dict(n=(1 << 31) - 1, bytes=1 << 50), "too many"),
     (loss, dict(t=None), "NULL"), (loss, dict(lse=None), "NULL"), (loss, dict(ws=None), "workspace"),
     (loss, dict(bytes=100), "workspace of 100 bytes"), (loss, dict(wstride=9, bytes=(4 << 20) + 1100), "pack"),
     (loss, dict(w=A + 2, bytes=(4 << 20) + 1100), "pack"),
@@ -115,3 +117,9 @@ def test_the_front_end_refuses():
         ops.VocabLossPlan(4, 10, 8, dtype=torch.float32)
     with pytest.raises(ValueError, match="sizes"):
         ops.VocabLossPlan(4, 0, 8)
+    for make in (lambda: ops.EmbedGradPlan(-1, 10, 8), lambda: ops.EmbedGradPlan(4, 1 << 31, 8),
+                 lambda: ops.EmbedGradPlan(4, 10, (1 << 32) + 8), lambda: ops.LayerNormGradPlan(-2, 8),
+                 lambda: ops.LayerNormGradPlan(4, 0), lambda: ops.VocabLossPlan(4, -1, 8),
+                 lambda: ops.VocabLossPlan(4, 10, 1 << 40)):
+        with pytest.raises(ValueError, match="sizes"):
+            make()
