@@ -10,7 +10,7 @@
 // several rows, so the parameters are loaded once, the next row is loaded while one is worked on, and the backward keeps
 // its part of dw and db in registers until its last row: one partial row a workgroup, which a second launch adds up in a
 // fixed order.  16384 rows of 4096 bf16 forward: 50 us, 5.4 TB/s (62 without the row ahead; a large copy reaches 5.1);
-// 16384 of 2048 backward: 49 us, 4.1 TB/s, 4 of it the second launch.
+// 16384 of 2048 backward: 42 us, 4.8 TB/s, 3 of it the second launch; 65536 of 1024: 75 us, 5.4 TB/s.
 // Rows of more than 16384 columns take the *_any kernels, which read a row again instead of holding it.
 #include "omr_elem.h"
 
@@ -67,9 +67,13 @@ struct Piece {
       for (int i = 0; i < VEC; ++i) v[i] = static_cast<uint32_t>(i) < n ? p[i] : static_cast<T>(0.0f);
     }
   }
+
+  __device__ __forceinline__ void arrive() { asm volatile("" : "+v"(v)); }  // it is waited for here
 };
 
-// Columns there are from c on: all VEC of them where rows are whole pieces (END false), known when compiling
+// Columns there are from c on: all VEC of them where rows are whole pieces (END false), known when compiling.
+// Lanes behind the end of such a row (in() false) hold its last piece once more (at()), write the same results to the same
+// place, and count in no sum: so neither loads nor stores need a branch.
 template <int VEC, bool END>
 __device__ __forceinline__ uint32_t have(uint32_t dim, uint32_t c) {
   return END ? dim - c : VEC;
@@ -82,6 +86,8 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
   // a lane's columns: VEC consecutive ones of every piece j
   const uint32_t t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
   auto col = [&](int j) { return (static_cast<uint32_t>(j) * 64 * WPR + t) * VEC; };
+  auto in = [&](int j) { return col(j) < a.dim; };
+  auto at = [&](int j) { return END ? col(j) : min(col(j), a.dim - VEC); };
   float w[NV][VEC], b[NV][VEC];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -90,78 +96,91 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
       w[j][i] = 1.0f;
       b[j][i] = 0.0f;
     }
-    if (col(j) >= a.dim) continue;
-    const uint32_t n = have<VEC, END>(a.dim, col(j));
-    if (a.w != nullptr) load_some<P, VEC>(static_cast<const P*>(a.w) + col(j), n, w[j]);
-    if (a.b != nullptr) load_some<P, VEC>(static_cast<const P*>(a.b) + col(j), n, b[j]);
+    if (END && !in(j)) continue;
+    const uint32_t n = have<VEC, END>(a.dim, at(j));
+    if (a.w != nullptr) load_some<P, VEC>(static_cast<const P*>(a.w) + at(j), n, w[j]);
+    if (a.b != nullptr) load_some<P, VEC>(static_cast<const P*>(a.b) + at(j), n, b[j]);
   }
-  // the next row is on its way while this one is worked on
+  // The next row is on its way while this one is worked on: loads and stores without a branch (a register that a branch
+  // may leave as it was is waited for and copied at once), and waited for behind this row's stores, whose number is known
+  // there, so that the stores need not be done.
   Piece<T, VEC> ahead[NV];
-  auto fetch = [&](uint64_t row) {
-    const T* p = static_cast<const T*>(a.x) + row * a.xstride;
+  auto arrive = [&]() {
+    if constexpr (!END) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (col(j) < a.dim) ahead[j].load(p + col(j), have<VEC, END>(a.dim, col(j)));
+      for (int j = 0; j < NV; ++j) ahead[j].arrive();
     }
+  };
+  auto fetch = [&](uint64_t row) {
+    const T* p = static_cast<const T*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.xstride;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (!END || in(j)) ahead[j].load(p + at(j), have<VEC, END>(a.dim, at(j)));
   };
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * RPB;
   uint64_t row = static_cast<uint64_t>(blockIdx.x) * RPB + (WPR == 1 ? threadIdx.x >> 6 : 0);
-  if (row < a.rows) fetch(row);
+  if (!END || row < a.rows) fetch(row);
+  arrive();
   for (; row < a.rows; row += step) {
     float v[NV][VEC];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = col(j) < a.dim ? static_cast<float>(ahead[j].v[i]) : 0.0f;
-    if (row + step < a.rows) fetch(row + step);
+      for (int i = 0; i < VEC; ++i) v[j][i] = !END || in(j) ? static_cast<float>(ahead[j].v[i]) : 0.0f;
+    if (!END || row + step < a.rows) fetch(row + step);
     float s = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      float piece = 0.0f;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s += v[j][i];
+      for (int i = 0; i < VEC; ++i) piece += v[j][i];
+      s += in(j) ? piece : 0.0f;
+    }
     const float mean = row_sum<WPR>(s, lds[0]) * a.inv_dim;
     float q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (col(j) < a.dim) {
+      float piece = 0.0f;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          v[j][i] = !END || col(j) + i < a.dim ? v[j][i] - mean : 0.0f;
-          q += v[j][i] * v[j][i];
-        }
+      for (int i = 0; i < VEC; ++i) {
+        v[j][i] = !END || col(j) + i < a.dim ? v[j][i] - mean : 0.0f;
+        piece += v[j][i] * v[j][i];
       }
+      q += in(j) ? piece : 0.0f;
     }
     const float rstd = 1.0f / sqrtf(row_sum<WPR>(q, lds[1]) * a.inv_dim + a.eps);
     T* out = static_cast<T*>(a.out) + row * a.ostride;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (col(j) < a.dim) {
+      if (END && !in(j)) continue;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * rstd * w[j][i] + b[j][i];
-        stream_some<T, VEC>(out + col(j), have<VEC, END>(a.dim, col(j)), v[j]);
-      }
+      for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * rstd * w[j][i] + b[j][i];
+      stream_some<T, VEC>(out + at(j), have<VEC, END>(a.dim, at(j)), v[j]);
     }
     if (WPR == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
+    arrive();
   }
 }
 
 // A workgroup of 8 waves holds 8 / WPR rows at a time (WPR 16: one row of 16 waves), in lockstep where a row is more
-// than a wave.
+// than a wave.  Registers for one workgroup a CU (see grad_blocks), or for two where rows end inside a piece.
 template <class T, class P, int WPR, bool END>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 512, 4) void k_norm_grad(NormArgs a) {
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 512, WPR == 16 || END ? 4 : 2) void k_norm_grad(NormArgs a) {
   constexpr int VEC = 16 / sizeof(T), NV = kCols / VEC, RPB = WPR == 16 ? 1 : 8 / WPR, WAVES = RPB * WPR, NT = 64 * WAVES;
   __shared__ float lds[2][2][WAVES];
   __shared__ float sum[RPB > 1 ? WAVES * 64 * kCols : 1];
-  const uint32_t wave = threadIdx.x >> 6, slot = wave / WPR, t = threadIdx.x - slot * 64 * WPR;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = wave / WPR,
+                 t = threadIdx.x - slot * 64 * WPR;
   auto col = [&](int j) { return (static_cast<uint32_t>(j) * 64 * WPR + t) * VEC; };
+  auto in = [&](int j) { return col(j) < a.dim; };
+  auto at = [&](int j) { return END ? col(j) : min(col(j), a.dim - VEC); };
   float dw[NV][VEC] = {}, db[NV][VEC] = {};
-  // Rows of 16-bit elements: the next row is on its way while this one is worked on (fp32 has no registers for that).
-  // The weight waits in LDS (a lane's columns together): with it in registers a CU holds half the waves (58 us against 49
-  // at 16384 x 2048 bf16).
-  constexpr bool kAhead = sizeof(T) == 2 && WPR <= 8;
+  // The next row is on its way while this one is worked on, where there are registers for it (8192 x 2048 fp32: 41 us
+  // against 46).  The weight waits in LDS (a lane's columns together).
+  constexpr bool kAhead = WPR <= 8 && (sizeof(T) == 2 || !END);
   __shared__ __attribute__((aligned(16))) float w[64 * WPR * kCols];
   if (slot == 0) {
 #pragma unroll
@@ -169,60 +188,74 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512, 4) void k_norm_grad(NormArg
       float f[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) f[i] = 1.0f;
-      if (a.w != nullptr && col(j) < a.dim)
-        load_some<P, VEC>(static_cast<const P*>(a.w) + col(j), have<VEC, END>(a.dim, col(j)), f);
+      if (a.w != nullptr && (!END || in(j)))
+        load_some<P, VEC>(static_cast<const P*>(a.w) + at(j), have<VEC, END>(a.dim, at(j)), f);
       store_f32<float, VEC>(&w[(j * 64 * WPR + t) * VEC], f);
     }
   }
   __syncthreads();
   Piece<T, VEC> xa[NV], da[NV];
+  float mean_a, rstd_a;
+  auto arrive = [&]() {
+    if constexpr (kAhead && !END) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        xa[j].arrive();
+        da[j].arrive();
+      }
+      asm volatile("" : "+v"(mean_a), "+v"(rstd_a));
+    }
+  };
   auto fetch = [&](uint64_t row) {
-    if (row >= a.rows) return;
+    row = row < a.rows ? row : a.rows - 1;
     const T* x = static_cast<const T*>(a.x) + row * a.xstride;
     const T* dy = static_cast<const T*>(a.dy) + row * a.dystride;
+    mean_a = a.mean[row];
+    rstd_a = a.rstd[row];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (col(j) < a.dim) {
-        xa[j].load(x + col(j), have<VEC, END>(a.dim, col(j)));
-        da[j].load(dy + col(j), have<VEC, END>(a.dim, col(j)));  // (zeros behind a row's end add nothing below)
+      if (!END || in(j)) {
+        xa[j].load(x + at(j), have<VEC, END>(a.dim, at(j)));
+        da[j].load(dy + at(j), have<VEC, END>(a.dim, at(j)));  // (zeros behind a row's end add nothing below)
       }
   };
   int flip = 0;
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * RPB;
   if (kAhead) fetch(static_cast<uint64_t>(blockIdx.x) * RPB + slot);
+  arrive();
   for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * RPB; first < a.rows; first += step) {
     const uint64_t row = first + slot;
     const bool real = row < a.rows;
     float v[NV][VEC], g[NV][VEC];
-    float mean = 0.0f, rstd = 0.0f, s1 = 0.0f, s2 = 0.0f;
+    float s1 = 0.0f, s2 = 0.0f;
+    if (!kAhead) fetch(row);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        v[j][i] = static_cast<float>(xa[j].v[i]);
+        g[j][i] = static_cast<float>(da[j].v[i]);
+      }
+    const float mean = mean_a, rstd = rstd_a;
+    if (kAhead) fetch(row + step);
     if (real) {
-      if (!kAhead) fetch(row);
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          v[j][i] = static_cast<float>(xa[j].v[i]);
-          g[j][i] = static_cast<float>(da[j].v[i]);
-        }
-      if (kAhead) fetch(row + step);
-      mean = a.mean[row];
-      rstd = a.rstd[row];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (col(j) < a.dim) {
-          float wj[VEC];
-          load_f32<float, VEC>(&w[(j * 64 * WPR + t) * VEC], wj);
+        if (END && !in(j)) continue;
+        float wj[VEC], p1 = 0.0f, p2 = 0.0f;
+        load_f32<float, VEC>(&w[(j * 64 * WPR + t) * VEC], wj);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float xh = (v[j][i] - mean) * rstd;
-            v[j][i] = xh;
-            dw[j][i] += g[j][i] * xh;
-            db[j][i] += g[j][i];
-            g[j][i] *= wj[i];
-            s1 += g[j][i];
-            s2 += g[j][i] * xh;
-          }
+        for (int i = 0; i < VEC; ++i) {
+          const float xh = (v[j][i] - mean) * rstd;
+          v[j][i] = xh;
+          dw[j][i] += g[j][i] * xh;
+          db[j][i] += g[j][i];
+          g[j][i] *= wj[i];
+          p1 += g[j][i];
+          p2 += g[j][i] * xh;
         }
+        s1 += in(j) ? p1 : 0.0f;
+        s2 += in(j) ? p2 : 0.0f;
       }
     }
     // both sums behind one barrier; the buffers alternate, so a wave that is a row ahead writes the other one
@@ -243,18 +276,21 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 512, 4) void k_norm_grad(NormArg
       }
       flip ^= 1;
     }
-    if (!real) continue;
+    if (!real) {
+      arrive();
+      break;
+    }
     s1 *= a.inv_dim;
     s2 *= a.inv_dim;
     T* out = static_cast<T*>(a.out) + row * a.ostride;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (col(j) < a.dim) {
+      if (END && !in(j)) continue;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) g[j][i] = (g[j][i] - s1 - v[j][i] * s2) * rstd;
-        stream_some<T, VEC>(out + col(j), have<VEC, END>(a.dim, col(j)), g[j]);
-      }
+      for (int i = 0; i < VEC; ++i) g[j][i] = (g[j][i] - s1 - v[j][i] * s2) * rstd;
+      stream_some<T, VEC>(out + at(j), have<VEC, END>(a.dim, at(j)), g[j]);
     }
+    arrive();  // (behind the stores, as in k_norm)
   }
   if (a.partial == nullptr) return;
   float* part = a.partial + static_cast<uint64_t>(blockIdx.x) * 2 * a.dim;
@@ -402,13 +438,15 @@ int waves_per_row(uint32_t dim) {
   return w;  // 32: too long for registers
 }
 
-// Workgroups of the backward: enough to fill the CUs with their registers' worth of waves, few enough that the partial
-// rows (2 dim floats each) stay small beside the rows themselves.
-constexpr uint32_t kGradBlocks = 512;
-uint32_t grad_blocks(uint64_t rows, uint32_t dim) {
+// Workgroups of the backward: one a CU.  Each ends in a partial row of 2 dim floats, written and read again; a second
+// workgroup a CU hides nothing that the row ahead does not, and doubles them (8192 x 4096 bf16: 50 us against 45, 4096 x
+// 8192: 56 against 48, 65536 x 1024: 81 against 75).  Rows that end inside a piece have branches between their loads, and
+// are held by one wave up to 1024 columns: there two hide more (16384 x 777 bf16: 24 us against 26).
+uint32_t grad_blocks(uint64_t rows, uint32_t dim, bool end) {
   const int wpr = waves_per_row(dim);
   const uint64_t want = wpr > 16 ? ceil_div(rows, kAnyWaves) : wpr == 16 ? rows : ceil_div(rows, 8 / wpr);
-  return static_cast<uint32_t>(want < kGradBlocks ? want : kGradBlocks);
+  const uint64_t most = end && wpr == 1 ? 512 : 256;
+  return static_cast<uint32_t>(want < most ? want : most);
 }
 
 // fn(WPR, whether rows end inside a piece) as integral constants
@@ -481,7 +519,7 @@ int omr_layer_norm(const void* x, int dtype, uint64_t rows, uint32_t dim, uint64
 }
 
 size_t omr_layer_norm_grad_workspace_bytes(uint64_t rows, uint32_t dim) {
-  return static_cast<size_t>(grad_blocks(rows, dim)) * 2 * dim * sizeof(float) + 16;
+  return static_cast<size_t>(grad_blocks(rows, dim, true)) * 2 * dim * sizeof(float) + 16;
 }
 
 int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* x, int dtype, uint64_t rows,
@@ -518,7 +556,8 @@ int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* 
   a.dim = dim;
   a.inv_dim = 1.0f / static_cast<float>(dim);
   const int wpr = waves_per_row(dim);
-  const uint32_t blocks = grad_blocks(rows, dim);
+  const bool end = dim % (16 / elem_bytes(dtype)) != 0;
+  const uint32_t blocks = grad_blocks(rows, dim, end);
   const int rc = with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto p) {
@@ -532,9 +571,9 @@ int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* 
         k_norm_dx_any<T, P><<<static_cast<unsigned>(rows < 2048 ? rows : 2048), 64 * kAnyWaves, 0, S(stream)>>>(a);
         return elaunch("omr_layer_norm_grad");
       }
-      return with_shape(dim % (16 / sizeof(T)) != 0, wpr, [&](auto waves, auto end) {
+      return with_shape(end, wpr, [&](auto waves, auto ends) {
         constexpr int WPR = decltype(waves)::value;
-        k_norm_grad<T, P, WPR, decltype(end)::value><<<blocks, WPR == 16 ? 1024 : 512, 0, S(stream)>>>(a);
+        k_norm_grad<T, P, WPR, decltype(ends)::value><<<blocks, WPR == 16 ? 1024 : 512, 0, S(stream)>>>(a);
         return elaunch("omr_layer_norm_grad");
       });
     };
