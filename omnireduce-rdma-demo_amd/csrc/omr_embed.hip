@@ -77,12 +77,13 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
 //     loads in flight at once.  A row within its chunk is done; of one that goes on (a frequent
 //     word) the chunk's piece goes to `partial`, and k_embed_join adds its pieces up in order, a launch later;
 //   - fill workgroups store the zeros of the rows that no token names.
-// 8192 tokens of 65536 x 1024 take 55 us with the sort and the join, 290 MB at 5.3 TB/s; the zeros alone, with the sort,
-// 41.  (Chunks of 32 in two flights of 16: 63.  Lane groups that summed or zeroed four rows each: 92, every row with
-// tokens two dependent loads behind the stores around it.  The chunks in a launch of their own in front of the zeros,
-// at 32: 64, and 94 against 88 at 32768 tokens.)
+// 8192 tokens of 65536 x 1024 take 63 us with the sort and the join where two tables take turns (torch's fill of one takes
+// 40: it is the last-level cache that the table does not fit beside the other), 55 where one is written again and again.
+// Non-temporal stores of the zeros: 52 us, but 109 instead of 98 together with the all-reduce's scan, which reads the
+// table next and finds part of it in that cache.  (Chunks of 32 in two flights of 16: 8 us more.  Lane groups that summed
+// or zeroed four rows each: 92, every row with tokens two dependent loads behind the stores around it.  The zeros, or the
+// chunks, in a launch of their own, beside or behind the sort: 64 to 66.)
 constexpr uint32_t kChunk = 16;
-constexpr int kFillRows = 4;
 
 struct SumArgs {
   const void* grad_out;
@@ -97,7 +98,7 @@ struct SumArgs {
   uint32_t rows, dim, chunks, tiles;  // tiles of columns of a chunk workgroup
   float scale;
   int accumulate;
-  int wide;  // every row of the table is whole aligned pieces
+  uint32_t fill;  // rows of a fill workgroup's wave
 };
 
 constexpr int VEC = 4;  // columns a lane: 16 bytes of the table
@@ -115,7 +116,7 @@ __device__ __forceinline__ void put(const SumArgs& a, uint32_t row, uint32_t c, 
   store_some<float, VEC>(o, a.dim - c, v);
 }
 
-// blocks [0, chunk_blocks): chunks, 256 VEC columns each; behind them: zeros, four rows a wave
+// blocks [0, chunk_blocks): chunks, 256 VEC columns each; behind them: zeros, `fill` rows a wave
 template <class T>
 __global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blocks) {
   const uint32_t lane = threadIdx.x & 63;
@@ -162,24 +163,12 @@ __global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blo
     }
     return;
   }
-  const uint64_t first = (static_cast<uint64_t>(blockIdx.x - chunk_blocks) * 4 + (threadIdx.x >> 6)) * kFillRows;
-  uint32_t at[kFillRows + 1];
-#pragma unroll
-  for (int q = 0; q <= kFillRows; ++q) at[q] = a.start[min(first + q, static_cast<uint64_t>(a.rows))];
-#pragma unroll
-  for (int q = 0; q < kFillRows; ++q) {
-    if (first + q >= a.rows || at[q] != at[q + 1]) continue;
-    float* o = a.out + (first + q) * a.ostride;
-    if (a.wide) {
-      // written through (sc0 sc1): no dirty lines are left in the L2s to be flushed behind the last wave (2 us)
-      typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-      const auto to = __builtin_amdgcn_make_buffer_rsrc(o, 0, static_cast<int>(a.dim * 4), 0x00020000);
-      for (uint32_t c = lane * VEC; c < a.dim; c += 64 * VEC)
-        __builtin_amdgcn_raw_buffer_store_b128(v4u{}, to, c * 4, 0, 17);
-    } else {
-      const float zero[VEC] = {};
-      for (uint32_t c = lane * VEC; c < a.dim; c += 64 * VEC) store_some<float, VEC>(o + c, a.dim - c, zero);
-    }
+  const uint64_t first = (static_cast<uint64_t>(blockIdx.x - chunk_blocks) * 4 + (threadIdx.x >> 6)) * a.fill;
+  for (uint64_t row = first; row < min(first + a.fill, static_cast<uint64_t>(a.rows)); ++row) {
+    if (a.start[row] != a.start[row + 1]) continue;
+    float* o = a.out + row * a.ostride;
+    const float zero[VEC] = {};
+    for (uint32_t c = lane * VEC; c < a.dim; c += 64 * VEC) store_some<float, VEC>(o + c, a.dim - c, zero);
   }
 }
 
@@ -308,10 +297,10 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
   a.chunks = num_ids != 0 ? static_cast<uint32_t>(ceil_div(num_ids, kChunk)) : 0;
   a.scale = scale;
   a.accumulate = accumulate != 0;
-  a.wide = dim % VEC == 0 && table_stride % VEC == 0 && aligned(grad_table, 16);
+  a.fill = static_cast<uint32_t>(ceil_div(num_rows, 1u << 25));  // one, but for a table of more than 2^25 rows
   a.tiles = static_cast<uint32_t>(ceil_div(dim, 256 * VEC));
   const uint64_t chunk_blocks = static_cast<uint64_t>(a.chunks) * a.tiles, join_tiles = ceil_div(dim, 64 * VEC),
-                 blocks = chunk_blocks + (accumulate ? 0 : ceil_div(num_rows, 4 * kFillRows));
+                 blocks = chunk_blocks + (accumulate ? 0 : ceil_div(num_rows, 4 * a.fill));
   if (blocks > kMaxBlocks || a.chunks * join_tiles > kMaxBlocks)
     return efail("embed_grad: too many tokens or rows for one call");
   const uint32_t range = sort_range(a.rows);
