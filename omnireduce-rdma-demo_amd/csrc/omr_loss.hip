@@ -271,18 +271,17 @@ __device__ __forceinline__ void stream8(T* p, uint32_t n, const vec_t<T, 8>& v) 
   }
 }
 
+// tile number `id` of a product, by the whole workgroup; lds: R (BM + BN) 64 elements
 template <class T, int EPI, int BM, int BN, int WM, int WN, int R>
-__global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
+__device__ __forceinline__ void gemm_tile(const GemmArgs<T>& a, uint32_t id, T* lds) {
   constexpr int NT = 64 * WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
   constexpr bool AC = EPI == kHidden || EPI == kWeight, BC = EPI == kWeight;
-  __shared__ __attribute__((aligned(1024))) T lds[R * (BM + BN) * kBK];
   static_assert((R & (R - 1)) == 0, "step t's buffers are those at t mod R");
   auto la = [&](uint32_t t) { return lds + (t & (R - 1)) * (BM * kBK); };
   auto lb = [&](uint32_t t) { return lds + R * BM * kBK + (t & (R - 1)) * (BN * kBK); };
   static_assert(BM * BN <= R * (BM + BN) * kBK, "the results pass through LDS as 16-bit elements");
   // Workgroup ids go round the 8 XCDs: give each XCD a contiguous stretch of tiles, and walk the stretch in groups of 8
   // tile rows, so the tiles that run together on an XCD share operands in its L2.
-  uint32_t id = blockIdx.x;
   const uint32_t all = a.mt * a.nt * a.splits, per = all / 8, rem = all % 8, xcd = id % 8;
   id = xcd * per + min(xcd, rem) + id / 8;
   const uint32_t split = id / (a.mt * a.nt);
@@ -612,6 +611,22 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
   }
 }
 
+template <class T, int EPI, int BM, int BN, int WM, int WN, int R>
+__global__ __launch_bounds__(64 * WM * WN) void k_gemm(GemmArgs<T> a) {
+  __shared__ __attribute__((aligned(1024))) T lds[R * (BM + BN) * kBK];
+  gemm_tile<T, EPI, BM, BN, WM, WN, R>(a, blockIdx.x, lds);
+}
+
+// Both products of a piece's G side by side: blocks [0, xtiles) are grad_hidden's.
+template <class T, int BM, int BN, int WM, int WN, int R>
+__global__ __launch_bounds__(64 * WM * WN) void k_both(GemmArgs<T> x, GemmArgs<T> y, uint32_t xtiles) {
+  __shared__ __attribute__((aligned(1024))) T lds[R * (BM + BN) * kBK];
+  if (blockIdx.x < xtiles)
+    gemm_tile<T, kHidden, BM, BN, WM, WN, R>(x, blockIdx.x, lds);
+  else
+    gemm_tile<T, kWeight, BM, BN, WM, WN, R>(y, blockIdx.x - xtiles, lds);
+}
+
 // ---------------------------------------------------------------- few tokens
 //
 // The forward of up to 32 tokens is bound by reading the weight.  The tiles above keep one step of it in flight a CU
@@ -887,6 +902,25 @@ int launch(GemmArgs<T>& a, uint32_t m, uint32_t n, int tile, hipStream_t stream)
   return elaunch("omr_vocab_loss");
 }
 
+// x (grad_hidden) and y (grad_weight) in one launch, by the rule above for their tiles together
+template <class T>
+int launch_both(GemmArgs<T>& x, GemmArgs<T>& y, uint32_t dim, uint32_t cols, hipStream_t stream) {
+  auto tiles = [&](GemmArgs<T>& a, uint32_t n, uint32_t t) {
+    a.mt = static_cast<uint32_t>(ceil_div(dim, t));
+    a.nt = static_cast<uint32_t>(ceil_div(n, t));
+    return a.mt * a.nt * a.splits;
+  };
+  const uint32_t small = tiles(x, x.tokens, kSmall) + tiles(y, cols, kSmall), t = small > 128 ? kSmall : kTiny;
+  const uint32_t xtiles = tiles(x, x.tokens, t), g = xtiles + tiles(y, cols, t);
+  if (small > 256)
+    k_both<T, 128, 128, 2, 2, 2><<<g, 256, 0, stream>>>(x, y, xtiles);
+  else if (small > 128)
+    k_both<T, 128, 128, 2, 2, 4><<<g, 256, 0, stream>>>(x, y, xtiles);
+  else
+    k_both<T, 64, 64, 2, 2, 4><<<g, 256, 0, stream>>>(x, y, xtiles);
+  return elaunch("omr_vocab_loss_grad");
+}
+
 // The piece of the vocabulary whose G is held at a time: about 256 MiB of it (what the last-level cache holds), at least
 // 1024 rows, in equal pieces of whole tiles.
 constexpr uint64_t kPieceBytes = 256ull << 20;
@@ -1151,38 +1185,39 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
       z.ksplit = dim;
       z.splits = 1;
       if (const int rc = launch<T, kGrad>(z, cols, z.tokens, tile_of(cols, tokens, 1), S(stream))) return rc;
-      if (grad_hidden != nullptr) {
-        GemmArgs<T> x = a;
-        x.a = {w.p + v0 * w.ld, w.ld, pdim};
-        x.b = {g, piece, x.tokens};
-        x.k = rows;
-        x.ksplit = ksplit;
-        x.splits = static_cast<uint32_t>(ceil_div(rows, ksplit));
-        x.first = v0 == 0;
-        const bool done = v0 + piece >= vocab;
-        x.last = done && splits == 1;
-        x.out = grad_hidden;
-        x.ostride = grad_hidden_stride;
-        if (const int rc = launch<T, kHidden>(x, dim, x.tokens, tile_of(dim, tokens, x.splits), S(stream))) return rc;
-        if (done && splits > 1) {
-          x.splits = splits;
-          const uint64_t blocks = ceil_div(tokens * dim, 256);
-          k_join<T><<<static_cast<unsigned>(blocks), 256, 0, S(stream)>>>(x);
-          if (const int rc = elaunch("omr_vocab_loss_grad (join)")) return rc;
-        }
+      GemmArgs<T> x = a, y = a;
+      x.a = {w.p + v0 * w.ld, w.ld, pdim};
+      x.b = {g, piece, x.tokens};
+      x.k = rows;
+      x.ksplit = ksplit;
+      x.splits = static_cast<uint32_t>(ceil_div(rows, ksplit));
+      x.first = v0 == 0;
+      const bool done = v0 + piece >= vocab;
+      x.last = done && splits == 1;
+      x.out = grad_hidden;
+      x.ostride = grad_hidden_stride;
+      y.a = {clean, pdim, pdim};
+      y.b = {g, piece, cols};
+      y.k = y.tokens;
+      y.ksplit = y.tokens;
+      y.splits = 1;
+      y.out = grad_weight;
+      y.ostride = grad_weight_stride;
+      y.out_f32 = grad_weight_dtype == OMR_F32;
+      y.accumulate = accumulate != 0;
+      const int xt = tile_of(dim, x.tokens, x.splits), yt = tile_of(dim, cols, 1);
+      if (grad_hidden != nullptr && grad_weight != nullptr && xt != kTileBig && yt != kTileBig) {
+        if (const int rc = launch_both<T>(x, y, dim, cols, S(stream))) return rc;
+      } else {
+        if (grad_hidden != nullptr)
+          if (const int rc = launch<T, kHidden>(x, dim, x.tokens, xt, S(stream))) return rc;
+        if (grad_weight != nullptr)
+          if (const int rc = launch<T, kWeight>(y, dim, cols, yt, S(stream))) return rc;
       }
-      if (grad_weight != nullptr) {
-        GemmArgs<T> y = a;
-        y.a = {clean, pdim, pdim};
-        y.b = {g, piece, cols};
-        y.k = y.tokens;
-        y.ksplit = y.tokens;
-        y.splits = 1;
-        y.out = grad_weight;
-        y.ostride = grad_weight_stride;
-        y.out_f32 = grad_weight_dtype == OMR_F32;
-        y.accumulate = accumulate != 0;
-        if (const int rc = launch<T, kWeight>(y, dim, cols, tile_of(dim, cols, 1), S(stream))) return rc;
+      if (grad_hidden != nullptr && done && splits > 1) {
+        x.splits = splits;
+        k_join<T><<<static_cast<unsigned>(ceil_div(tokens * dim, 256)), 256, 0, S(stream)>>>(x);
+        if (const int rc = elaunch("omr_vocab_loss_grad (join)")) return rc;
       }
     }
     return 0;
