@@ -627,6 +627,98 @@ __global__ __launch_bounds__(64 * WM * WN) void k_both(GemmArgs<T> x, GemmArgs<T
     gemm_tile<T, kWeight, BM, BN, WM, WN, R>(y, blockIdx.x - xtiles, lds);
 }
 
+// ---------------------------------------------------------------- what the products need
+
+// The largest |grad_loss| of the tokens with a target, in every thread of a workgroup of WAVES waves.  (A NaN counts as the
+// largest: the gradient shall have it.)
+template <class T, int WAVES>
+__device__ __forceinline__ float largest(const GemmArgs<T>& a, float* lds) {
+  float m = 0.0f;
+  auto more = [&](float g) { m = m != m || g <= m ? m : g; };
+  for (uint64_t n0 = threadIdx.x; n0 < a.tokens; n0 += 4 * 64 * WAVES) {  // four tokens in flight
+    float g[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t n = n0 + i * 64 * WAVES;
+      g[i] = n < a.tokens ? fabsf(factor_of(a, static_cast<uint32_t>(n))) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) more(g[i]);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) more(__shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = lds[0];
+  for (int w = 1; w < WAVES; ++w) more(lds[w]);
+  return m;
+}
+
+// What grad_weight's product needs besides G, by workgroups of WAVES waves: blocks [0, sorters) sort the tokens by target;
+// the others copy the hidden states into whole 16-byte pieces, zeros behind dim, each row times its share of the largest
+// grad_loss, and zeros for tokens without a target, whatever they hold.  Up to kFindHere tokens each of these finds the
+// largest itself: a launch less, 3 to 4 us of a backward pass up to 2048 tokens, nothing at 6000 to 8192, and 12 us lost
+// at 16384, where every block would read that many.
+constexpr uint32_t kFindHere = 4096;
+
+template <class T>
+struct PrepareArgs {
+  uint32_t blocks, sorters, range;
+  uint32_t *start, *perm;
+  const T* src;  // hidden
+  uint64_t stride;
+  uint32_t pdim, lpr_log;  // 2^lpr_log lanes a row
+  float* amax;
+  T* dst;
+};
+
+template <class T, class I, int WAVES>
+__device__ __forceinline__ void prepare(const GemmArgs<T>& a, const PrepareArgs<T>& p, uint32_t block,
+                                        SortSpace<WAVES>& space) {
+  if (block < p.sorters) {
+    sort_by_row<I, WAVES>(space, block, static_cast<const I*>(a.targets), a.tokens, a.vocab, p.range, p.start, p.perm,
+                          nullptr);
+    return;
+  }
+  block -= p.sorters;
+  float most;
+  if (a.tokens <= kFindHere) {
+    most = largest<T, WAVES>(a, reinterpret_cast<float*>(space.wsum));
+    if (block == 0 && threadIdx.x == 0) *p.amax = most;
+  } else {
+    most = *p.amax;
+  }
+  const uint64_t row = (static_cast<uint64_t>(block) * 64 * WAVES + threadIdx.x) >> p.lpr_log;
+  if (row >= a.tokens) return;
+  const float g = factor_of(a, static_cast<uint32_t>(row)), by = g == 0.0f ? 0.0f : g / most;
+  for (uint32_t c = (threadIdx.x & ((1u << p.lpr_log) - 1)) * 8; c < p.pdim; c += 8u << p.lpr_log) {
+    float v[8] = {};
+    if (by != 0.0f) {
+      load_some<T, 8>(p.src + row * p.stride + c, a.dim - c, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= by;
+    }
+    store_f32<T, 8>(p.dst + row * p.pdim + c, v);
+  }
+}
+
+template <class T, class I>
+__global__ __launch_bounds__(1024) void k_prepare(GemmArgs<T> a, PrepareArgs<T> p) {
+  __shared__ SortSpace<16> space;
+  prepare<T, I, 16>(a, p, blockIdx.x, space);
+}
+
+// The same beside the first piece's G, where that has few tiles: blocks [0, p.blocks) prepare.
+template <class T, class I, int BM, int BN, int WM, int WN, int R>
+__global__ __launch_bounds__(64 * WM * WN) void k_grad_prepare(GemmArgs<T> a, PrepareArgs<T> p) {
+  __shared__ __attribute__((aligned(1024))) T lds[R * (BM + BN) * kBK];
+  static_assert(sizeof(SortSpace<WM * WN>) <= sizeof(lds), "they share LDS");
+  if (blockIdx.x < p.blocks)
+    prepare<T, I, WM * WN>(a, p, blockIdx.x, *reinterpret_cast<SortSpace<WM * WN>*>(lds));
+  else
+    gemm_tile<T, kGrad, BM, BN, WM, WN, R>(a, blockIdx.x - p.blocks, lds);
+}
+
 // ---------------------------------------------------------------- few tokens
 //
 // The forward of up to 32 tokens is bound by reading the weight.  The tiles above keep one step of it in flight a CU
@@ -761,35 +853,10 @@ __global__ __launch_bounds__(256) void k_merge(GemmArgs<T> a, float* loss, float
   loss[tok] = target_of(a, tok) >= 0 ? l - a.ztarget[tok] : 0.0f;
 }
 
-// The largest |grad_loss| of the tokens with a target, in every thread of a workgroup of 1024.  (A NaN counts as the
-// largest: the gradient shall have it.)
-template <class T>
-__device__ __forceinline__ float largest(const GemmArgs<T>& a, float* lds) {
-  float m = 0.0f;
-  auto more = [&](float g) { m = m != m || g <= m ? m : g; };
-  for (uint64_t n0 = threadIdx.x; n0 < a.tokens; n0 += 4 * 1024) {  // four tokens in flight
-    float g[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint64_t n = n0 + i * 1024;
-      g[i] = n < a.tokens ? fabsf(factor_of(a, static_cast<uint32_t>(n))) : 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) more(g[i]);
-  }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) more(__shfl_xor(m, d));
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
-  __syncthreads();
-  m = lds[0];
-  for (int w = 1; w < 16; ++w) more(lds[w]);
-  return m;
-}
-
 template <class T>
 __global__ __launch_bounds__(1024) void k_largest(GemmArgs<T> a, float* amax) {
   __shared__ float lds[16];
-  const float m = largest(a, lds);
+  const float m = largest<T, 16>(a, lds);
   if (threadIdx.x == 0) *amax = m;
 }
 
@@ -802,46 +869,6 @@ __global__ __launch_bounds__(256) void k_pack(const T* src, uint64_t stride, uin
   for (uint32_t c = (threadIdx.x & ((1u << lpr_log) - 1)) * 8; c < pdim; c += 8u << lpr_log) {
     float v[8];
     load_some<T, 8>(src + row * stride + c, dim - c, v);
-    store_f32<T, 8>(dst + row * pdim + c, v);
-  }
-}
-
-// What grad_weight's product needs, in one launch: blocks [0, sorters) sort the tokens by target; the others copy the
-// hidden states into whole pieces as k_pack does, each row times its share of the largest grad_loss, and zeros for tokens
-// without a target, whatever they hold.  Up to kFindHere tokens each of these finds the largest itself: a launch less,
-// 3 to 4 us of a backward pass up to 2048 tokens, nothing at 6000 to 8192, and 12 us lost at 16384, where every block
-// would read that many.
-constexpr uint32_t kFindHere = 4096;
-
-template <class T, class I>
-__global__ __launch_bounds__(64 * kSortWaves) void k_prepare(GemmArgs<T> a, uint32_t sorters, uint32_t range,
-                                                             uint32_t* start, uint32_t* perm, const T* src,
-                                                             uint64_t stride, uint32_t pdim, uint32_t lpr_log,
-                                                             float* amax, T* dst) {
-  static_assert(kSortWaves == 16, "largest() takes 1024 threads");
-  __shared__ SortSpace space;
-  if (blockIdx.x < sorters) {
-    sort_by_row<I>(space, blockIdx.x, static_cast<const I*>(a.targets), a.tokens, a.vocab, range, start, perm, nullptr);
-    return;
-  }
-  const uint32_t block = blockIdx.x - sorters;
-  float most;
-  if (a.tokens <= kFindHere) {
-    most = largest(a, reinterpret_cast<float*>(space.wsum));
-    if (block == 0 && threadIdx.x == 0) *amax = most;
-  } else {
-    most = *amax;
-  }
-  const uint64_t row = (static_cast<uint64_t>(block) * 1024 + threadIdx.x) >> lpr_log;
-  if (row >= a.tokens) return;
-  const float g = factor_of(a, static_cast<uint32_t>(row)), by = g == 0.0f ? 0.0f : g / most;
-  for (uint32_t c = (threadIdx.x & ((1u << lpr_log) - 1)) * 8; c < pdim; c += 8u << lpr_log) {
-    float v[8] = {};
-    if (by != 0.0f) {
-      load_some<T, 8>(src + row * stride + c, a.dim - c, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= by;
-    }
     store_f32<T, 8>(dst + row * pdim + c, v);
   }
 }
@@ -900,6 +927,22 @@ int launch(GemmArgs<T>& a, uint32_t m, uint32_t n, int tile, hipStream_t stream)
     default: k_gemm<T, EPI, 64, 64, 2, 2, 4><<<g, 256, 0, stream>>>(a); break;
   }
   return elaunch("omr_vocab_loss");
+}
+
+// G's product (of fewer than kTileBig's tiles) and, in front of it, what grad_weight's needs
+template <class T, class I>
+int launch_grad_prepare(GemmArgs<T>& a, const PrepareArgs<T>& p, uint32_t cols, int tile, hipStream_t stream) {
+  const uint32_t t = tile_rows(tile);
+  a.mt = static_cast<uint32_t>(ceil_div(cols, t));
+  a.nt = static_cast<uint32_t>(ceil_div(a.tokens, t));
+  const uint32_t g = p.blocks + a.mt * a.nt;
+  if (tile == kTileSmall)
+    k_grad_prepare<T, I, 128, 128, 2, 2, 2><<<g, 256, 0, stream>>>(a, p);
+  else if (tile == kTileSmallDeep)
+    k_grad_prepare<T, I, 128, 128, 2, 2, 4><<<g, 256, 0, stream>>>(a, p);
+  else
+    k_grad_prepare<T, I, 64, 64, 2, 2, 4><<<g, 256, 0, stream>>>(a, p);
+  return elaunch("omr_vocab_loss_grad");
 }
 
 // x (grad_hidden) and y (grad_weight) in one launch, by the rule above for their tiles together
@@ -1146,23 +1189,38 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     a.up = grad_loss;
     a.upstride = grad_loss_stride;
     a.amax = amax;
-    if (grad_weight != nullptr) {
-      if (tokens > kFindHere) {
-        k_largest<T><<<1, 1024, 0, S(stream)>>>(a, amax);
-        if (const int rc = elaunch("omr_vocab_loss_grad (largest)")) return rc;
-      }
-      const uint32_t range = sort_range(a.vocab), lpr_log = lanes_log(pdim);
-      const uint64_t sorters = ceil_div(vocab, range), blocks = sorters + ceil_div(tokens, 1024u >> lpr_log);
-      if (blocks >= (1u << 22)) return efail("vocab_loss_grad: too many tokens or rows for one call");
-      auto prepare = [&](auto i) {
-        k_prepare<T, decltype(i)><<<static_cast<unsigned>(blocks), 64 * kSortWaves, 0, S(stream)>>>(
-            a, static_cast<uint32_t>(sorters), range, start, perm, static_cast<const T*>(hidden), hidden_stride, pdim,
-            lpr_log, amax, clean);
-        return elaunch("omr_vocab_loss_grad (prepare)");
-      };
-      if (const int rc = targets64 ? prepare(int64_t{}) : prepare(int32_t{})) return rc;
-    }
     const uint32_t piece = piece_rows(tokens, vocab);
+    const uint32_t first_cols = static_cast<uint32_t>(up(std::min<uint64_t>(piece, vocab), 256));
+    // (a piece's columns of G that are written: zeros behind the vocabulary)
+    const bool beside = tokens <= kFindHere && tile_of(first_cols, tokens, 1) != kTileBig;
+    PrepareArgs<T> p{};
+    if (grad_weight != nullptr) {
+      const uint32_t threads = beside ? 256 : 1024;
+      p.lpr_log = lanes_log(pdim);
+      p.range = beside ? sort_range<4>(a.vocab) : sort_range<16>(a.vocab);
+      p.sorters = static_cast<uint32_t>(ceil_div(vocab, p.range));
+      const uint64_t blocks = p.sorters + ceil_div(tokens, threads >> p.lpr_log);
+      if (blocks >= (1u << 22)) return efail("vocab_loss_grad: too many tokens or rows for one call");
+      p.blocks = static_cast<uint32_t>(blocks);
+      p.start = start;
+      p.perm = perm;
+      p.src = static_cast<const T*>(hidden);
+      p.stride = hidden_stride;
+      p.pdim = pdim;
+      p.amax = amax;
+      p.dst = clean;
+      if (!beside) {
+        if (tokens > kFindHere) {
+          k_largest<T><<<1, 1024, 0, S(stream)>>>(a, amax);
+          if (const int rc = elaunch("omr_vocab_loss_grad (largest)")) return rc;
+        }
+        if (targets64)
+          k_prepare<T, int64_t><<<p.blocks, 1024, 0, S(stream)>>>(a, p);
+        else
+          k_prepare<T, int32_t><<<p.blocks, 1024, 0, S(stream)>>>(a, p);
+        if (const int rc = elaunch("omr_vocab_loss_grad (prepare)")) return rc;
+      }
+    }
     a.lse = lse;
     a.g = g;
     a.ldg = piece;
@@ -1176,7 +1234,7 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     const uint32_t splits = static_cast<uint32_t>(ceil_div(whole, ksplit));  // of a whole piece; the last may have fewer
     for (uint64_t v0 = 0; v0 < vocab; v0 += piece) {
       const uint32_t rows = static_cast<uint32_t>(std::min<uint64_t>(piece, vocab - v0));
-      const uint32_t cols = static_cast<uint32_t>(up(rows, 256));  // columns of G that are written (zeros behind rows)
+      const uint32_t cols = static_cast<uint32_t>(up(rows, 256));
       a.v0 = static_cast<uint32_t>(v0);
       GemmArgs<T> z = a;
       z.a = {w.p + v0 * w.ld, w.ld, rows};
@@ -1184,7 +1242,14 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
       z.k = dim;
       z.ksplit = dim;
       z.splits = 1;
-      if (const int rc = launch<T, kGrad>(z, cols, z.tokens, tile_of(cols, tokens, 1), S(stream))) return rc;
+      const int zt = tile_of(cols, tokens, 1);
+      if (grad_weight != nullptr && beside && v0 == 0) {
+        if (const int rc = targets64 ? launch_grad_prepare<T, int64_t>(z, p, cols, zt, S(stream))
+                                     : launch_grad_prepare<T, int32_t>(z, p, cols, zt, S(stream)))
+          return rc;
+      } else if (const int rc = launch<T, kGrad>(z, cols, z.tokens, zt, S(stream))) {
+        return rc;
+      }
       GemmArgs<T> x = a, y = a;
       x.a = {w.p + v0 * w.ld, w.ld, pdim};
       x.b = {g, piece, x.tokens};

@@ -14,7 +14,7 @@ __device__ __forceinline__ bool id_ok(I id, uint32_t rows) {
 // Groups the tokens by row in ONE launch without any exchange between workgroups: workgroup p owns the rows
 // [p R, p R + R) and reads ALL ids itself (they sit in the L2s: 64 KiB for 8192 int64 ids), counting its own and how
 // many are below its range, which is where its piece of the sorted list begins.
-//   pass 1  wave w counts the ids of its contiguous sixteenth of the tokens in hist[w][id - lo], and notes the tokens it
+//   pass 1  wave w counts the ids of its contiguous part of the tokens in hist[w][id - lo], and notes the tokens it
 //           counted, in order, in a list of its own
 //   scan    start[v] = ids below v; hist[w][.] = where wave w's first token of that row goes
 //   pass 2  the waves walk their lists (or, where a list is full, their tokens again) and place them: within 64 tokens
@@ -22,29 +22,33 @@ __device__ __forceinline__ bool id_ok(I id, uint32_t rows) {
 //           order within a row is token order; named[i], where it is wanted, is the row of the i-th of the sorted list
 // Every workgroup reads T ids: hidden in the L2 up to some 100 k tokens, where a radix sort would take three launches
 // for each of three digits.
-constexpr int kSortWaves = 16;
-constexpr int kSortRange = 1024;  // rows per workgroup at most: 64 KiB of histogram
-constexpr int kSortBits = 10;
 constexpr uint32_t kNoRow = ~0u;
-constexpr uint32_t kSortList = 512;  // tokens a wave notes: 32 KiB
+constexpr uint32_t kSortList = 512;  // tokens a wave notes
 
+// of a workgroup of WAVES waves: 96 KiB for 16, 12 KiB for 4
+template <int WAVES>
 struct SortSpace {
-  uint32_t hist[kSortWaves * kSortRange];
-  uint32_t list[kSortWaves][kSortList];  // (token - the wave's first) << 10 | local id
-  uint32_t wsum[kSortWaves], below_w[kSortWaves], valid;
+  static constexpr uint32_t kRange = 64 * WAVES;  // rows at most: one a thread
+  static constexpr int kBits = WAVES == 16 ? 10 : 8;
+  static_assert(kRange == 1u << kBits, "a local id's bits");
+  uint32_t hist[WAVES * kRange];
+  uint32_t list[WAVES][kSortList];  // (token - the wave's first) << kBits | local id
+  uint32_t wsum[WAVES], below_w[WAVES], valid;
 };
 
 // rows per workgroup: one workgroup a CU where the table is small enough for that
+template <int WAVES>
 inline uint32_t sort_range(uint32_t rows) {
   const uint32_t each = (rows + 255) / 256;
-  return each < 16 ? 16 : each > kSortRange ? kSortRange : each;
+  return each < 16 ? 16 : each > SortSpace<WAVES>::kRange ? SortSpace<WAVES>::kRange : each;
 }
 
-// Workgroup `block` of 64 kSortWaves threads: the positions of the ids that name one of its rows, by row and in order
+// Workgroup `block` of WAVES waves: the positions of the ids that name one of its rows, by row and in order
 // within it: those of row v at perm[start[v] .. start[v + 1]).  start: rows + 1, perm and named (or null): one an id.
-template <class I>
-__device__ __forceinline__ void sort_by_row(SortSpace& space, uint32_t block, const I* ids, uint32_t tokens, uint32_t rows,
+template <class I, int WAVES>
+__device__ __forceinline__ void sort_by_row(SortSpace<WAVES>& space, uint32_t block, const I* ids, uint32_t tokens, uint32_t rows,
                                             uint32_t range, uint32_t* start, uint32_t* perm, uint32_t* named) {
+  constexpr int kSortWaves = WAVES, kSortBits = SortSpace<WAVES>::kBits;
   auto& hist = space.hist;
   auto& list = space.list;
   auto &wsum = space.wsum, &below_w = space.below_w;
@@ -115,7 +119,7 @@ __device__ __forceinline__ void sort_by_row(SortSpace& space, uint32_t block, co
     }
   }
   __syncthreads();
-  // (a list holds token distances of 22 bits)
+  // (a list holds token distances of 32 - kBits bits)
   const bool listed = noted <= kSortList && span <= 1u << (32 - kSortBits);
   const uint32_t steps = listed ? noted : t1 - t0;
   for (uint32_t i = 0; i < steps; i += 64) {
@@ -123,7 +127,7 @@ __device__ __forceinline__ void sort_by_row(SortSpace& space, uint32_t block, co
     if (i + lane < steps) {
       if (listed) {
         const uint32_t e = list[wave][i + lane];
-        v = e & (kSortRange - 1);
+        v = e & (SortSpace<WAVES>::kRange - 1);
         t = t0 + (e >> kSortBits);
       } else if (id_ok(ids[t], rows)) {
         v = static_cast<uint32_t>(ids[t]) - lo;
