@@ -21,7 +21,8 @@ __device__ __forceinline__ bool id_ok(I id, uint32_t rows) {
 //           the lanes of equal ids rank themselves by lane (match by ballots over the bits of the local id), so the
 //           order within a row is token order; named[i], where it is wanted, is the row of the i-th of the sorted list
 // Every workgroup reads T ids: hidden in the L2 up to some 100 k tokens, where a radix sort would take three launches
-// for each of three digits.
+// for each of three digits.  8192 ids of 65536 rows: 6.9 us; 20011 of 1009: 10.5, whether 8 or 20 loads are in flight and
+// 16 or 4 rows are a workgroup's.
 constexpr uint32_t kNoRow = ~0u;
 constexpr uint32_t kSortList = 512;  // tokens a wave notes
 
