@@ -79,12 +79,16 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_embed_sort(const I* ids, ui
 //     loads in flight at once.  A row within its chunk is done; of one that goes on (a frequent
 //     word) the chunk's piece goes to `partial`, and k_embed_join adds its pieces up in order, a launch later;
 //   - fill workgroups store the zeros of the rows that no token names.
-// 8192 tokens of 65536 x 1024 take 63 us with the sort and the join where two tables take turns (torch's fill of one takes
-// 40: it is the last-level cache that the table does not fit beside the other), 55 where one is written again and again.
-// Non-temporal stores of the zeros: 52 us, but 109 instead of 98 together with the all-reduce's scan, which reads the
-// table next and finds part of it in that cache.  (Chunks of 32 in two flights of 16: 8 us more.  Lane groups that summed
-// or zeroed four rows each: 92, every row with tokens two dependent loads behind the stores around it.  The zeros, or the
-// chunks, in a launch of their own, beside or behind the sort: 64 to 66.)
+// Of every four rows of zeros one is stored as any store and three non-temporally.  The scan of the all-reduce reads the
+// table next, and finds some of it in the last-level cache (256 MiB); but a table that fills that cache with dirty lines
+// pays for their way out.  8192 tokens of 65536 x 1024 (256 MiB), two tables in turn, with the sort and the join, and
+// then together with the scan: 54 us and 100; all stores ordinary 64 and 98, all non-temporal 53 and 110, every second
+// one 55 and 97.  32768 tokens: 76 and 129, against 93 and 135, 73 and 134, 82 and 129.  131072 x 1024: 111 and 189,
+// against 115 and 194, 100 and 209, 113 and 180.  8192 tokens of 49152 x 1024: 39 and 82, against 48 and 80, 41 and 87,
+// 39 and 81.  (Torch's fill of 256 MiB alone takes 40 us.)
+// Other forms.  Chunks of 32 in two flights of 16: 8 us more at 65536 x 1024.  Lane groups that sum or zero four rows each:
+// 30 more, every row with tokens two dependent loads behind the stores around it.  The zeros, or the chunks, in a launch
+// of their own, beside or behind the sort: 1 to 3 more.
 constexpr uint32_t kChunk = 16;
 
 struct SumArgs {
@@ -170,7 +174,12 @@ __global__ __launch_bounds__(256) void k_embed_sum(SumArgs a, uint32_t chunk_blo
     if (a.start[row] != a.start[row + 1]) continue;
     float* o = a.out + row * a.ostride;
     const float zero[VEC] = {};
-    for (uint32_t c = lane * VEC; c < a.dim; c += 64 * VEC) store_some<float, VEC>(o + c, a.dim - c, zero);
+    for (uint32_t c = lane * VEC; c < a.dim; c += 64 * VEC) {
+      if (row % 4 != 0)
+        stream_some<float, VEC>(o + c, a.dim - c, zero);
+      else
+        store_some<float, VEC>(o + c, a.dim - c, zero);
+    }
   }
 }
 
