@@ -375,7 +375,8 @@ def loss_ref(h, w, t, off):
 
 
 LOSS_SIZES = [(1, 1, 8), (1, 7, 1), (3, 300, 72), (16, 70, 2120), (17, 129, 264), (32, 200, 1000), (33, 200, 64), (64, 1000, 128), (130, 257, 61), (257, 2000, 200),
-              (300, 5003, 520), (1025, 700, 96), (16, 40000, 64), (700, 70000, 64), (2048, 8192, 256), (5, 256, 4096)]
+              (300, 5003, 520), (1025, 700, 96), (16, 40000, 64), (700, 70000, 64), (2048, 8192, 256), (5, 256, 4096),
+              (5000, 300, 40), (600, 4100, 136), (900, 4100, 200), (1500, 5000, 400)]
 
 
 @pytest.mark.parametrize("T,V,D", LOSS_SIZES)
@@ -526,10 +527,10 @@ def test_vocab_loss_strides_and_untouched_memory(gpu, D, pad, offset, dtype):
                 ops.VocabLossPlan(T, V, D, dtype=dtype, grads=False).forward(h, w, t)
 
 
-def test_vocab_loss_pieces(gpu, dtype=BF16):
-    """More logits than one piece holds (tokens x vocabulary x 2 bytes over 256 MiB): three pieces, the last ragged."""
+@pytest.mark.parametrize("T,V,D", [(4100, 70001, 32), (32768, 5000, 136)])
+def test_vocab_loss_pieces(gpu, T, V, D, dtype=BF16):
+    """More logits than one piece holds (tokens x vocabulary x 2 bytes over 256 MiB): pieces, the last ragged."""
     g = gen(12)
-    T, V, D = 4100, 70001, 32
     h, w, t, off = loss_inputs(T, V, D, dtype, g)
     plan = ops.VocabLossPlan(T, V, D)
     loss, lse = plan.forward(h, w, t)
