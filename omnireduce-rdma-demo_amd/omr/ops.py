@@ -295,6 +295,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _MAX_DIM = 1 << 24  # OMR_MAX_DIM
+_F32 = torch.float32
 
 
 def _sizes(count: int, rows: int, dim: int, least: int = 0):
@@ -304,33 +305,36 @@ def _sizes(count: int, rows: int, dim: int, least: int = 0):
 
 
 class _Call:
-    """The device and stream of one call: every tensor must be on that device, which `with` makes the current one.
-    (Short calls are bound by what is done here: a check costs a tenth of a microsecond or two, and is made once.)"""
+    """The device and stream of one call; every tensor must be on that device.  (Short calls are bound by what is done
+    here: a look at a tensor costs 50 to 80 ns, and is made once.)"""
 
-    __slots__ = ("device", "index", "stream", "ptr", "_guard")
+    __slots__ = ("index", "stream", "ptr")
 
     def __init__(self, t: torch.Tensor, stream: Optional[torch.cuda.Stream]):
-        device = t.device
-        if device.type != "cuda":
+        self.index = index = t.get_device()
+        if index < 0:
             raise ValueError("expected a device (HIP) tensor")
-        self.device, self.index, self.stream, self._guard = device, device.index, stream, None
+        self.stream = stream
         if stream is None:
-            self.ptr = _raw_stream(self.index)
-        elif stream.device != device:
-            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+            self.ptr = _raw_stream(index)
+        elif stream.device.index != index:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {self.device}")
         else:
             self.ptr = stream.cuda_stream
 
-    def __enter__(self):
-        if _current_device() != self.index:
-            self._guard = torch.cuda.device(self.device)
-            self._guard.__enter__()
-        return self
+    @property
+    def device(self) -> torch.device:
+        return torch.device("cuda", self.index)
 
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-        return False
+    def launch(self, what: str, fn, *args) -> None:
+        """fn(*args, stream) with the tensors' device as the current one."""
+        if _current_device() == self.index:
+            rc = fn(*args, self.ptr)
+        else:
+            with torch.cuda.device(self.index):
+                rc = fn(*args, self.ptr)
+        if rc != 0:
+            _lib.check(rc, what)
 
     def empty(self, shape, dtype) -> torch.Tensor:
         if self.stream is None:
@@ -348,37 +352,40 @@ class _Call:
         """(pointer, rows, dim, row stride) of a tensor taken as rows of its last dimension."""
         if t.dtype not in _DTYPES if dtype is None else t.dtype is not dtype:
             raise ValueError(f"{name}: element type {t.dtype}" + (f", expected {dtype}" if dtype is not None else ""))
-        ptr = self.on(t, name)
         shape = t.shape
+        strides = t.stride()
         dims = len(shape)
-        if dims == 0 or not 0 < shape[-1] <= _MAX_DIM or (dim is not None and shape[-1] != dim):
+        if dims == 2:
+            n, d = shape
+            stride, one = strides
+        else:
+            d = shape[-1] if dims else 0
+            n, stride, one = t.numel() // max(d, 1), d, strides[-1] if dims else 1
+            if not t.is_contiguous() and dims > 1:
+                raise ValueError(f"{name}: more than two dimensions must be contiguous (stride {strides})")
+        if not 0 < d <= _MAX_DIM or (dim is not None and d != dim):
             raise ValueError(f"{name}: rows of {dim if dim is not None else f'1 to {_MAX_DIM}'} elements expected, got "
                              f"shape {tuple(shape)}")
-        d = shape[-1]
-        n = shape[0] if dims == 2 else t.numel() // d
         if rows is not None and n != rows:
             raise ValueError(f"{name}: {rows} rows expected, got shape {tuple(shape)}")
-        strides = t.stride()
-        if d > 1 and strides[-1] != 1:
+        if one != 1 and d > 1:
             raise ValueError(f"{name}: the elements of a row must be consecutive (stride {strides})")
-        if n <= 1 or dims == 1:
-            return ptr, n, d, d
-        if dims == 2:
-            stride = strides[0]
-        elif t.is_contiguous():
+        if n <= 1:
             stride = d
-        else:
-            raise ValueError(f"{name}: more than two dimensions must be contiguous (stride {strides})")
-        if out and stride < d:
+        elif out and stride < d:
             raise ValueError(f"{name}: an output's rows must not overlap (stride {strides})")
-        return ptr, n, d, stride
+        if t.get_device() != self.index:
+            self.on(t, name)
+        return t.data_ptr(), n, d, stride
 
-    def vector(self, t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype = torch.float32) -> Optional[int]:
+    def vector(self, t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype = _F32) -> Optional[int]:
         if t is None:
             return None
         if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{name}: expected contiguous {dtype}[{n}], got {t.dtype}{tuple(t.shape)}")
-        return self.on(t, name)
+        if t.get_device() != self.index:
+            return self.on(t, name)  # (says so)
+        return t.data_ptr()
 
     def ids(self, t: torch.Tensor, name: str):
         wide = t.dtype is torch.int64
@@ -394,33 +401,34 @@ class _Workspace:
         self.bytes = nbytes
         self.tensor = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
         self.device = self.tensor.device
+        self.ptr = self.tensor.data_ptr()
         self._home = torch.cuda.current_stream(self.device).cuda_stream
 
     def lend(self, call: _Call) -> int:
-        if call.device != self.device:
+        if call.index != self.device.index:
             raise ValueError(f"the plan is on {self.device}, the tensors on {call.device}")
         if call.ptr != self._home:  # used away from the stream it was allocated on: not reused before that work is done
             self.tensor.record_stream(call.stream if call.stream is not None
-                                      else torch.cuda.current_stream(call.device))
-        return self.tensor.data_ptr()
+                                      else torch.cuda.current_stream(call.index))
+        return self.ptr
 
 
 def embed(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None,
           out_dtype: Optional[torch.dtype] = None, stream=None) -> torch.Tensor:
     """Embedding lookup: out[..., :] = scale * table[ids, :], rounded once to out's type (default: the table's).  An id
     outside [0, rows) names no row (padding): a row of zeros."""
-    with _Call(table, stream) as call:
-        if table.dim() != 2:
-            raise ValueError(f"table: expected [rows, dim], got shape {tuple(table.shape)}")
-        tp, rows, dim, tstride = call.rows(table, "table")
-        ip, ids64, n = call.ids(ids, "ids")
-        if out_dtype is not None and out_dtype not in _DTYPES:
-            raise ValueError(f"out_dtype: element type {out_dtype}")
-        if out is None:
-            out = call.empty((*ids.shape, dim), out_dtype if out_dtype is not None else table.dtype)
-        op, _, _, ostride = call.rows(out, "out", dim, n, out_dtype, out=True)
-        _lib.check(_lib.load().omr_embed(tp, _DTYPES[table.dtype], rows, dim, tstride, ip, ids64, n, scale, op,
-                                         _DTYPES[out.dtype], ostride, call.ptr), "omr_embed")
+    call = _Call(table, stream)
+    if table.dim() != 2:
+        raise ValueError(f"table: expected [rows, dim], got shape {tuple(table.shape)}")
+    tp, rows, dim, tstride = call.rows(table, "table")
+    ip, ids64, n = call.ids(ids, "ids")
+    if out_dtype is not None and out_dtype not in _DTYPES:
+        raise ValueError(f"out_dtype: element type {out_dtype}")
+    if out is None:
+        out = call.empty((*ids.shape, dim), out_dtype if out_dtype is not None else table.dtype)
+    op, _, _, ostride = call.rows(out, "out", dim, n, out_dtype, out=True)
+    call.launch("omr_embed", _lib.load().omr_embed, tp, _DTYPES[table.dtype], rows, dim, tstride, ip, ids64, n, scale, op,
+                _DTYPES[out.dtype], ostride)
     return out
 
 
@@ -436,20 +444,19 @@ class EmbedGradPlan:
             scale: float = 1.0, accumulate: bool = False, stream=None) -> torch.Tensor:
         """grad_table[v, :] = scale * (sum of grad_out's rows whose id is v, in token order), every row of it, or added
         to the rows that tokens name (accumulate).  Ids outside [0, rows) contribute nothing."""
-        with _Call(grad_out, stream) as call:
-            ip, ids64, n = call.ids(ids, "ids")
-            if n > self.max_tokens:
-                raise ValueError(f"{n} tokens, the plan is for {self.max_tokens}")
-            gp, _, _, gstride = call.rows(grad_out, "grad_out", self.dim, n)
-            if grad_table is None:
-                if accumulate:
-                    raise ValueError("accumulate needs a grad_table")
-                grad_table = call.empty((self.num_rows, self.dim), torch.float32)
-            tp, _, _, tstride = call.rows(grad_table, "grad_table", self.dim, self.num_rows, torch.float32, out=True)
-            _lib.check(_lib.load().omr_embed_grad_f32(gp, _DTYPES[grad_out.dtype], gstride, ip, ids64, n, self.num_rows,
-                                                      self.dim, scale, tp, tstride, int(accumulate),
-                                                      self.workspace.lend(call), self.workspace.bytes, call.ptr),
-                       "omr_embed_grad_f32")
+        call = _Call(grad_out, stream)
+        ip, ids64, n = call.ids(ids, "ids")
+        if n > self.max_tokens:
+            raise ValueError(f"{n} tokens, the plan is for {self.max_tokens}")
+        gp, _, _, gstride = call.rows(grad_out, "grad_out", self.dim, n)
+        if grad_table is None:
+            if accumulate:
+                raise ValueError("accumulate needs a grad_table")
+            grad_table = call.empty((self.num_rows, self.dim), torch.float32)
+        tp, _, _, tstride = call.rows(grad_table, "grad_table", self.dim, self.num_rows, torch.float32, out=True)
+        call.launch("omr_embed_grad_f32", _lib.load().omr_embed_grad_f32, gp, _DTYPES[grad_out.dtype], gstride, ip, ids64,
+                    n, self.num_rows, self.dim, scale, tp, tstride, int(accumulate), self.workspace.lend(call),
+                    self.workspace.bytes)
         return grad_table
 
 
@@ -468,31 +475,33 @@ class LayerNormGrads:
 
 
 def _param(call: _Call, t: Optional[torch.Tensor], name: str, x: torch.Tensor, dim: int):
-    if t is not None and t.dtype not in (torch.float32, x.dtype):
-        raise ValueError(f"{name}: expected fp32 or {x.dtype}, got {t.dtype}")
-    return call.vector(t, name, dim, t.dtype if t is not None else torch.float32)
+    if t is None:
+        return None
+    dtype = t.dtype
+    if dtype is not _F32 and dtype is not x.dtype:
+        raise ValueError(f"{name}: expected fp32 or {x.dtype}, got {dtype}")
+    return call.vector(t, name, dim, dtype)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5, out: Optional[torch.Tensor] = None, mean: Optional[torch.Tensor] = None,
                rstd: Optional[torch.Tensor] = None, stream=None) -> LayerNormResult:
     """Layer norm over the last dimension; out may be x.  mean and rstd (fp32, one a row) are what the gradient takes."""
-    with _Call(x, stream) as call:
-        xp, n, dim, xstride = call.rows(x, "x")
-        if weight is not None and bias is not None and weight.dtype != bias.dtype:
-            raise ValueError("weight and bias must have one element type")
-        wp, bp = _param(call, weight, "weight", x, dim), _param(call, bias, "bias", x, dim)
-        pdt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-        if out is None:
-            out = call.empty(x.shape, x.dtype)
-        op, _, _, ostride = call.rows(out, "out", dim, n, x.dtype, out=True)
-        if mean is None:
-            mean = call.empty(x.shape[:-1], torch.float32)
-        if rstd is None:
-            rstd = call.empty(x.shape[:-1], torch.float32)
-        _lib.check(_lib.load().omr_layer_norm(xp, _DTYPES[x.dtype], n, dim, xstride, wp, bp, _DTYPES[pdt], eps, op,
-                                              ostride, call.vector(mean, "mean", n), call.vector(rstd, "rstd", n),
-                                              call.ptr), "omr_layer_norm")
+    call = _Call(x, stream)
+    xp, n, dim, xstride = call.rows(x, "x")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias must have one element type")
+    wp, bp = _param(call, weight, "weight", x, dim), _param(call, bias, "bias", x, dim)
+    pdt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+    if out is None:
+        out = call.empty(x.shape, x.dtype)
+    op, _, _, ostride = call.rows(out, "out", dim, n, x.dtype, out=True)
+    if mean is None:
+        mean = call.empty(x.shape[:-1], torch.float32)
+    if rstd is None:
+        rstd = call.empty(x.shape[:-1], torch.float32)
+    call.launch("omr_layer_norm", _lib.load().omr_layer_norm, xp, _DTYPES[x.dtype], n, dim, xstride, wp, bp, _DTYPES[pdt],
+                eps, op, ostride, call.vector(mean, "mean", n), call.vector(rstd, "rstd", n))
     return LayerNormResult(out, mean, rstd)
 
 
@@ -511,30 +520,29 @@ class LayerNormGradPlan:
             accumulate: bool = False, params: bool = True, stream=None) -> LayerNormGrads:
         """grad_x (may be grad_out or x), and the fp32 gradients of weight and bias, written or added to what is there
         (accumulate).  params=False: grad_x alone."""
-        with _Call(x, stream) as call:
-            xp, n, dim, xstride = call.rows(x, "x", self.dim)
-            if n > self.max_rows:
-                raise ValueError(f"{n} rows, the plan is for {self.max_rows}")
-            gp, _, _, gstride = call.rows(grad_out, "grad_out", dim, n, x.dtype)
-            wp = _param(call, weight, "weight", x, dim)
-            pdt = weight.dtype if weight is not None else torch.float32
-            if grad_x is None:
-                grad_x = call.empty(x.shape, x.dtype)
-            op, _, _, ostride = call.rows(grad_x, "grad_x", dim, n, x.dtype, out=True)
-            if not params:
-                if grad_weight is not None or grad_bias is not None:
-                    raise ValueError("params=False takes no grad_weight or grad_bias")
-            elif accumulate:
-                if grad_weight is None and grad_bias is None:
-                    raise ValueError("accumulate needs a grad_weight or a grad_bias")
-            else:
-                grad_weight = grad_weight if grad_weight is not None else call.empty((dim,), torch.float32)
-                grad_bias = grad_bias if grad_bias is not None else call.empty((dim,), torch.float32)
-            _lib.check(_lib.load().omr_layer_norm_grad(
-                gp, gstride, xp, _DTYPES[x.dtype], n, dim, xstride, call.vector(mean, "mean", n),
-                call.vector(rstd, "rstd", n), wp, _DTYPES[pdt], op, ostride, call.vector(grad_weight, "grad_weight", dim),
-                call.vector(grad_bias, "grad_bias", dim), int(accumulate), self.workspace.lend(call),
-                self.workspace.bytes, call.ptr), "omr_layer_norm_grad")
+        call = _Call(x, stream)
+        xp, n, dim, xstride = call.rows(x, "x", self.dim)
+        if n > self.max_rows:
+            raise ValueError(f"{n} rows, the plan is for {self.max_rows}")
+        gp, _, _, gstride = call.rows(grad_out, "grad_out", dim, n, x.dtype)
+        wp = _param(call, weight, "weight", x, dim)
+        pdt = weight.dtype if weight is not None else torch.float32
+        if grad_x is None:
+            grad_x = call.empty(x.shape, x.dtype)
+        op, _, _, ostride = call.rows(grad_x, "grad_x", dim, n, x.dtype, out=True)
+        if not params:
+            if grad_weight is not None or grad_bias is not None:
+                raise ValueError("params=False takes no grad_weight or grad_bias")
+        elif accumulate:
+            if grad_weight is None and grad_bias is None:
+                raise ValueError("accumulate needs a grad_weight or a grad_bias")
+        else:
+            grad_weight = grad_weight if grad_weight is not None else call.empty((dim,), torch.float32)
+            grad_bias = grad_bias if grad_bias is not None else call.empty((dim,), torch.float32)
+        call.launch("omr_layer_norm_grad", _lib.load().omr_layer_norm_grad, gp, gstride, xp, _DTYPES[x.dtype], n, dim,
+                    xstride, call.vector(mean, "mean", n), call.vector(rstd, "rstd", n), wp, _DTYPES[pdt], op, ostride,
+                    call.vector(grad_weight, "grad_weight", dim), call.vector(grad_bias, "grad_bias", dim),
+                    int(accumulate), self.workspace.lend(call), self.workspace.bytes)
         return LayerNormGrads(grad_x, grad_weight, grad_bias)
 
 
@@ -567,15 +575,14 @@ class VocabLossPlan:
     def forward(self, hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
                 loss: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, stream=None):
         """(loss, lse), fp32, one a token: loss = lse - logit of the target; 0 where the target names no row."""
-        with _Call(hidden, stream) as call:
-            args, n = self._inputs(call, hidden, weight, targets)
-            if loss is None:
-                loss = call.empty(targets.shape, torch.float32)
-            if lse is None:
-                lse = call.empty(targets.shape, torch.float32)
-            _lib.check(_lib.load().omr_vocab_loss(*args, call.vector(loss, "loss", n), call.vector(lse, "lse", n),
-                                                  self.workspace.lend(call), self.workspace.bytes, call.ptr),
-                       "omr_vocab_loss")
+        call = _Call(hidden, stream)
+        args, n = self._inputs(call, hidden, weight, targets)
+        if loss is None:
+            loss = call.empty(targets.shape, torch.float32)
+        if lse is None:
+            lse = call.empty(targets.shape, torch.float32)
+        call.launch("omr_vocab_loss", _lib.load().omr_vocab_loss, *args, call.vector(loss, "loss", n),
+                    call.vector(lse, "lse", n), self.workspace.lend(call), self.workspace.bytes)
         return loss, lse
 
     def backward(self, hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
@@ -586,38 +593,38 @@ class VocabLossPlan:
         weight's type (default), written or added to (accumulate); need_hidden / need_weight=False leave one out."""
         if not self.grads:
             raise ValueError("the plan was made with grads=False")
-        with _Call(hidden, stream) as call:
-            args, n = self._inputs(call, hidden, weight, targets)
-            if grad_loss.dtype != torch.float32 or grad_loss.numel() not in (n, 1):
-                raise ValueError(f"grad_loss: fp32, {n} or one, got {grad_loss.dtype}{tuple(grad_loss.shape)}")
-            if grad_loss.numel() == 1 or all(s == 0 for s in grad_loss.stride()):
-                gstride = 0  # (also the gradient of a sum: one value, expanded)
-            elif grad_loss.is_contiguous():
-                gstride = 1
-            else:
-                raise ValueError(f"grad_loss must be contiguous or one value (stride {grad_loss.stride()})")
-            hp = wp = None
-            hstride = wstride = self.dim
-            if need_hidden:
-                if grad_hidden is None:
-                    grad_hidden = call.empty(hidden.shape, self.dtype)
-                hp, _, _, hstride = call.rows(grad_hidden, "grad_hidden", self.dim, n, self.dtype, out=True)
-            elif grad_hidden is not None:
-                raise ValueError("need_hidden=False takes no grad_hidden")
-            if need_weight:
-                if grad_weight is None:
-                    if accumulate:
-                        raise ValueError("accumulate needs a grad_weight")
-                    grad_weight = call.empty(weight.shape, self.dtype)
-                if grad_weight.dtype not in (torch.float32, self.dtype):
-                    raise ValueError(f"grad_weight: fp32 or {self.dtype}, got {grad_weight.dtype}")
-                wp, _, _, wstride = call.rows(grad_weight, "grad_weight", self.dim, self.vocab, out=True)
-            elif grad_weight is not None or accumulate:
-                raise ValueError("need_weight=False takes no grad_weight")
-            _lib.check(_lib.load().omr_vocab_loss_grad(
-                *args, call.vector(lse, "lse", n), call.on(grad_loss, "grad_loss"), gstride, hp, hstride, wp,
-                _DTYPES[grad_weight.dtype] if wp is not None else 0, wstride, int(accumulate),
-                self.workspace.lend(call), self.workspace.bytes, call.ptr), "omr_vocab_loss_grad")
+        call = _Call(hidden, stream)
+        args, n = self._inputs(call, hidden, weight, targets)
+        if grad_loss.dtype != torch.float32 or grad_loss.numel() not in (n, 1):
+            raise ValueError(f"grad_loss: fp32, {n} or one, got {grad_loss.dtype}{tuple(grad_loss.shape)}")
+        if grad_loss.numel() == 1 or all(s == 0 for s in grad_loss.stride()):
+            gstride = 0  # (also the gradient of a sum: one value, expanded)
+        elif grad_loss.is_contiguous():
+            gstride = 1
+        else:
+            raise ValueError(f"grad_loss must be contiguous or one value (stride {grad_loss.stride()})")
+        hp = wp = None
+        hstride = wstride = self.dim
+        if need_hidden:
+            if grad_hidden is None:
+                grad_hidden = call.empty(hidden.shape, self.dtype)
+            hp, _, _, hstride = call.rows(grad_hidden, "grad_hidden", self.dim, n, self.dtype, out=True)
+        elif grad_hidden is not None:
+            raise ValueError("need_hidden=False takes no grad_hidden")
+        if need_weight:
+            if grad_weight is None:
+                if accumulate:
+                    raise ValueError("accumulate needs a grad_weight")
+                grad_weight = call.empty(weight.shape, self.dtype)
+            if grad_weight.dtype not in (torch.float32, self.dtype):
+                raise ValueError(f"grad_weight: fp32 or {self.dtype}, got {grad_weight.dtype}")
+            wp, _, _, wstride = call.rows(grad_weight, "grad_weight", self.dim, self.vocab, out=True)
+        elif grad_weight is not None or accumulate:
+            raise ValueError("need_weight=False takes no grad_weight")
+        call.launch("omr_vocab_loss_grad", _lib.load().omr_vocab_loss_grad, *args, call.vector(lse, "lse", n),
+                    call.on(grad_loss, "grad_loss"), gstride, hp, hstride, wp,
+                    _DTYPES[grad_weight.dtype] if wp is not None else 0, wstride, int(accumulate),
+                    self.workspace.lend(call), self.workspace.bytes)
         return grad_hidden, grad_weight
 
 
