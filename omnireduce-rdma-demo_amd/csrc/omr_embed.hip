@@ -314,7 +314,7 @@ int omr_embed_grad_f32(const void* grad_out, int grad_dtype, uint64_t grad_strid
                  blocks = chunk_blocks + (accumulate ? 0 : ceil_div(num_rows, 4 * a.fill));
   if (blocks > kMaxBlocks || a.chunks * join_tiles > kMaxBlocks)
     return efail("embed_grad: too many tokens or rows for one call");
-  const uint32_t range = sort_range<kSortWaves>(a.rows);
+  const uint32_t range = sort_range(a.rows);
   const unsigned sorters = static_cast<unsigned>(ceil_div(a.rows, range));
   if (ids64)
     k_embed_sort<int64_t><<<sorters, 64 * kSortWaves, 0, S(stream)>>>(static_cast<const int64_t*>(ids), a.tokens, a.rows,

@@ -984,12 +984,19 @@ uint64_t piece_bytes_most(uint64_t tokens, uint64_t vocab) {
   return std::min(std::max(kPieceBytes, tokens * 1024 * 2), tokens * up(vocab, 256) * 2);
 }
 
-// Parts of grad_hidden's inner dimension (the vocabulary piece): two small tiles a CU where its tiles do not fill them, of
-// no less than 512 rows each.
+// Parts of grad_hidden's inner dimension (the vocabulary piece) where its tiles do not fill the CUs, of no less than 512
+// rows each; the parts' sums are written and read again.
+//   - where grad_weight's product goes beside it (launch_both): tiles for one a CU, and parts no shorter than that product's
+//     inner dimension, the tokens (2048 x 4096 x 2048: 138 us backward, 154 with two a CU; 1500 x 3000 x 512: 56, 60)
+//   - else up to 256 tokens, where it is bound by reading the weight: for half the CUs (100 x 32000 x 1024: 73 us, 83 with
+//     two a CU; 128 x 131072 x 1024: 267, 259)
+//   - else for two a CU (1024 x 32000 x 1024: 239 us, 260 with one)
 uint32_t hidden_splits(uint64_t tokens, uint64_t dim, uint32_t piece) {
   if (tile_of(dim, tokens, 1) == kTileBig) return 1;
-  const uint64_t tiles = ceil_div(dim, kSmall) * ceil_div(tokens, kSmall);
-  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(512 / std::min<uint64_t>(tiles, 512), piece / 512)));
+  const bool both = tile_of(dim, piece, 1) != kTileBig;
+  const uint64_t tiles = ceil_div(dim, kSmall) * ceil_div(tokens, kSmall), most = both ? 256 : tokens <= 256 ? 128 : 512;
+  return static_cast<uint32_t>(std::max<uint64_t>(
+      1, std::min<uint64_t>(most / std::min(tiles, most), piece / std::max<uint64_t>(512, both ? tokens : 0))));
 }
 uint64_t acc_bytes_most(uint64_t tokens, uint64_t dim) {
   // splits * tokens * dim * 4 with splits <= 512 / tiles and tokens * dim <= tiles * 128^2
@@ -1205,7 +1212,8 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     if (grad_weight != nullptr) {
       const uint32_t threads = beside ? 256 : 1024;
       p.lpr_log = lanes_log(pdim);
-      p.range = beside ? sort_range<4>(a.vocab) : sort_range<16>(a.vocab);
+      // (beside the product few sorters: they hold places of its tiles)
+      p.range = beside ? SortSpace<4>::kRange : sort_range(a.vocab);
       p.sorters = static_cast<uint32_t>(ceil_div(vocab, p.range));
       const uint64_t blocks = p.sorters + ceil_div(tokens, threads >> p.lpr_log);
       if (blocks >= (1u << 22)) return efail("vocab_loss_grad: too many tokens or rows for one call");

@@ -37,11 +37,10 @@ struct SortSpace {
   uint32_t wsum[WAVES], below_w[WAVES], valid;
 };
 
-// rows per workgroup: one workgroup a CU where the table is small enough for that
-template <int WAVES>
+// rows per workgroup of 16 waves: one workgroup a CU where the table is small enough for that
 inline uint32_t sort_range(uint32_t rows) {
   const uint32_t each = (rows + 255) / 256;
-  return each < 16 ? 16 : each > SortSpace<WAVES>::kRange ? SortSpace<WAVES>::kRange : each;
+  return each < 16 ? 16 : each > SortSpace<16>::kRange ? SortSpace<16>::kRange : each;
 }
 
 // Workgroup `block` of WAVES waves: the positions of the ids that name one of its rows, by row and in order
