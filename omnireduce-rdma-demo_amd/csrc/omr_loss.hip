@@ -868,16 +868,28 @@ __global__ __launch_bounds__(1024) void k_largest(GemmArgs<T> a, float* amax) {
   if (threadIdx.x == 0) *amax = m;
 }
 
-// Rows copied into whole 16-byte pieces [rows][pdim], zeros behind dim; 2^lpr_log lanes a row.
+// Rows copied into whole 16-byte pieces [rows][pdim], zeros behind dim; 2^lpr_log lanes a row.  Two matrices, either of
+// which may have no rows: a launch less (4 us).
 template <class T>
-__global__ __launch_bounds__(256) void k_pack(const T* src, uint64_t stride, uint32_t rows, uint32_t dim, uint32_t pdim,
-                                              uint32_t lpr_log, T* dst) {
-  const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x) >> lpr_log;
-  if (row >= rows) return;
+struct PackArgs {
+  const T* src;
+  uint64_t stride, rows;
+  T* dst;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void k_pack(PackArgs<T> x, PackArgs<T> y, uint32_t dim, uint32_t pdim,
+                                              uint32_t lpr_log) {
+  uint64_t row = (static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x) >> lpr_log;
+  if (row >= x.rows + y.rows) return;
+  const bool first = row < x.rows;
+  if (!first) row -= x.rows;
+  const T* src = (first ? x.src : y.src) + row * (first ? x.stride : y.stride);
+  T* dst = (first ? x.dst : y.dst) + row * pdim;
   for (uint32_t c = (threadIdx.x & ((1u << lpr_log) - 1)) * 8; c < pdim; c += 8u << lpr_log) {
     float v[8];
-    load_some<T, 8>(src + row * stride + c, dim - c, v);
-    store_f32<T, 8>(dst + row * pdim + c, v);
+    load_some<T, 8>(src + c, dim - c, v);
+    store_f32<T, 8>(dst + c, v);
   }
 }
 
@@ -1042,36 +1054,29 @@ uint32_t lanes_log(uint32_t pdim) {  // lanes that a row of pdim elements fills,
   return l;
 }
 
-template <class T>
-int pack_rows(const void* src, uint64_t stride, uint64_t rows, uint32_t dim, T* dst, hipStream_t stream) {
-  const uint32_t pdim = static_cast<uint32_t>(up(dim, 8)), lpr_log = lanes_log(pdim);
-  const uint64_t blocks = ceil_div(rows, 256u >> lpr_log);
-  if (blocks >= (1u << 24)) return efail("vocab_loss: too many rows to lay out in one call");
-  k_pack<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T*>(src), stride,
-                                                               static_cast<uint32_t>(rows), dim, pdim, lpr_log, dst);
-  return elaunch("omr_vocab_loss (layout)");
-}
-
 // hidden and weight as row operands of whole 16-byte pieces: the caller's, or copies in the workspace
 template <class T>
 int operands(const void* hidden, uint64_t hstride, const void* weight, uint64_t wstride, uint64_t tokens, uint64_t vocab,
              uint32_t dim, const Space& sp, char* ws, Operand<T>* h, Operand<T>* w, hipStream_t stream) {
-  const uint32_t pdim = static_cast<uint32_t>(up(dim, 8));
+  const uint32_t pdim = static_cast<uint32_t>(up(dim, 8)), lpr_log = lanes_log(pdim);
   *h = {static_cast<const T*>(hidden), hstride, static_cast<uint32_t>(tokens)};
   *w = {static_cast<const T*>(weight), wstride, static_cast<uint32_t>(vocab)};
+  PackArgs<T> x{w->p, wstride, 0, reinterpret_cast<T*>(ws + sp.w)}, y{h->p, hstride, 0, reinterpret_cast<T*>(ws + sp.h)};
   if (dim % 8 != 0 || !rows_ok(weight, wstride)) {
-    T* to = reinterpret_cast<T*>(ws + sp.w);
-    if (const int rc = pack_rows<T>(weight, wstride, vocab, dim, to, stream)) return rc;
-    w->p = to;
+    x.rows = vocab;
+    w->p = x.dst;
     w->ld = pdim;
   }
   if (dim % 8 != 0 || !rows_ok(hidden, hstride)) {
-    T* to = reinterpret_cast<T*>(ws + sp.h);
-    if (const int rc = pack_rows<T>(hidden, hstride, tokens, dim, to, stream)) return rc;
-    h->p = to;
+    y.rows = tokens;
+    h->p = y.dst;
     h->ld = pdim;
   }
-  return 0;
+  if (x.rows + y.rows == 0) return 0;
+  const uint64_t blocks = ceil_div(x.rows + y.rows, 256u >> lpr_log);
+  if (blocks >= (1u << 24)) return efail("vocab_loss: too many rows to lay out in one call");
+  k_pack<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(x, y, dim, pdim, lpr_log);
+  return elaunch("omr_vocab_loss (layout)");
 }
 
 int check_space(const char* what, const void* hidden, uint64_t hstride, const void* weight, uint64_t wstride,
