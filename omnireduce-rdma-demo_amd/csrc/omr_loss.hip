@@ -16,7 +16,7 @@
 // grad_hidden (the library, on these layouts, 470 to 510 and 440 to 460): 3.4 ms in all, 1.3 PFLOP/s.  2048 tokens of 4096
 // against 131072 rows forward: 1.57 ms, 1.40 PFLOP/s, as the library's product.  What bounds them is the power: the clock
 // falls to 1.6 to 1.9 GHz of 2.4, with the matrix units busy 66 to 74 % of it.  The passes over few tiles (333 tokens of
-// 520 against 5003 rows: 14 us forward, 35 back) are bound by their two and three launches, each too short to fill the
+// 520 against 5003 rows: 14 us forward, 34 back) are bound by their two and three launches, each too short to fill the
 // CUs' pipelines.
 //
 // Roundings to 16 bits, besides the outputs':
