@@ -189,6 +189,24 @@ def test_embed_grad_strides_and_untouched_memory(gpu, dim, pad, offset, dtype):
     within(plan.run(one, ids), ref, tol, "broadcast")
 
 
+@pytest.mark.parametrize("rows,dim", [((1 << 25) + 5, 3), ((1 << 20) + 1, 4100)])
+def test_embed_grad_of_a_large_table(gpu, rows, dim):
+    """More rows than a fill workgroup's wave takes one of, and offsets past 2^32 elements."""
+    g = gen(9)
+    ids = torch.tensor([rows - 1, 0, rows - 1, rows, -1, 1 << 20, 77], device="cuda")
+    grad = rand((7, dim), F32, g)
+    out = torch.full((rows, dim), 1.0, device="cuda")
+    ops.EmbedGradPlan(7, rows, dim).run(grad, ids, out)
+    want = {rows - 1: grad[0] + grad[2], 0: grad[1], 77: grad[6]}
+    want[1 << 20] = grad[5] if rows - 1 != 1 << 20 else grad[0] + grad[2] + grad[5]
+    want[rows - 1] = want[1 << 20] if rows - 1 == 1 << 20 else want[rows - 1]
+    for r, v in want.items():
+        assert torch.equal(out[r], v)
+        out[r] = 0
+    step = (1 << 28) // dim
+    assert not any(out[i:i + step].any() for i in range(0, rows, step))
+
+
 def test_embed_grad_is_the_lookups(gpu):
     """<grad(dy), E> = <dy, embed(E)> for any E: the backward is the forward's transpose (in 64 bits of its outputs)."""
     g = gen(3)
@@ -548,6 +566,52 @@ def test_vocab_loss_pieces(gpu, T, V, D, dtype=BF16):
     tw = ((aG * upd.abs()[:, None]).t() @ h.double().abs()) * (2 * half(dtype) * 1.1 + (T + 4) * U) + 1e-6
     within(gh, gh_ref, th + half(dtype) * gh_ref.abs(), "grad_hidden")
     within(gw, gw_ref, tw, "grad_weight")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_vocab_loss_adds_to_a_gradient_of_its_type(gpu, dtype):
+    """What is there is added in fp32, in front of the one rounding: the fp32 gradient's sum with it, rounded."""
+    g = gen(31)
+    for T, V, D in ((60, 300, 72), (700, 2100, 136)):
+        h, w, t, off = loss_inputs(T, V, D, dtype, g)
+        plan = ops.VocabLossPlan(T, V, D, dtype=dtype)
+        _, lse = plan.forward(h, w, t)
+        up = rand((T,), F32, g)
+        fine = plan.backward(h, w, t, lse, up, grad_weight=torch.empty(V, D, device="cuda"), need_hidden=False)[1]
+        base = rand((V, D), dtype, g)
+        got = base.clone()
+        plan.backward(h, w, t, lse, up, grad_weight=got, accumulate=True, need_hidden=False)
+        assert torch.equal(got, (base.float() + fine).to(dtype))
+
+
+def test_optional_parameters_and_expanded_inputs(gpu):
+    g = gen(32)
+    x, dy, w, b = rand((37, 264), F32, g), rand((37, 264), F32, g), rand((264,), F32, g), rand((264,), F32, g)
+    ones, zeros = torch.ones(264, device="cuda"), torch.zeros(264, device="cuda")
+    for weight, bias in ((None, None), (w, None), (None, b)):
+        f = ops.layer_norm(x, weight, bias)
+        assert torch.equal(f.out, ops.layer_norm(x, ones if weight is None else w, zeros if bias is None else b).out)
+    plan = ops.LayerNormGradPlan(37, 264)
+    full = plan.run(dy, x, f.mean, f.rstd, w)
+    assert torch.equal(plan.run(dy, x, f.mean, f.rstd).grad_x, plan.run(dy, x, f.mean, f.rstd, ones).grad_x)
+    for k in ("grad_weight", "grad_bias"):  # one alone, added to
+        base = rand((264,), F32, g)
+        r = plan.run(dy, x, f.mean, f.rstd, w, accumulate=True, **{k: base.clone()})
+        assert torch.equal(getattr(r, k), base + getattr(full, k)) and torch.equal(r.grad_x, full.grad_x)
+        assert getattr(r, {"grad_weight": "grad_bias", "grad_bias": "grad_weight"}[k]) is None
+    one = dy[:1].expand(37, 264)  # a row for all: a stride of 0
+    r, q = (plan.run(d, x, f.mean, f.rstd, w) for d in (one, one.contiguous()))
+    assert torch.equal(r.grad_x, q.grad_x) and torch.equal(r.grad_weight, q.grad_weight)
+    ids = make_ids(37, 11, g, "any")
+    e = ops.EmbedGradPlan(37, 11, 264)
+    assert torch.equal(e.run(one, ids), e.run(one.contiguous(), ids))
+    table = dy[:1].expand(11, 264)
+    assert torch.equal(ops.embed(table, ids), ops.embed(table.contiguous(), ids))
+    loss = ops.VocabLossPlan(37, 11, 264, pack=True)
+    t = torch.randint(0, 11, (37,), generator=g, device="cuda")
+    hb, wb = one.to(BF16)[:1].expand(37, 264), rand((11, 264), BF16, g)
+    (la, ea), (lb, eb) = loss.forward(hb, wb, t), loss.forward(hb.contiguous(), wb, t)
+    assert torch.equal(la, lb) and torch.equal(ea, eb)
 
 
 # ---------------------------------------------------------------------------------------------------- streams, graphs
