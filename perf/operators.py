@@ -17,21 +17,14 @@ own = False
 DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 
 
-_module = None
-
-
 def _ops():
-    """The package's operators, imported once."""
-    global _module
-    if _module is None:
-        root = os.path.join(os.getcwd(), "omnireduce-rdma-demo_amd")  # the working folder is the repository's root
-        if not os.path.isdir(root):
-            root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "omnireduce-rdma-demo_amd")
-        if root not in sys.path:
-            sys.path.insert(0, root)
-        from omr import ops
-        _module = ops
-    return _module
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "omnireduce-rdma-demo_amd")
+    if not os.path.isdir(root):  # the working folder is the repository's root
+        root = os.path.join(os.getcwd(), "omnireduce-rdma-demo_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from omr import ops
+    return ops
 
 
 # ---------------------------------------------------------------------------------------------------- the cases
