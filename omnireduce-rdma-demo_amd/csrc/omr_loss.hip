@@ -21,9 +21,10 @@
 //
 // Roundings to 16 bits, besides the outputs':
 //   - G, times 2^12 so that fp16 keeps the small probabilities normal (2^-26 and up).  The targets' entries, exp(..) - 1,
-//     outweigh the others together: what their rounding loses (`lost`, one value a token) is added to both products in
-//     fp32 (to a row of grad_weight only where it is at most kFewTargets tokens' target: more tokens' errors average out).
-//     Without that a few tokens' gradient was off by up to 2^-8 in bf16, twice what the output's own rounding is.
+//     outweigh the others together: what their rounding loses (`lost`, one value a token) is added to both products, to
+//     grad_hidden in fp32, to grad_weight as a product of its own in 16 bits (2^-18 of the entry remains in bf16).  Without
+//     that a target's row was off by up to 2^-9 in bf16, however many tokens share it: 2^12 (p - 1) rounds to -2^12 for
+//     every p below 2^-9, always to the same side.
 //   - hidden[n] * (grad_loss[n] / max |grad_loss|) for grad_weight's sum over tokens: exact where grad_loss is the same
 //     for every token (the mean and the sum), else one rounding.
 // Sums are in fp32 throughout.
@@ -37,7 +38,6 @@ using namespace omr_elem;
 
 namespace {
 
-constexpr uint32_t kFewTargets = 8;
 constexpr float kGScale = 4096.0f, kLog2E = 1.44269504f;
 constexpr uint32_t kMaxStride = 1u << 22;  // elements: a tile's 32-bit byte offsets hold 256 rows of it
 
@@ -131,6 +131,22 @@ struct Tile {
                  : "memory");
   }
   __device__ __forceinline__ void advance() { base += inc; }
+
+  // a column operand's tile whose k-th row is row which[k] of the operand, k < left; zeros behind them
+  __device__ __forceinline__ void load_rows(const Operand<T>& o, uint32_t row0, const uint32_t* which, uint32_t left,
+                                            uint32_t to) const {
+    static_assert(COL, "rows of k");
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t k = kfirst(i), at = off[i] - static_cast<uint32_t>(k * o.ld * sizeof(T));
+      const char* src = k < left ? reinterpret_cast<const char*>(o.p + which[k] * o.ld + row0) + at
+                                 : reinterpret_cast<const char*>(g_zero);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                   :
+                   : "s"(to + i * NT * 16), "v"(src)
+                   : "memory");
+    }
+  }
 
   // a tile of `left` k, zeros behind them
   __device__ __forceinline__ void load_end(uint32_t to, uint32_t left) const {
@@ -576,26 +592,46 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs<T>& a, uint32_t id, T* 
   } else {
     const float scale = *a.amax / kGScale;
     const bool direct = a.out_f32 || a.accumulate;  // (a sum with what is there is rounded once, behind the addition)
+    // What rounding took from the targets' entries: a product with the tokens whose target is one of the tile's rows, which
+    // lie together in perm, 64 of them at a time.  A token's entry is in one row; its place and value wait in LDS.
+    T* const lv = lds + R * BM * kBK;
+    uint16_t* const lr = reinterpret_cast<uint16_t*>(lv + kBK);
+    const uint32_t s1 = a.start[min(a.v0 + n0 + BN, a.vocab)];
+    for (uint32_t s = a.start[min(a.v0 + n0, a.vocab)]; s < s1; s += kBK) {
+      ta.load_rows(a.a, m0, a.perm + s, s1 - s, ta.place(lds));
+      if (threadIdx.x < kBK) {
+        const bool real = s + threadIdx.x < s1;
+        const uint32_t tok = real ? a.perm[s + threadIdx.x] : 0;
+        lv[threadIdx.x] = real ? static_cast<T>(a.lost[tok]) : static_cast<T>(0.0f);
+        lr[threadIdx.x] = real ? static_cast<uint16_t>(target_of(a, tok) - static_cast<int>(a.v0 + n0)) : 0;
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const uint32_t g = lane >> 4;
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
+      for (int h = 0; h < 2; ++h) {
+        fa.touch();
+        const frag<T> value = *reinterpret_cast<const frag<T>*>(lv + 32 * h + 8 * g);
+        const vec_t<uint16_t, 8> place = *reinterpret_cast<const vec_t<uint16_t, 8>*>(lr + 32 * h + 8 * g);
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            y[0][j][e] = place[e] == wn * NW + 16 * j + (lane & 15) ? value[e] : static_cast<T>(0.0f);
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+          x[0][i] = fa.get(lds, h, i);
+#pragma unroll
+          for (int j = 0; j < NF; ++j) acc[i][j] = mma(x[0][i], y[0][j], acc[i][j]);
+        }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; direct && j < NF; ++j) {
       const uint32_t row = n + 16 * j;
       if (a.v0 + row >= a.vocab) continue;
       const uint64_t o = static_cast<uint64_t>(a.v0 + row) * a.ostride;
-      const uint32_t t0 = a.start[a.v0 + row], t1 = a.start[a.v0 + row + 1];
-      if (t1 - t0 <= kFewTargets)
-        for (uint32_t t = t0; t < t1; ++t) {
-          const uint32_t tok = a.perm[t];
-          const float lost = a.lost[tok];
-#pragma unroll
-          for (int i = 0; i < MF; ++i)
-            if (m + 16 * i < a.dim) {
-              float f[4];
-              load_f32<T, 4>(a.a.p + tok * a.a.ld + m + 16 * i, f);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) acc[i][j][r] += lost * f[r];
-            }
-        }
-      if (!direct) continue;
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         const uint32_t c = m + 16 * i;

@@ -1,0 +1,76 @@
+"""Where 16-bit storage could cost the operators more than their outputs' own rounding: what is held of the
+loss's gradient for the targets.
+
+Tolerances are worst-case rounding bounds, as in test_accuracy_operators.py."""
+import pytest
+import torch
+
+from omr import ops
+from test_accuracy_operators import BF16, F16, U, gen, half, rand, tiny, within
+
+pytestmark = pytest.mark.gpu
+
+
+def check_gradients(plan, h, w, t, up, dtype, grad_weight):
+    """The backward pass against 64 bits.  G of a token's target has no rounding to 16 bits: what that loses is added to
+    grad_hidden in fp32, and to grad_weight as one more 16-bit value (half a step of half a step).  The other entries have
+    one, or what fp16 loses of them below its range (2^-25 / 2^12; no more than the entry itself).  Hidden states times
+    their share of the largest factor are rounded once, and not at all where all factors are equal; their smallest step in
+    fp16 is that of a row whose largest product is stored as 2^12 or more."""
+    T, V, D = h.shape[0], w.shape[0], h.shape[1]
+    off = (t < 0) | (t >= V)
+    who = torch.arange(T, device="cuda")[~off]
+    _, lse = plan.forward(h, w, t)
+    H, W, AW = torch.where(off[:, None], 0.0, h.double()), w.double(), w.double().abs()
+    e = ((H.abs() @ AW.t()).amax(1) * D * U)[:, None] + 100 * U  # a logit's error, the exponential's, its argument's
+    P = torch.exp(H @ W.t() - lse.double()[:, None])
+    G = P.clone()
+    G[who, t[who]] -= 1
+    G[off], P[off] = 0, 0
+    upd = torch.where(off, 0.0, up.double())
+    dG = torch.minimum(G.abs() * half(dtype) + 2.0 ** -37, G.abs())
+    dG[who, t[who]] = 0
+    dG += P * 2 * e
+    at = torch.zeros_like(G)
+    at[who, t[who]] = G[who, t[who]].abs()
+    AG = G.abs()
+    gh, gw = plan.backward(h, w, t, lse, up, grad_weight=grad_weight)
+    gh_ref = upd[:, None] * (G @ W)
+    tol = upd.abs()[:, None] * ((dG + at * 4 * U) @ AW + (V + 4) * U * (AG @ AW))
+    within(gh, gh_ref, tol * (1 + half(dtype)) + half(dtype) * gh_ref.abs() + tiny(dtype), "grad_hidden")
+    gw_ref = (G * upd[:, None]).t() @ H
+    one = bool((up[~off] == up[~off][:1]).all())
+    entry = dG + at * half(dtype) ** 2 + AG * ((T + 4) * U + (0 if one else half(dtype)))
+    tol = (entry * upd.abs()[:, None]).t() @ H.abs()
+    if not one and dtype == F16:
+        tol += AG.sum(0)[:, None] * 2.0 ** -37 * (upd[:, None] * H).abs().max()
+    round_ = half(gw.dtype)
+    within(gw, gw_ref, tol * (1 + round_) + round_ * gw_ref.abs() + tiny(gw.dtype), "grad_weight")
+    assert torch.equal(plan.backward(h, w, t, lse, up)[0], gh)  # the same bits
+
+
+def targets_of(T, V, g, kind):
+    if kind == "one":
+        return torch.full((T,), V // 2, device="cuda")
+    if kind == "words":  # a few low ids take many of the tokens
+        return (torch.rand(T, generator=g, device="cuda", dtype=torch.float64) ** 3 * V).long().clamp_(max=V - 1)
+    return torch.arange(T, device="cuda") // 9 % V  # nine tokens each
+
+
+@pytest.mark.parametrize("T,V,D,kind", [
+    (9, 300, 64, "one"), (64, 1000, 72, "one"), (65, 1000, 61, "one"), (512, 1000, 128, "one"), (512, 1000, 128, "nine"),
+    (333, 5003, 520, "words"), (8, 20000, 136, "one"), (700, 70000, 64, "words"), (2048, 8192, 256, "words"),
+    (4100, 70001, 72, "words"), (1500, 3000, 1040, "nine")])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_targets_lose_nothing_to_rounding(gpu, T, V, D, kind, dtype):
+    """However many tokens share a target: in bf16 2^12 (p - 1) is -2^12 for every p below 2^-9, always to the same side, so
+    without the correction a row of many such tokens is off by the mean of their p."""
+    g = gen(T + V)
+    w = rand((V, D), dtype, g, std=0.5 * D ** -0.5)
+    h = rand((T, D), dtype, g)
+    t = targets_of(T, V, g, kind)
+    if T > 20:
+        t[3::17] = -1
+    plan = ops.VocabLossPlan(T, V, D, dtype=dtype)
+    for gw in (torch.empty(V, D, device="cuda"), None):
+        check_gradients(plan, h, w, t, torch.full((T,), 1.0 / T, device="cuda"), dtype, gw)
