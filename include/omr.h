@@ -512,7 +512,9 @@ int omr_vocab_loss(const void* hidden, uint64_t hidden_stride, const void* weigh
  *   grad_weight[v, :] = sum over n of G[n, v] grad_loss[n] hidden[n, :]        (grad_weight_dtype: fp32 or dtype)
  * either may be NULL; accumulate != 0 adds to grad_weight.  Tokens without a target contribute nothing and get a row of
  * zeros, whatever their hidden states and grad_loss hold.  An fp32 grad_weight (a bucket of the all-reduce) is summed
- * in fp32 from terms of `dtype`'s precision.  The workspace needs grads != 0 above. */
+ * in fp32 from terms of `dtype`'s precision: each G and each grad_loss hidden is rounded to it once (in fp16 that holds for
+ * G from 2^-26 on, and for grad_loss hidden from 2^-27 of the largest of them on; what is smaller is held in steps of 2^-36,
+ * and of 2^-37 of the largest).  The workspace needs grads != 0 above. */
 int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* weight, uint64_t weight_stride,
                         int dtype, uint64_t tokens, uint64_t vocab, uint32_t dim, const void* targets, int targets64,
                         const float* lse, const float* grad_loss, uint64_t grad_loss_stride, void* grad_hidden,

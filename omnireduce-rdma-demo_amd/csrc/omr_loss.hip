@@ -26,7 +26,9 @@
 //     that a target's row was off by up to 2^-9 in bf16, however many tokens share it: 2^12 (p - 1) rounds to -2^12 for
 //     every p below 2^-9, always to the same side.
 //   - hidden[n] * (grad_loss[n] / max |grad_loss|) for grad_weight's sum over tokens: exact where grad_loss is the same
-//     for every token (the mean and the sum), else one rounding.
+//     for every token (the mean and the sum), else one rounding.  In fp16 these products are scaled by the power of two that
+//     brings the largest of them to 2^13 or more: the one rounding then holds down to 2^-27 of the largest (without it, one
+//     of 1e-6 of the largest |grad_loss| was off by 2 %, and one of 1e-8 lost).
 // Sums are in fp32 throughout.
 #include "omr_sort.h"
 
@@ -223,7 +225,7 @@ struct GemmArgs {
   int first, last;          // the sum over the pieces begins; is complete and goes to `out`
   const float* up;          // grad_loss, upstride apart
   uint64_t upstride;
-  const float* amax;        // [1] the largest |grad_loss| of the tokens with a target
+  const float* amax;        // [2] the largest |grad_loss| of the tokens with a target; the scale of the hidden states' copy
   float* lost;              // [tokens] what the target's entry of G lost in rounding
   Operand<T> w;             // kHidden: the whole weight
   const uint32_t *start, *perm;  // kWeight: the tokens by target
@@ -590,7 +592,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs<T>& a, uint32_t id, T* 
                          a.ostride, v);
           });
   } else {
-    const float scale = *a.amax / kGScale;
+    const float most = a.amax[0], unscale = 1.0f / (kGScale * a.amax[1]);  // (a power of two: exact, and first)
     const bool direct = a.out_f32 || a.accumulate;  // (a sum with what is there is rounded once, behind the addition)
     // What rounding took from the targets' entries: a product with the tokens whose target is one of the tile's rows, which
     // lie together in perm, 64 of them at a time.  A token's entry is in one row; its place and value wait in LDS.
@@ -636,7 +638,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs<T>& a, uint32_t id, T* 
       for (int i = 0; i < MF; ++i) {
         const uint32_t c = m + 16 * i;
         if (c >= a.dim) continue;
-        const v4f v = acc[i][j] * scale;
+        const v4f v = acc[i][j] * unscale * most;
         if (a.out_f32)
           put4<float>(static_cast<float*>(a.out) + o + c, v, a.dim - c, a.accumulate);
         else
@@ -649,7 +651,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs<T>& a, uint32_t id, T* 
           [&](int i, int j) {
             vec_t<T, 4> o;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(acc[i][j][r] * scale);
+            for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(acc[i][j][r] * unscale * most);
             return o;
           },
           [&](uint32_t row, uint32_t c, const vec_t<T, 8>& v) {
@@ -703,6 +705,65 @@ __device__ __forceinline__ float largest(const GemmArgs<T>& a, float* lds) {
   return m;
 }
 
+// What of the hidden states' copy has to fit fp16, by a workgroup: the largest |grad_loss| of some tokens with a target, and
+// the least e with |grad_loss[n] hidden[n, c]| < 2^e for all of them (from the factors' exponents: the product may pass
+// fp32's range).
+struct Reach {
+  float most;
+  int e;
+};
+constexpr int kNoReach = -1000;
+constexpr uint32_t kReachBlocks = 256;
+
+template <class T>
+__global__ __launch_bounds__(256) void k_reach(GemmArgs<T> a, const T* hidden, uint64_t stride, uint32_t lpr_log, Reach* out) {
+  __shared__ Reach part[4];
+  Reach r{0.0f, kNoReach};
+  const uint64_t step = gridDim.x * (256u >> lpr_log);
+  for (uint64_t row = (static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x) >> lpr_log; row < a.tokens; row += step) {
+    const float g = fabsf(factor_of(a, static_cast<uint32_t>(row)));
+    if (g == 0.0f) continue;
+    r.most = r.most != r.most || g <= r.most ? r.most : g;
+    float top = 0.0f;
+    for (uint32_t c = (threadIdx.x & ((1u << lpr_log) - 1)) * 8; c < a.dim; c += 8u << lpr_log) {
+      float v[8];
+      load_some<T, 8>(hidden + row * stride + c, a.dim - c, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+    }
+    const float m = __builtin_amdgcn_frexp_mantf(g) * __builtin_amdgcn_frexp_mantf(top);
+    if (top != 0.0f)
+      r.e = max(r.e, __builtin_amdgcn_frexp_expf(g) + __builtin_amdgcn_frexp_expf(top) + __builtin_amdgcn_frexp_expf(m));
+  }
+  auto more = [&](float most, int e) {
+    r.most = r.most != r.most || most <= r.most ? r.most : most;
+    r.e = max(r.e, e);
+  };
+#pragma unroll
+  for (int d = 32; d; d >>= 1) more(__shfl_xor(r.most, d), __shfl_xor(r.e, d));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = r;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 4; ++w) more(part[w].most, part[w].e);
+  out[blockIdx.x] = r;
+}
+
+// The parts of all of k_reach's workgroups together, in every lane of a wave: the largest |grad_loss|, and the power of two
+// that the shares are scaled by: |grad_loss[n] / most hidden[n, c]| < 2^(e - exponent of most + 1), which goes to 2^15.
+// (Not below 1: a share is no larger than the hidden state itself.)
+__device__ __forceinline__ float2 reach_of(const Reach* parts, uint32_t n) {
+  Reach r{0.0f, kNoReach};
+  auto more = [&](float most, int e) {
+    r.most = r.most != r.most || most <= r.most ? r.most : most;
+    r.e = max(r.e, e);
+  };
+  for (uint32_t i = threadIdx.x & 63; i < n; i += 64) more(parts[i].most, parts[i].e);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) more(__shfl_xor(r.most, d), __shfl_xor(r.e, d));
+  const int up = r.e == kNoReach ? 0 : 14 - r.e + __builtin_amdgcn_frexp_expf(r.most);
+  return make_float2(r.most, __builtin_ldexpf(1.0f, min(max(up, 0), 40)));
+}
+
 // What grad_weight's product needs besides G, by workgroups of WAVES waves: blocks [0, sorters) sort the tokens by target;
 // the others copy the hidden states into whole 16-byte pieces, zeros behind dim, each row times its share of the largest
 // grad_loss, and zeros for tokens without a target, whatever they hold.  Up to kFindHere tokens each of these finds the
@@ -718,6 +779,8 @@ struct PrepareArgs {
   uint64_t stride;
   uint32_t pdim, lpr_log;  // 2^lpr_log lanes a row
   float* amax;
+  const Reach* parts;      // fp16 with a factor for each token, else null: every token's scale is 1
+  uint32_t nparts;
   T* dst;
 };
 
@@ -730,16 +793,23 @@ __device__ __forceinline__ void prepare(const GemmArgs<T>& a, const PrepareArgs<
     return;
   }
   block -= p.sorters;
-  float most;
-  if (a.tokens <= kFindHere) {
+  float most, scale = 1.0f;
+  if (p.parts != nullptr) {
+    const float2 r = reach_of(p.parts, p.nparts);
+    most = r.x;
+    scale = r.y;
+  } else if (a.tokens <= kFindHere) {
     most = largest<T, WAVES>(a, reinterpret_cast<float*>(space.wsum));
-    if (block == 0 && threadIdx.x == 0) *p.amax = most;
   } else {
     most = *p.amax;
   }
+  if (block == 0 && threadIdx.x == 0) {
+    if (p.parts != nullptr || a.tokens <= kFindHere) p.amax[0] = most;  // (else it is there)
+    p.amax[1] = scale;
+  }
   const uint64_t row = (static_cast<uint64_t>(block) * 64 * WAVES + threadIdx.x) >> p.lpr_log;
   if (row >= a.tokens) return;
-  const float g = factor_of(a, static_cast<uint32_t>(row)), by = g == 0.0f ? 0.0f : g / most;
+  const float g = factor_of(a, static_cast<uint32_t>(row)), by = g == 0.0f ? 0.0f : g / most * scale;
   for (uint32_t c = (threadIdx.x & ((1u << p.lpr_log) - 1)) * 8; c < p.pdim; c += 8u << p.lpr_log) {
     float v[8] = {};
     if (by != 0.0f) {
@@ -1073,7 +1143,7 @@ Space layout(uint64_t tokens, uint64_t vocab, uint64_t dim, bool pack, bool grad
   s.h = s.w + (pack ? up(vocab * pdim * 2, 256) : 0);
   s.rest = s.h + (pack ? up(tokens * pdim * 2, 256) : 0);
   uint64_t fwd = up(tokens * 4, 256) + stats_bytes_most(tokens, vocab);
-  uint64_t bwd = 256 + 2 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) +
+  uint64_t bwd = 256 + kReachBlocks * sizeof(Reach) + 2 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) +
                  up(piece_bytes_most(tokens, vocab), 256) + acc_bytes_most(tokens, dim);
   s.bytes = s.rest + (grads ? std::max(fwd, bwd) : fwd) + 256;
   return s;
@@ -1234,7 +1304,8 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
       at += up(bytes, 256);
       return p;
     };
-    float* amax = reinterpret_cast<float*>(take(4));
+    float* amax = reinterpret_cast<float*>(take(8));
+    Reach* reach = reinterpret_cast<Reach*>(take(kReachBlocks * sizeof(Reach)));
     float* lost = reinterpret_cast<float*>(take(tokens * 4));
     uint32_t* perm = reinterpret_cast<uint32_t*>(take(tokens * 4));
     uint32_t* start = reinterpret_cast<uint32_t*>(take(4 * vocab + 4));
@@ -1271,8 +1342,14 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
       p.pdim = pdim;
       p.amax = amax;
       p.dst = clean;
+      if (dtype == OMR_F16 && grad_loss_stride != 0) {
+        p.parts = reach;
+        p.nparts = static_cast<uint32_t>(std::min<uint64_t>(ceil_div(tokens, 256u >> p.lpr_log), kReachBlocks));
+        k_reach<T><<<p.nparts, 256, 0, S(stream)>>>(a, p.src, p.stride, p.lpr_log, reach);
+        if (const int rc = elaunch("omr_vocab_loss_grad (reach)")) return rc;
+      }
       if (!beside) {
-        if (tokens > kFindHere) {
+        if (p.parts == nullptr && tokens > kFindHere) {
           k_largest<T><<<1, 1024, 0, S(stream)>>>(a, amax);
           if (const int rc = elaunch("omr_vocab_loss_grad (largest)")) return rc;
         }

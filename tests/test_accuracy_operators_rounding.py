@@ -1,5 +1,5 @@
-"""Where 16-bit storage could cost the operators more than their outputs' own rounding: what is held of the
-loss's gradient for the targets.
+"""Where 16-bit storage or a large mean could cost the operators more than their outputs' own rounding: what is held of the
+loss's gradient for the targets, and tokens of very unequal factors.
 
 Tolerances are worst-case rounding bounds, as in test_accuracy_operators.py."""
 import pytest
@@ -16,7 +16,7 @@ def check_gradients(plan, h, w, t, up, dtype, grad_weight):
     grad_hidden in fp32, and to grad_weight as one more 16-bit value (half a step of half a step).  The other entries have
     one, or what fp16 loses of them below its range (2^-25 / 2^12; no more than the entry itself).  Hidden states times
     their share of the largest factor are rounded once, and not at all where all factors are equal; their smallest step in
-    fp16 is that of a row whose largest product is stored as 2^12 or more."""
+    fp16 is that of a row whose largest product is stored as 2^13 or more."""
     T, V, D = h.shape[0], w.shape[0], h.shape[1]
     off = (t < 0) | (t >= V)
     who = torch.arange(T, device="cuda")[~off]
@@ -43,7 +43,7 @@ def check_gradients(plan, h, w, t, up, dtype, grad_weight):
     entry = dG + at * half(dtype) ** 2 + AG * ((T + 4) * U + (0 if one else half(dtype)))
     tol = (entry * upd.abs()[:, None]).t() @ H.abs()
     if not one and dtype == F16:
-        tol += AG.sum(0)[:, None] * 2.0 ** -37 * (upd[:, None] * H).abs().max()
+        tol += AG.sum(0)[:, None] * 2.0 ** -38 * (upd[:, None] * H).abs().max()
     round_ = half(gw.dtype)
     within(gw, gw_ref, tol * (1 + round_) + round_ * gw_ref.abs() + tiny(gw.dtype), "grad_weight")
     assert torch.equal(plan.backward(h, w, t, lse, up)[0], gh)  # the same bits
@@ -74,3 +74,28 @@ def test_targets_lose_nothing_to_rounding(gpu, T, V, D, kind, dtype):
     plan = ops.VocabLossPlan(T, V, D, dtype=dtype)
     for gw in (torch.empty(V, D, device="cuda"), None):
         check_gradients(plan, h, w, t, torch.full((T,), 1.0 / T, device="cuda"), dtype, gw)
+
+
+@pytest.mark.parametrize("T,D", [(40, 64), (200, 77), (1500, 136), (5000, 64)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_tokens_of_small_factors_count(gpu, T, D, dtype):
+    """Factors from 1 to 1e-8 of the largest.  Every token is sure of a word of its own kind (logits of some 80 against 8
+    and less) that is not its target, and its target is nobody else's: that row of grad_weight is its hidden state times
+    its factor, whatever the others' factors are."""
+    g = gen(T + D)
+    V, K = T + 32, 32
+    w = rand((V, D), dtype, g, std=0.01)
+    w[:K] = 0
+    w[torch.arange(K), torch.arange(K)] = 8.0
+    h = (torch.rand(T, D, generator=g, device="cuda") * 0.7 + 0.3).to(dtype)
+    h[torch.arange(T), torch.arange(T) % K] = 10.0
+    t = K + torch.randperm(T, generator=g, device="cuda")
+    up = 10.0 ** (-8 * torch.rand(T, generator=g, device="cuda"))
+    up[0], up[1:4] = 1.0, torch.tensor([1e-6, -1e-7, 0.0], device="cuda")
+    up[T // 2::7] *= -1
+    plan = ops.VocabLossPlan(T, V, D, dtype=dtype)
+    for scale in (1.0, 1e-6, 1e3):
+        check_gradients(plan, h, w, t, up * scale, dtype, torch.empty(V, D, device="cuda"))
+    check_gradients(plan, (h.float() * 1e-3).to(dtype), w, t, up, dtype, torch.empty(V, D, device="cuda"))
+    check_gradients(plan, (h.float() * 300).to(dtype), (w.float() / 300).to(dtype), t, up, dtype,
+                    torch.empty(V, D, device="cuda"))
