@@ -6,7 +6,9 @@
 //
 // Both are bound by HBM (the forward reads and writes each element once, the backward reads two and writes one), so a
 // row is read once and held in registers: WPR waves hold a row, 16 columns a lane, and statistics are two-pass sums over
-// the registers (the mean first, then the squared distances), which lose nothing to a large mean.  Workgroups walk
+// the registers: the mean first, then the distances d from it and their squares.  A mean far from zero is off by some of its
+// own roundings, which the distances' mean c shows: mean + c, d - c and mean(d^2) - c^2 lose nothing to it (without that
+// a row of 1000 times 10000.1 gave -0.3 for each, where it gives 0).  Workgroups walk
 // several rows, so the parameters are loaded once, the next row is loaded while one is worked on, and the backward keeps
 // its part of dw and db in registers until its last row: one partial row a workgroup, which a second launch adds up in a
 // fixed order.  16384 rows of 4096 bf16 forward: 50 us, 5.4 TB/s (62 without the row ahead; a large copy reaches 5.1);
@@ -54,6 +56,39 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
   return v;
 }
 
+// Two such sums behind one barrier.
+template <int WPR>
+__device__ __forceinline__ float2 row_sum2(float v, float q, float2* lds) {
+  v = wave_sum(v);
+  q = wave_sum(q);
+  if constexpr (WPR > 1) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = make_float2(v, q);
+    __syncthreads();
+    v = lds[0].x;
+    q = lds[0].y;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) {
+      v += lds[w].x;
+      q += lds[w].y;
+    }
+  }
+  return make_float2(v, q);
+}
+
+// The mean's first estimate, rounded: one value for the distances and for what their mean is added to (a product joined to
+// the subtraction behind it, as the compiler may, would give the distances from another one).
+__device__ __forceinline__ float estimate(float sum, float inv_dim) {
+  float near = sum * inv_dim;
+  asm volatile("" : "+v"(near));
+  return near;
+}
+
+// 1 / sqrt(variance + eps) from the means of the distances and of their squares (which round to less than nothing at times)
+__device__ __forceinline__ float rstd_of(float c, float squares, float eps) {
+  const float var = squares - c * c;
+  return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+}
+
 // VEC elements as they lie in memory, at any alignment; of a row's last piece the first n
 template <class T, int VEC>
 struct Piece {
@@ -82,7 +117,8 @@ __device__ __forceinline__ uint32_t have(uint32_t dim, uint32_t c) {
 template <class T, class P, int WPR, bool END>
 __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) {
   constexpr int VEC = 16 / sizeof(T), NV = kCols / VEC, RPB = WPR == 1 ? 4 : 1;
-  __shared__ float lds[2][WPR];
+  __shared__ float lds[WPR];
+  __shared__ float2 lds2[WPR];
   // a lane's columns: VEC consecutive ones of every piece j
   const uint32_t t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
   auto col = [&](int j) { return (static_cast<uint32_t>(j) * 64 * WPR + t) * VEC; };
@@ -136,25 +172,28 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
       for (int i = 0; i < VEC; ++i) piece += v[j][i];
       s += in(j) ? piece : 0.0f;
     }
-    const float mean = row_sum<WPR>(s, lds[0]) * a.inv_dim;
-    float q = 0.0f;
+    const float near = estimate(row_sum<WPR>(s, lds), a.inv_dim);
+    float d = 0.0f, q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      float piece = 0.0f;
+      float piece = 0.0f, squares = 0.0f;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        v[j][i] = !END || col(j) + i < a.dim ? v[j][i] - mean : 0.0f;
-        piece += v[j][i] * v[j][i];
+        v[j][i] = !END || col(j) + i < a.dim ? v[j][i] - near : 0.0f;
+        piece += v[j][i];
+        squares += v[j][i] * v[j][i];
       }
-      q += in(j) ? piece : 0.0f;
+      d += in(j) ? piece : 0.0f;
+      q += in(j) ? squares : 0.0f;
     }
-    const float rstd = 1.0f / sqrtf(row_sum<WPR>(q, lds[1]) * a.inv_dim + a.eps);
+    const float2 sums = row_sum2<WPR>(d, q, lds2);
+    const float c = sums.x * a.inv_dim, mean = near + c, rstd = rstd_of(c, sums.y * a.inv_dim, a.eps);
     T* out = static_cast<T*>(a.out) + row * a.ostride;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (END && !in(j)) continue;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = v[j][i] * rstd * w[j][i] + b[j][i];
+      for (int i = 0; i < VEC; ++i) v[j][i] = (v[j][i] - c) * rstd * w[j][i] + b[j][i];
       stream_some<T, VEC>(out + at(j), have<VEC, END>(a.dim, at(j)), v[j]);
     }
     if (WPR == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) {
@@ -329,26 +368,29 @@ constexpr int kAnyWaves = 16;
 
 template <class T, class P>
 __global__ __launch_bounds__(64 * kAnyWaves) void k_norm_any(NormArgs a) {
-  __shared__ float lds[2][kAnyWaves];
+  __shared__ float lds[kAnyWaves];
+  __shared__ float2 lds2[kAnyWaves];
   for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.xstride;
     T* out = static_cast<T*>(a.out) + row * a.ostride;
     float s = 0.0f;
     for (uint32_t c = threadIdx.x; c < a.dim; c += 64 * kAnyWaves) s += static_cast<float>(x[c]);
-    const float mean = row_sum<kAnyWaves>(s, lds[0]) * a.inv_dim;
-    float q = 0.0f;
+    const float near = estimate(row_sum<kAnyWaves>(s, lds), a.inv_dim);
+    float d = 0.0f, q = 0.0f;
     for (uint32_t c = threadIdx.x; c < a.dim; c += 64 * kAnyWaves) {
-      const float d = static_cast<float>(x[c]) - mean;
-      q += d * d;
+      const float v = static_cast<float>(x[c]) - near;
+      d += v;
+      q += v * v;
     }
-    const float rstd = 1.0f / sqrtf(row_sum<kAnyWaves>(q, lds[1]) * a.inv_dim + a.eps);
+    const float2 sums = row_sum2<kAnyWaves>(d, q, lds2);
+    const float off = sums.x * a.inv_dim, rstd = rstd_of(off, sums.y * a.inv_dim, a.eps);
     for (uint32_t c = threadIdx.x; c < a.dim; c += 64 * kAnyWaves) {
       const float w = a.w != nullptr ? static_cast<float>(static_cast<const P*>(a.w)[c]) : 1.0f;
       const float b = a.b != nullptr ? static_cast<float>(static_cast<const P*>(a.b)[c]) : 0.0f;
-      out[c] = static_cast<T>((static_cast<float>(x[c]) - mean) * rstd * w + b);
+      out[c] = static_cast<T>((static_cast<float>(x[c]) - near - off) * rstd * w + b);
     }
     if (threadIdx.x == 0) {
-      a.mean[row] = mean;
+      a.mean[row] = near + off;
       a.rstd[row] = rstd;
     }
   }

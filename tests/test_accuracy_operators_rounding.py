@@ -1,12 +1,12 @@
 """Where 16-bit storage or a large mean could cost the operators more than their outputs' own rounding: what is held of the
-loss's gradient for the targets, and tokens of very unequal factors.
+loss's gradient for the targets, tokens of very unequal factors, and rows far from zero.
 
 Tolerances are worst-case rounding bounds, as in test_accuracy_operators.py."""
 import pytest
 import torch
 
 from omr import ops
-from test_accuracy_operators import BF16, F16, U, gen, half, rand, tiny, within
+from test_accuracy_operators import BF16, F16, F32, TYPES, U, depth, gen, half, rand, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,30 @@ def test_tokens_of_small_factors_count(gpu, T, D, dtype):
     check_gradients(plan, (h.float() * 1e-3).to(dtype), w, t, up, dtype, torch.empty(V, D, device="cuda"))
     check_gradients(plan, (h.float() * 300).to(dtype), (w.float() / 300).to(dtype), t, up, dtype,
                     torch.empty(V, D, device="cuda"))
+
+
+@pytest.mark.parametrize("rows,dim", [(3, 1000), (5, 777), (2, 61), (1, 4095), (2, 4104), (2, 16384), (2, 20001), (700, 1000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_norm_far_from_zero(gpu, rows, dim, dtype):
+    """A large mean costs nothing: it is found to k u of the distances from the first estimate, which itself is off by m = k u
+    mean|x|.  So with b = max|x - mean| + m the output is off by (k + 4) u b rstd, and by rstd's own error, whatever the
+    mean is; rows of one value give zeros."""
+    g = gen(rows + dim)
+    k = depth(dim) + 2
+    eps = torch.tensor(1e-5, dtype=F32).item()
+    for mean, std in ((10000.1, 0.0), (1000.3, 0.0), (-10000.1, 1.0), (1e6, 30.0), (300.0, 0.01)):
+        x = rand((rows, dim), F32, g, std=std, mean=mean).clamp_(-6e4, 6e4).to(dtype)
+        r = ops.layer_norm(x)
+        xd = x.double()
+        mu = xd.mean(1, keepdim=True)
+        var = (xd - mu).square().mean(1, keepdim=True)
+        rstd = 1 / torch.sqrt(var + eps)
+        y = (xd - mu) * rstd
+        m = k * U * xd.abs().mean(1, keepdim=True)
+        b = (xd - mu).abs().amax(1, keepdim=True) + m
+        # the squares' sum is off by (k + 4) u of itself, it and the square taken off it are at most var + m^2, m^2
+        rel = ((k + 6) * U * (var + 2 * m * m) + 2 * (k + 4) * U * b * m) / (var + eps) / 2 + 6 * U
+        within(r.rstd, rstd[:, 0], (rel * rstd)[:, 0], ("rstd", mean, std))
+        within(r.mean, mu[:, 0], (k * U * b + U * mu.abs())[:, 0], ("mean", mean, std))
+        tol = (k + 4) * U * b * rstd * (1 + rel) + y.abs() * rel + 2 * U * y.abs()
+        within(r.out, y, tol * (1 + half(dtype)) + half(dtype) * y.abs() + tiny(dtype), ("out", mean, std))
