@@ -1043,14 +1043,19 @@ int tile_of(uint64_t m, uint64_t n, uint64_t splits) {
 }
 uint32_t tile_rows(int tile) { return tile == kTileBig ? kBig : tile == kTileTiny ? kTiny : kSmall; }
 
+// A launch holds fewer than 2^32 threads.  The calls look at all of theirs before the first.
+constexpr uint64_t kMaxTiles = 1u << 22, kMaxBlocks = (1u << 24) - 1;
+bool tiles_fit(uint64_t m, uint64_t n, uint64_t splits) {
+  const uint32_t t = tile_rows(tile_of(m, n, splits));
+  return ceil_div(m, t) * ceil_div(n, t) * splits < kMaxTiles;
+}
+
 template <class T, int EPI>
 int launch(GemmArgs<T>& a, uint32_t m, uint32_t n, int tile, hipStream_t stream) {
   const uint32_t t = tile_rows(tile);
   a.mt = static_cast<uint32_t>(ceil_div(m, t));
   a.nt = static_cast<uint32_t>(ceil_div(n, t));
-  const uint64_t grid = static_cast<uint64_t>(a.mt) * a.nt * a.splits;
-  if (grid >= (1u << 22)) return efail("vocab_loss: too many tiles for one call");
-  const unsigned g = static_cast<unsigned>(grid);
+  const unsigned g = a.mt * a.nt * a.splits;
   switch (tile) {
     case kTileBig: k_gemm<T, EPI, 256, 256, 2, 4, 2><<<g, 512, 0, stream>>>(a); break;
     case kTileSmall: k_gemm<T, EPI, 128, 128, 2, 2, 2><<<g, 256, 0, stream>>>(a); break;
@@ -1165,35 +1170,43 @@ uint32_t lanes_log(uint32_t pdim) {  // lanes that a row of pdim elements fills,
   return l;
 }
 
+// which of weight and hidden are laid out again, and by how many workgroups
+struct Pack {
+  bool w, h;
+  uint64_t blocks;
+};
+Pack pack_of(const void* hidden, uint64_t hstride, const void* weight, uint64_t wstride, uint64_t tokens, uint64_t vocab,
+             uint32_t dim) {
+  Pack p{dim % 8 != 0 || !rows_ok(weight, wstride), dim % 8 != 0 || !rows_ok(hidden, hstride), 0};
+  p.blocks = ceil_div((p.w ? vocab : 0) + (p.h ? tokens : 0), 256u >> lanes_log(static_cast<uint32_t>(up(dim, 8))));
+  return p;
+}
+
 // hidden and weight as row operands of whole 16-byte pieces: the caller's, or copies in the workspace
 template <class T>
 int operands(const void* hidden, uint64_t hstride, const void* weight, uint64_t wstride, uint64_t tokens, uint64_t vocab,
-             uint32_t dim, const Space& sp, char* ws, Operand<T>* h, Operand<T>* w, hipStream_t stream) {
+             uint32_t dim, const Pack& pack, const Space& sp, char* ws, Operand<T>* h, Operand<T>* w, hipStream_t stream) {
   const uint32_t pdim = static_cast<uint32_t>(up(dim, 8)), lpr_log = lanes_log(pdim);
   *h = {static_cast<const T*>(hidden), hstride, static_cast<uint32_t>(tokens)};
   *w = {static_cast<const T*>(weight), wstride, static_cast<uint32_t>(vocab)};
   PackArgs<T> x{w->p, wstride, 0, reinterpret_cast<T*>(ws + sp.w)}, y{h->p, hstride, 0, reinterpret_cast<T*>(ws + sp.h)};
-  if (dim % 8 != 0 || !rows_ok(weight, wstride)) {
+  if (pack.w) {
     x.rows = vocab;
     w->p = x.dst;
     w->ld = pdim;
   }
-  if (dim % 8 != 0 || !rows_ok(hidden, hstride)) {
+  if (pack.h) {
     y.rows = tokens;
     h->p = y.dst;
     h->ld = pdim;
   }
-  if (x.rows + y.rows == 0) return 0;
-  const uint64_t blocks = ceil_div(x.rows + y.rows, 256u >> lpr_log);
-  if (blocks >= (1u << 24)) return efail("vocab_loss: too many rows to lay out in one call");
-  k_pack<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(x, y, dim, pdim, lpr_log);
+  if (pack.blocks == 0) return 0;
+  k_pack<T><<<static_cast<unsigned>(pack.blocks), 256, 0, stream>>>(x, y, dim, pdim, lpr_log);
   return elaunch("omr_vocab_loss (layout)");
 }
 
-int check_space(const char* what, const void* hidden, uint64_t hstride, const void* weight, uint64_t wstride,
-                uint64_t tokens, uint64_t vocab, uint32_t dim, bool grads, const void* workspace, size_t bytes,
-                Space* sp) {
-  const bool pack = dim % 8 != 0 || !rows_ok(hidden, hstride) || !rows_ok(weight, wstride);
+int check_space(const char* what, bool pack, uint64_t tokens, uint64_t vocab, uint32_t dim, bool grads,
+                const void* workspace, size_t bytes, Space* sp) {
   *sp = layout(tokens, vocab, dim, pack, grads);
   if (workspace == nullptr || !aligned(workspace, 16)) return efail("%s: the workspace must be 16-byte aligned", what);
   if (bytes < sp->bytes)
@@ -1218,15 +1231,19 @@ int omr_vocab_loss(const void* hidden, uint64_t hidden_stride, const void* weigh
   if (hidden == nullptr || weight == nullptr || targets == nullptr || loss == nullptr || lse == nullptr)
     return efail("vocab_loss: NULL pointer");
   Space sp;
-  if (const int rc = check_space("vocab_loss", hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, false,
-                                 workspace, workspace_bytes, &sp))
+  const Pack pack = pack_of(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim);
+  if (const int rc = check_space("vocab_loss", pack.w || pack.h, tokens, vocab, dim, false, workspace, workspace_bytes, &sp))
     return rc;
+  const bool few = tokens <= kFewTokens;
+  if (pack.blocks > kMaxBlocks || (few ? ceil_div(vocab, 64) > kMaxBlocks : !tiles_fit(vocab, tokens, 1)) ||
+      ceil_div(tokens, 4) > kMaxBlocks)
+    return efail("vocab_loss: too many tokens or rows for one call");
   char* ws = static_cast<char*>(workspace);
   auto go = [&](auto t) {
     using T = decltype(t);
     GemmArgs<T> a{};
-    if (const int rc = operands<T>(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, sp, ws, &a.b, &a.a,
-                                   S(stream)))
+    if (const int rc = operands<T>(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, pack, sp, ws, &a.b,
+                                   &a.a, S(stream)))
       return rc;
     const int tile = tile_of(vocab, tokens, 1);
     a.k = dim;
@@ -1238,14 +1255,12 @@ int omr_vocab_loss(const void* hidden, uint64_t hidden_stride, const void* weigh
     a.tokens = static_cast<uint32_t>(tokens);
     a.ztarget = reinterpret_cast<float*>(ws + sp.rest);
     a.stats = reinterpret_cast<float*>(ws + sp.rest + up(tokens * 4, 256));
-    if (tokens <= kFewTokens) {
+    if (few) {
       a.pieces = static_cast<uint32_t>(ceil_div(vocab, 64));
-      const unsigned grid = a.pieces;
-      if (grid > (1u << 24) - 1) return efail("vocab_loss: too many tiles for one call");
       if (tokens <= 16)
-        k_few<T, 1><<<grid, 256, 0, S(stream)>>>(a);
+        k_few<T, 1><<<a.pieces, 256, 0, S(stream)>>>(a);
       else
-        k_few<T, 2><<<grid, 256, 0, S(stream)>>>(a);
+        k_few<T, 2><<<a.pieces, 256, 0, S(stream)>>>(a);
       if (const int rc = elaunch("omr_vocab_loss")) return rc;
     } else {
       a.pieces = static_cast<uint32_t>(ceil_div(vocab, tile_rows(tile)) * 2);  // two waves' parts a tile
@@ -1287,15 +1302,30 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     return elaunch("omr_vocab_loss_grad");
   }
   Space sp;
-  if (const int rc = check_space("vocab_loss_grad", hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim,
-                                 true, workspace, workspace_bytes, &sp))
+  const Pack pack = pack_of(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim);
+  if (const int rc = check_space("vocab_loss_grad", pack.w || pack.h, tokens, vocab, dim, true, workspace, workspace_bytes,
+                                 &sp))
     return rc;
+  const uint32_t pdim = static_cast<uint32_t>(up(dim, 8)), piece = piece_rows(tokens, vocab);
+  const uint32_t whole = static_cast<uint32_t>(std::min<uint64_t>(piece, vocab));  // rows of a piece but the last
+  const uint32_t first_cols = static_cast<uint32_t>(up(whole, 256));
+  // (a piece's columns of G that are written: zeros behind the vocabulary)
+  const uint32_t ksplit = static_cast<uint32_t>(up(ceil_div(whole, hidden_splits(tokens, dim, piece)), kBK));
+  const uint32_t splits = static_cast<uint32_t>(ceil_div(whole, ksplit));  // of a whole piece; the last may have fewer
+  const bool beside = tokens <= kFindHere && tile_of(first_cols, tokens, 1) != kTileBig;
+  // (beside the product few sorters: they hold places of its tiles)
+  const uint32_t lpr_log = lanes_log(pdim), sort_rows = beside ? SortSpace<4>::kRange : sort_range(static_cast<uint32_t>(vocab));
+  const uint64_t sorters = ceil_div(vocab, sort_rows),
+                 prepare_blocks = sorters + ceil_div(tokens, (beside ? 256u : 1024u) >> lpr_log);
+  if (pack.blocks > kMaxBlocks || !tiles_fit(first_cols, tokens, 1) ||
+      (grad_hidden != nullptr && !tiles_fit(dim, tokens, splits)) ||
+      (grad_weight != nullptr && (!tiles_fit(dim, first_cols, 1) || prepare_blocks >= kMaxTiles)))
+    return efail("vocab_loss_grad: too many tokens or rows for one call");
   char* ws = static_cast<char*>(workspace);
   auto go = [&](auto t) {
     using T = decltype(t);
-    const uint32_t pdim = static_cast<uint32_t>(up(dim, 8));
     Operand<T> h, w;
-    if (const int rc = operands<T>(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, sp, ws, &h, &w,
+    if (const int rc = operands<T>(hidden, hidden_stride, weight, weight_stride, tokens, vocab, dim, pack, sp, ws, &h, &w,
                                    S(stream)))
       return rc;
     uint64_t at = sp.rest;
@@ -1321,20 +1351,12 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     a.up = grad_loss;
     a.upstride = grad_loss_stride;
     a.amax = amax;
-    const uint32_t piece = piece_rows(tokens, vocab);
-    const uint32_t first_cols = static_cast<uint32_t>(up(std::min<uint64_t>(piece, vocab), 256));
-    // (a piece's columns of G that are written: zeros behind the vocabulary)
-    const bool beside = tokens <= kFindHere && tile_of(first_cols, tokens, 1) != kTileBig;
     PrepareArgs<T> p{};
     if (grad_weight != nullptr) {
-      const uint32_t threads = beside ? 256 : 1024;
-      p.lpr_log = lanes_log(pdim);
-      // (beside the product few sorters: they hold places of its tiles)
-      p.range = beside ? SortSpace<4>::kRange : sort_range(a.vocab);
-      p.sorters = static_cast<uint32_t>(ceil_div(vocab, p.range));
-      const uint64_t blocks = p.sorters + ceil_div(tokens, threads >> p.lpr_log);
-      if (blocks >= (1u << 22)) return efail("vocab_loss_grad: too many tokens or rows for one call");
-      p.blocks = static_cast<uint32_t>(blocks);
+      p.lpr_log = lpr_log;
+      p.range = sort_rows;
+      p.sorters = static_cast<uint32_t>(sorters);
+      p.blocks = static_cast<uint32_t>(prepare_blocks);
       p.start = start;
       p.perm = perm;
       p.src = static_cast<const T*>(hidden);
@@ -1368,9 +1390,6 @@ int omr_vocab_loss_grad(const void* hidden, uint64_t hidden_stride, const void* 
     a.w = w;
     a.start = start;
     a.perm = perm;
-    const uint32_t whole = static_cast<uint32_t>(std::min<uint64_t>(piece, vocab));
-    const uint32_t ksplit = static_cast<uint32_t>(up(ceil_div(whole, hidden_splits(tokens, dim, piece)), kBK));
-    const uint32_t splits = static_cast<uint32_t>(ceil_div(whole, ksplit));  // of a whole piece; the last may have fewer
     for (uint64_t v0 = 0; v0 < vocab; v0 += piece) {
       const uint32_t rows = static_cast<uint32_t>(std::min<uint64_t>(piece, vocab - v0));
       const uint32_t cols = static_cast<uint32_t>(up(rows, 256));

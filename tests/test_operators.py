@@ -123,3 +123,20 @@ def test_the_front_end_refuses():
                  lambda: ops.VocabLossPlan(4, 10, 1 << 40)):
         with pytest.raises(ValueError, match="sizes"):
             make()
+
+
+@pytest.mark.parametrize("call,arg", [
+    (loss, dict(n=1 << 25, vocab=1 << 20)),                      # 2^17 x 2^12 tiles
+    (loss, dict(n=1 << 25, vocab=1 << 20, wstride=9)),           # and rows to be laid out first
+    (loss, dict(vocab=(1 << 31) - 300)),                         # a few tokens, 2^25 workgroups
+    (loss, dict(n=4, vocab=(1 << 31) - 300, wstride=9)),
+    (loss, dict(n=(1 << 26) - 2, vocab=10)),                     # 2^24 workgroups that join
+    (loss_grad, dict(n=1 << 25, dim=1 << 20, hs=1 << 20, wstride=1 << 20, ghs=1 << 20, gws=1 << 20)),  # grad_hidden's tiles
+    (loss_grad, dict(n=1 << 25, dim=1 << 20, hs=1 << 20, wstride=1 << 20, ghs=1 << 20, gw=None)),
+    (loss_grad, dict(vocab=(1 << 31) - 300, dim=1001, hs=1001, wstride=1001, ghs=1001, gws=1001)),  # 2^29 that lay out rows
+    (loss_grad, dict(n=(1 << 26) - 1, vocab=1 << 29, dim=1 << 10, hs=1 << 10, wstride=1 << 10, ghs=1 << 10, gws=1 << 10)),
+])
+def test_sizes_no_launch_takes_are_refused_first(call, arg):
+    """Before anything is launched, the laying out of rows and the sort among it: without a GPU a launch would say that there
+    is none."""
+    refused(call(**{"bytes": 1 << 62, **arg}), "too many")
