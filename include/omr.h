@@ -452,6 +452,7 @@ int omr_msg_unpack_f32(const float* replies, const uint32_t* reply_imm, const vo
  *     whole 16-byte pieces run fastest;
  *   - a row is at most OMR_MAX_DIM elements;
  *   - every sum has a fixed order: the same inputs give the same bits;
+ *   - a workspace's size is 0 where no call takes such sizes;
  *   - a workspace holds nothing from one call to the next and needs no initial value; calls that may run at the same
  *     time (two streams, two captured graphs that are replayed side by side) need one each;
  *   - outputs must not overlap inputs or each other unless a comment says so. */

@@ -270,6 +270,7 @@ int omr_embed(const void* table, int table_dtype, uint64_t num_rows, uint32_t di
 }
 
 size_t omr_embed_grad_workspace_bytes(uint64_t num_ids, uint64_t num_rows, uint32_t dim) {
+  if (dim == 0 || dim > OMR_MAX_DIM || num_rows >= (1ull << 31) || num_ids >= (1ull << 31)) return 0;
   const uint64_t chunks = num_ids != 0 ? ceil_div(num_ids, kChunk) : 0;
   return round16(4 * (num_rows + 1)) + 2 * round16(4 * num_ids) + 2 * chunks * round16(4ull * dim);
 }

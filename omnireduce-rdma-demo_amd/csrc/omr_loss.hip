@@ -1156,11 +1156,14 @@ Space layout(uint64_t tokens, uint64_t vocab, uint64_t dim, bool pack, bool grad
 
 bool rows_ok(const void* p, uint64_t stride) { return aligned(p, 16) && stride % 8 == 0 && stride < kMaxStride; }
 
+constexpr uint32_t kMaxDim = 1u << 20;
+constexpr uint64_t kMaxVocab = (1ull << 31) - 257, kMaxTokens = (1ull << 26) - 1;
+
 int check(const char* what, int dtype, uint64_t tokens, uint64_t vocab, uint32_t dim) {
   if (dtype != OMR_BF16 && dtype != OMR_F16) return efail("%s: hidden and weight are bf16 or fp16", what);
-  if (dim == 0 || dim > (1u << 20)) return efail("%s: dim must be 1..%u", what, 1u << 20);
-  if (vocab == 0 || vocab >= (1ull << 31) - 256) return efail("%s: vocab must be 1..2^31 - 257", what);
-  if (tokens >= (1ull << 26)) return efail("%s: tokens must be below 2^26", what);
+  if (dim == 0 || dim > kMaxDim) return efail("%s: dim must be 1..%u", what, kMaxDim);
+  if (vocab == 0 || vocab > kMaxVocab) return efail("%s: vocab must be 1..2^31 - 257", what);
+  if (tokens > kMaxTokens) return efail("%s: tokens must be below 2^26", what);
   return 0;
 }
 
@@ -1220,6 +1223,7 @@ int check_space(const char* what, bool pack, uint64_t tokens, uint64_t vocab, ui
 extern "C" {
 
 size_t omr_vocab_loss_workspace_bytes(uint64_t max_tokens, uint64_t vocab, uint32_t dim, int pack, int grads) {
+  if (dim == 0 || dim > kMaxDim || vocab == 0 || vocab > kMaxVocab || max_tokens > kMaxTokens) return 0;
   return layout(max_tokens, vocab, dim, pack || dim % 8 != 0, grads).bytes;
 }
 

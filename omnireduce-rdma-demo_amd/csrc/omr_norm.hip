@@ -504,11 +504,13 @@ int with_shape(bool end, int wpr, F&& fn) {
   }
 }
 
+constexpr uint64_t kMaxRows = 1ull << 40;
+
 int check_args(const char* what, int dtype, int param_dtype, uint64_t rows, uint32_t dim) {
   if (!dtype_ok(dtype) || (param_dtype != OMR_F32 && param_dtype != dtype))
     return efail("%s: elements are fp32, bf16 or fp16, and parameters fp32 or of the elements' type", what);
   if (dim == 0 || dim > OMR_MAX_DIM) return efail("%s: dim must be 1..%u", what, OMR_MAX_DIM);
-  if (rows >= (1ull << 40)) return efail("%s: too many rows", what);
+  if (rows >= kMaxRows) return efail("%s: too many rows", what);
   return 0;
 }
 
@@ -561,6 +563,7 @@ int omr_layer_norm(const void* x, int dtype, uint64_t rows, uint32_t dim, uint64
 }
 
 size_t omr_layer_norm_grad_workspace_bytes(uint64_t rows, uint32_t dim) {
+  if (dim == 0 || dim > OMR_MAX_DIM || rows >= kMaxRows) return 0;
   return static_cast<size_t>(grad_blocks(rows, dim, true)) * 2 * dim * sizeof(float) + 16;
 }
 

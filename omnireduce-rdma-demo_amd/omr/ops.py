@@ -398,8 +398,10 @@ class _Workspace:
     """Device memory of a plan: allocated once, lent to one call at a time."""
 
     def __init__(self, nbytes: int, device):
+        if nbytes == 0:
+            raise ValueError("no call takes such sizes: too many tokens or rows, or rows too long")
         self.bytes = nbytes
-        self.tensor = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+        self.tensor = torch.empty(nbytes, dtype=torch.uint8, device=device)
         self.device = self.tensor.device
         self.ptr = self.tensor.data_ptr()
         self._home = torch.cuda.current_stream(self.device).cuda_stream

@@ -140,3 +140,28 @@ def test_sizes_no_launch_takes_are_refused_first(call, arg):
     """Before anything is launched, the laying out of rows and the sort among it: without a GPU a launch would say that there
     is none."""
     refused(call(**{"bytes": 1 << 62, **arg}), "too many")
+
+
+def test_workspaces_of_sizes_no_call_takes():
+    """Are 0 bytes, and no plan is made for them: their products would pass 64 bits (2^40 tokens of 2^24), and a plan's first
+    call would be refused."""
+    lib = _lib.load()
+    for size in (lib.omr_vocab_loss_workspace_bytes(1 << 26, 100, 64, 0, 1),
+                 lib.omr_vocab_loss_workspace_bytes(1 << 39, 100, 1 << 24, 0, 1),
+                 lib.omr_vocab_loss_workspace_bytes(10, 100, (1 << 20) + 1, 0, 1),
+                 lib.omr_vocab_loss_workspace_bytes(10, (1 << 31) - 256, 64, 0, 1),
+                 lib.omr_vocab_loss_workspace_bytes(10, 0, 64, 0, 1), lib.omr_vocab_loss_workspace_bytes(10, 9, 0, 0, 1),
+                 lib.omr_embed_grad_workspace_bytes(1 << 31, 10, 8), lib.omr_embed_grad_workspace_bytes(10, 1 << 31, 8),
+                 lib.omr_embed_grad_workspace_bytes(10, 10, (1 << 24) + 1), lib.omr_embed_grad_workspace_bytes(10, 10, 0),
+                 lib.omr_layer_norm_grad_workspace_bytes(1 << 40, 8), lib.omr_layer_norm_grad_workspace_bytes(8, 0),
+                 lib.omr_layer_norm_grad_workspace_bytes(8, (1 << 24) + 1)):
+        assert size == 0
+    for least in (lib.omr_vocab_loss_workspace_bytes(0, 1, 1, 0, 0), lib.omr_embed_grad_workspace_bytes(0, 0, 1),
+                  lib.omr_layer_norm_grad_workspace_bytes(0, 1)):
+        assert least >= 16
+    for make in (lambda: ops.VocabLossPlan(1 << 26, 100, 64, device="cpu"),
+                 lambda: ops.VocabLossPlan(1 << 39, 100, 1 << 24, device="cpu"),
+                 lambda: ops.VocabLossPlan(4, 10, (1 << 20) + 8, device="cpu"),
+                 lambda: ops.EmbedGradPlan(1 << 31, 10, 8, device="cpu")):
+        with pytest.raises(ValueError, match="sizes"):
+            make()
