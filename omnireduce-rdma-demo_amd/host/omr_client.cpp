@@ -649,10 +649,11 @@ int main(int argc, char* argv[]) {
       case 'C': o.colocated = true; break;
       case 'H': o.host = true; break;
       case 'E': {
-        char* end = nullptr;
-        o.dim = static_cast<uint32_t>(strtoul(optarg, &end, 0));
-        o.tokens = *end == ':' ? strtoull(end + 1, nullptr, 0) : 0;
-        if (o.dim == 0 || o.tokens == 0) {
+        char *end = nullptr, *last = nullptr;
+        const unsigned long long dim = strtoull(optarg, &end, 0);
+        o.tokens = *end == ':' ? strtoull(end + 1, &last, 0) : 0;
+        o.dim = dim < 1ull << 32 ? static_cast<uint32_t>(dim) : 0;  // (below: what the operators take)
+        if (o.dim == 0 || o.tokens == 0 || *last != 0) {
           fprintf(stderr, "-E needs <dim>:<tokens>\n");
           usage(argv[0]);
           return 1;
@@ -667,8 +668,9 @@ int main(int argc, char* argv[]) {
     usage(argv[0]);
     return 1;
   }
-  if (o.dim != 0 && (o.dim % 8 != 0 || o.n % o.dim != 0 || o.tokens >= 1u << 30)) {
-    fprintf(stderr, "-E: dim must be a multiple of 8 that divides -n, and tokens below 2^30\n");
+  if (o.dim != 0 && (o.dim % 8 != 0 || o.n % o.dim != 0 ||
+                     omr_vocab_loss_workspace_bytes(o.tokens, o.n / o.dim, o.dim, 0, 1) == 0)) {
+    fprintf(stderr, "-E: dim must be a multiple of 8 that divides -n, at most 2^20, and tokens below 2^26\n");
     return 1;
   }
   int ndev = 0;

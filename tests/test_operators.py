@@ -1,6 +1,7 @@
 """The operators that make the gradient, without a GPU: what they refuse (before anything is launched), and the sizes of
 their workspaces."""
-import ctypes
+import os
+import subprocess
 
 import pytest
 import torch
@@ -165,3 +166,14 @@ def test_workspaces_of_sizes_no_call_takes():
                  lambda: ops.EmbedGradPlan(1 << 31, 10, 8, device="cpu")):
         with pytest.raises(ValueError, match="sizes"):
             make()
+
+
+@pytest.mark.parametrize("value", ["4294967304:5", "8:5x", "8x:5", "-8:5", "8:-5", "8:", ":5", "8", "", "0:5", "8:0",
+                                   "8:18446744073709551617", "12:5", "56:5", "8:1073741824", "1048584:5"])
+def test_the_client_refuses_sizes(value):
+    """./omr_client -E <dim>:<tokens>, before it looks for a device: numbers that are not two of their range, or no
+    multiple of 8 that divides the tensor."""
+    exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "omnireduce-rdma-demo_amd", "bin",
+                       "omr_client")
+    p = subprocess.run([exe, "-L", "1", "-n", str(1048584 << 4), "-E", value], capture_output=True, text=True, timeout=60)
+    assert p.returncode == 1 and "-E" in p.stderr and "device" not in p.stderr, p.stderr
