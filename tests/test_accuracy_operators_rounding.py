@@ -1,12 +1,12 @@
 """Where 16-bit storage or a large mean could cost the operators more than their outputs' own rounding: what is held of the
-loss's gradient for the targets, tokens of very unequal factors, and rows far from zero.
+loss's gradient for the targets, tokens of very unequal factors, rows far from zero, and the largest tiles.
 
 Tolerances are worst-case rounding bounds, as in test_accuracy_operators.py."""
 import pytest
 import torch
 
 from omr import ops
-from test_accuracy_operators import BF16, F16, F32, TYPES, U, depth, gen, half, rand, tiny, within
+from test_accuracy_operators import BF16, F16, F32, TYPES, U, depth, gen, half, loss_inputs, rand, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -99,6 +99,20 @@ def test_tokens_of_small_factors_count(gpu, T, D, dtype):
     check_gradients(plan, (h.float() * 1e-3).to(dtype), w, t, up, dtype, torch.empty(V, D, device="cuda"))
     check_gradients(plan, (h.float() * 300).to(dtype), (w.float() / 300).to(dtype), t, up, dtype,
                     torch.empty(V, D, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_large_tiles_of_both_products(gpu, dtype):
+    """Sizes whose grad_hidden and grad_weight both have a tile of 256 x 256 a CU, with two pieces of the vocabulary, the
+    last of them ragged, and every size ragged for the tiles."""
+    T, V, D = 8200, 20003, 2056
+    g = gen(77)
+    h, w, t, off = loss_inputs(T, V, D, dtype, g)
+    t[::3] = torch.where(off[::3], t[::3], targets_of(t[::3].numel(), V, g, "words"))
+    plan = ops.VocabLossPlan(T, V, D, dtype=dtype)
+    up = rand((T,), F32, g)
+    check_gradients(plan, h, w, t, up, dtype, None)
+    check_gradients(plan, h, w, t, up, dtype, torch.empty(V, D, device="cuda"))
 
 
 @pytest.mark.parametrize("rows,dim", [(3, 1000), (5, 777), (2, 61), (1, 4095), (2, 4104), (2, 16384), (2, 20001), (700, 1000)])
