@@ -56,23 +56,32 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
   return v;
 }
 
-// Two such sums behind one barrier.
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+// Two such sums behind one barrier, and for the exchanges of one: behind the first, lanes 0..31 carry v's and 32..63 q's.
+// (16384 x 2048 bf16 read from the last-level cache: 23.5 us, 24.0 with 12 exchanges, 22.4 without the distances' sum, which
+// is hidden where rows come from HBM.)
 template <int WPR>
 __device__ __forceinline__ float2 row_sum2(float v, float q, float2* lds) {
-  v = wave_sum(v);
-  q = wave_sum(q);
-  if constexpr (WPR > 1) {
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = make_float2(v, q);
+  const uint32_t lane = threadIdx.x & 63;
+  float s = (lane < 32 ? v : q) + __shfl_xor(lane < 32 ? q : v, 32);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) s += __shfl_xor(s, d);
+  if constexpr (WPR == 1) {
+    return make_float2(lane_of(s, 0), lane_of(s, 32));
+  } else {
+    if (lane % 32 == 0) reinterpret_cast<float*>(lds)[2 * (threadIdx.x >> 6) + lane / 32] = s;
     __syncthreads();
-    v = lds[0].x;
-    q = lds[0].y;
+    float2 sums = lds[0];
 #pragma unroll
     for (int w = 1; w < WPR; ++w) {
-      v += lds[w].x;
-      q += lds[w].y;
+      sums.x += lds[w].x;
+      sums.y += lds[w].y;
     }
+    return sums;
   }
-  return make_float2(v, q);
 }
 
 // The mean's first estimate, rounded: one value for the distances and for what their mean is added to (a product joined to
@@ -187,13 +196,13 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void k_norm(NormArgs a) 
       q += in(j) ? squares : 0.0f;
     }
     const float2 sums = row_sum2<WPR>(d, q, lds2);
-    const float c = sums.x * a.inv_dim, mean = near + c, rstd = rstd_of(c, sums.y * a.inv_dim, a.eps);
+    const float c = sums.x * a.inv_dim, mean = near + c, rstd = rstd_of(c, sums.y * a.inv_dim, a.eps), shift = -c * rstd;
     T* out = static_cast<T*>(a.out) + row * a.ostride;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (END && !in(j)) continue;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = (v[j][i] - c) * rstd * w[j][i] + b[j][i];
+      for (int i = 0; i < VEC; ++i) v[j][i] = __builtin_fmaf(v[j][i], rstd, shift) * w[j][i] + b[j][i];
       stream_some<T, VEC>(out + at(j), have<VEC, END>(a.dim, at(j)), v[j]);
     }
     if (WPR == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) {
