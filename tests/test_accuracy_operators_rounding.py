@@ -140,3 +140,79 @@ def test_layer_norm_far_from_zero(gpu, rows, dim, dtype):
         within(r.mean, mu[:, 0], (k * U * b + U * mu.abs())[:, 0], ("mean", mean, std))
         tol = (k + 4) * U * b * rstd * (1 + rel) + y.abs() * rel + 2 * U * y.abs()
         within(r.out, y, tol * (1 + half(dtype)) + half(dtype) * y.abs() + tiny(dtype), ("out", mean, std))
+
+
+def test_captured_backward_of_unequal_factors(gpu):
+    """The fp16 loss with a factor for each token, captured: every replay, on new inputs and with eager work between, gives
+    the eager bits."""
+    T, V, D = 300, 900, 136
+    g = gen(41)
+    h, w, t, _ = loss_inputs(T, V, D, F16, g)
+    up = rand((T,), F32, g)
+    eager, plan = ops.VocabLossPlan(T, V, D, dtype=F16), ops.VocabLossPlan(T, V, D, dtype=F16)
+    gw = torch.empty(V, D, device="cuda")
+
+    def run(p, gw):
+        loss, lse = p.forward(h, w, t)
+        return [loss, lse, *p.backward(h, w, t, lse, up, grad_weight=gw)]
+
+    run(plan, gw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(plan, gw)
+    for k in range(4):
+        for old, new in zip((h, w, t), loss_inputs(T, V, D, F16, gen(50 + k))):
+            old.copy_(new)
+        up.copy_(rand((T,), F32, gen(60 + k)) * 10.0 ** -k)
+        want = run(eager, torch.empty(V, D, device="cuda"))
+        gw.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_backward_of_expanded_rows(gpu, dtype):
+    """One hidden state for all tokens, or one row for the whole vocabulary: a stride of 0, the same bits."""
+    T, V, D = 70, 300, 64
+    g = gen(42)
+    h, w, t, _ = loss_inputs(T, V, D, dtype, g)
+    up = rand((T,), F32, g)
+    plan = ops.VocabLossPlan(T, V, D, dtype=dtype)
+    for hh, ww in ((h[:1].expand(T, D), w), (h, w[:1].expand(V, D))):
+        _, lse = plan.forward(hh, ww, t)
+        a = plan.backward(hh, ww, t, lse, up, torch.empty_like(h), torch.empty_like(w))
+        b = plan.backward(hh.contiguous(), ww.contiguous(), t, lse, up)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_backward_without_given_outputs_of_expanded_rows(gpu):
+    """What is not given is allocated with rows of its own."""
+    h, w, t, _ = loss_inputs(20, 30, 64, BF16, gen(43))
+    plan = ops.VocabLossPlan(20, 30, 64)
+    _, lse = plan.forward(h[:1].expand(20, 64), w, t)
+    gh, gw = plan.backward(h[:1].expand(20, 64), w, t, lse, torch.ones(20, device="cuda"))
+    assert gh.stride() == (64, 1) and gw.stride() == (64, 1)
+
+
+def test_calls_on_two_streams(gpu):
+    """Two losses at once, a plan each."""
+    T, V, D = 260, 4000, 264
+    sets = [loss_inputs(T, V, D, F16, gen(70 + k)) for k in range(2)]
+    plans = [ops.VocabLossPlan(T, V, D, dtype=F16) for _ in range(2)]
+    up = rand((T,), F32, gen(3))
+
+    def run(k, stream=None):
+        h, w, t, _ = sets[k]
+        loss, lse = plans[k].forward(h, w, t, stream=stream)
+        return [loss, lse, *plans[k].backward(h, w, t, lse, up, stream=stream)]
+
+    want = [run(k) for k in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[run(k, streams[k]) for k in range(2)] for _ in range(8)]
+    torch.cuda.synchronize()
+    for both in got:
+        for k in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(both[k], want[k]))
