@@ -1115,14 +1115,15 @@ uint64_t piece_bytes_most(uint64_t tokens, uint64_t vocab) {
 // Parts of grad_hidden's inner dimension (the vocabulary piece) where its tiles do not fill the CUs, of no less than 512
 // rows each; the parts' sums are written and read again.
 //   - where grad_weight's product goes beside it (launch_both): tiles for one a CU, and parts no shorter than that product's
-//     inner dimension, the tokens (2048 x 4096 x 2048: 138 us backward, 154 with two a CU; 1500 x 3000 x 512: 56, 60)
-//   - else up to 256 tokens, where it is bound by reading the weight: for half the CUs (100 x 32000 x 1024: 73 us, 83 with
-//     two a CU; 128 x 131072 x 1024: 267, 259)
-//   - else for two a CU (1024 x 32000 x 1024: 239 us, 260 with one)
+//     inner dimension, the tokens (2048 x 4096 x 2048: 137 us backward, 153 with two a CU; 1500 x 3000 x 512: 50 both ways)
+//   - else up to one row of tiles, where it is bound by reading the weight: for half the CUs (100 x 32000 x 1024: 70 us, 81
+//     with two a CU; 64 x 49152 x 1024: 76, 101; 128 x 131072 x 1024: 266, 264)
+//   - else for two a CU (256 x 32000 x 2048: 155 us, 165 with half; 200 x 65536 x 1024: 161, 165; 1024 x 32000 x 1024: 240,
+//     263 with one a CU)
 uint32_t hidden_splits(uint64_t tokens, uint64_t dim, uint32_t piece) {
   if (tile_of(dim, tokens, 1) == kTileBig) return 1;
   const bool both = tile_of(dim, piece, 1) != kTileBig;
-  const uint64_t tiles = ceil_div(dim, kSmall) * ceil_div(tokens, kSmall), most = both ? 256 : tokens <= 256 ? 128 : 512;
+  const uint64_t tiles = ceil_div(dim, kSmall) * ceil_div(tokens, kSmall), most = both ? 256 : tokens <= kSmall ? 128 : 512;
   return static_cast<uint32_t>(std::max<uint64_t>(
       1, std::min<uint64_t>(most / std::min(tiles, most), piece / std::max<uint64_t>(512, both ? tokens : 0))));
 }
