@@ -12,12 +12,12 @@
 // hidden states.
 //
 // 8192 tokens of 2048 against 32768 bf16 rows: 870 us forward (1.26 PFLOP/s; a library product of these sizes that stores
-// its result takes 890), then 483 for each half of the vocabulary's G, 437 for its part of grad_weight and 430 for that of
+// its result takes 890), then 480 for each half of the vocabulary's G, 427 for its part of grad_weight and as much for that of
 // grad_hidden (the library, on these layouts, 470 to 510 and 440 to 460): 3.4 ms in all, 1.3 PFLOP/s.  2048 tokens of 4096
 // against 131072 rows forward: 1.57 ms, 1.40 PFLOP/s, as the library's product.  What bounds them is the power: the clock
 // falls to 1.6 to 1.9 GHz of 2.4, with the matrix units busy 66 to 74 % of it.  The passes over few tiles (333 tokens of
-// 520 against 5003 rows: 14 us forward, 34 back) are bound by their two and three launches, each too short to fill the
-// CUs' pipelines.
+// 520 against 5003 rows: 14 us forward, 33 to 35 back) are bound by their two and three (in fp16 four) launches, each too
+// short to fill the CUs' pipelines.
 //
 // Roundings to 16 bits, besides the outputs':
 //   - G, times 2^12 so that fp16 keeps the small probabilities normal (2^-26 and up).  The targets' entries, exp(..) - 1,
@@ -286,8 +286,8 @@ __device__ __forceinline__ void put_tile(T* stage, Q&& quad, R&& row) {
 }
 
 // Eight elements of which the first n exist, in rows `stride` apart; they are not read here again.  Whole pieces go out
-// non-temporally (2048 x 32000 x 1024: 411 us backward, 419 else); where rows end inside one, by the L2, which joins the
-// two rows that share a line (1 x 49855 x 667: 93 us, 101 else).
+// non-temporally (128 x 131072 x 1024: 266 us backward, 295 else; 2048 x 32000 x 1024: 427, 430); where rows end inside
+// one, by the L2, which joins the two rows that share a line (1 x 49855 x 667: 90 us, 101 non-temporally).
 template <class T>
 __device__ __forceinline__ void stream8(T* p, uint32_t n, uint64_t stride, const vec_t<T, 8>& v) {
   if (n >= 8 && stride % 8 == 0) {
@@ -707,13 +707,14 @@ __device__ __forceinline__ float largest(const GemmArgs<T>& a, float* lds) {
 
 // What of the hidden states' copy has to fit fp16, by a workgroup: the largest |grad_loss| of some tokens with a target, and
 // the least e with |grad_loss[n] hidden[n, c]| < 2^e for all of them (from the factors' exponents: the product may pass
-// fp32's range).
+// fp32's range).  A launch of its own, 3 us at 333 x 520, 12 at 8192 x 2048 (27 by 256 workgroups), where fp16 takes a
+// factor for each token.  One factor for all needs none: every share is 1.
 struct Reach {
   float most;
   int e;
 };
 constexpr int kNoReach = -1000;
-constexpr uint32_t kReachBlocks = 256;
+constexpr uint32_t kReachBlocks = 1024;
 
 template <class T>
 __global__ __launch_bounds__(256) void k_reach(GemmArgs<T> a, const T* hidden, uint64_t stride, uint32_t lpr_log, Reach* out) {
@@ -757,6 +758,7 @@ __device__ __forceinline__ float2 reach_of(const Reach* parts, uint32_t n) {
     r.most = r.most != r.most || most <= r.most ? r.most : most;
     r.e = max(r.e, e);
   };
+#pragma unroll 4
   for (uint32_t i = threadIdx.x & 63; i < n; i += 64) more(parts[i].most, parts[i].e);
 #pragma unroll
   for (int d = 32; d; d >>= 1) more(__shfl_xor(r.most, d), __shfl_xor(r.e, d));

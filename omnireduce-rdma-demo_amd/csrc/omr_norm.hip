@@ -11,8 +11,8 @@
 // a row of 1000 times 10000.1 gave -0.3 for each, where it gives 0).  Workgroups walk
 // several rows, so the parameters are loaded once, the next row is loaded while one is worked on, and the backward keeps
 // its part of dw and db in registers until its last row: one partial row a workgroup, which a second launch adds up in a
-// fixed order.  16384 rows of 4096 bf16 forward: 50 us, 5.4 TB/s (62 without the row ahead; a large copy reaches 5.1);
-// 16384 of 2048 backward: 42 us, 4.8 TB/s, 3 of it the second launch; 65536 of 1024: 75 us, 5.4 TB/s.
+// fixed order.  16384 rows of 4096 bf16 forward: 49 us, 5.5 TB/s (62 without the row ahead; a large copy reaches 5.1);
+// 16384 of 2048 backward: 42 us, 4.8 TB/s, 4.6 of it the second launch; 65536 of 1024: 75 us, 5.4 TB/s.
 // Rows of more than 16384 columns take the *_any kernels, which read a row again instead of holding it.
 #include "omr_elem.h"
 
