@@ -497,8 +497,9 @@ int omr_layer_norm_grad(const void* grad_out, uint64_t grad_stride, const void* 
 
 /* Softmax cross entropy over a large vocabulary, without keeping the logits z = hidden weight^T:
  *   lse[n] = log(sum over v of exp(z[n, v])),  loss[n] = lse[n] - z[n, targets[n]]     (fp32, both required)
- * hidden [tokens, dim] and weight [vocab, dim]: bf16 or fp16 (`dtype`), dim <= 2^20, tokens < 2^26, vocab < 2^31 - 256.  targets: int32, or int64 with
- * targets64 != 0; a target outside [0, vocab) is none: its loss is 0 (its lse is still that of its row).
+ * hidden [tokens, dim] and weight [vocab, dim]: bf16 or fp16 (`dtype`), dim <= 2^20, tokens < 2^26, vocab < 2^31 - 256, and
+ * no more of them together than a launch has tiles for (refused else).  targets: int32, or int64 with targets64 != 0; a
+ * target outside [0, vocab) is none: its loss is 0 (its lse is still that of its row).
  * Rows of hidden and weight that are whole 16-byte pieces (dim, strides and addresses; strides below 2^22) are read as
  * they are; others are laid out again in the workspace by each call, which then has to be asked for with pack != 0 (a
  * dim that is no multiple of 8 implies it). */

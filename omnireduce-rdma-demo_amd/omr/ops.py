@@ -285,10 +285,11 @@ def block_sum(inputs: Sequence[torch.Tensor], block_list: torch.Tensor, num: int
 # ------------------------------------------------------------------ operators that make the gradient
 
 # The two ends of a language model: their parameter gradients are the fp32 tensors the all-reduce sums.  Every output may
-# be given (a view of the flat gradient, say); what is not given is allocated on the call's stream.  Work runs on
-# `stream`, or on the current stream of the tensors' device.  A plan's workspace serves one call at a time: calls that
-# may overlap (two streams, two captured graphs replayed side by side) need a plan each, and a captured graph needs its
-# plan and its tensors for as long as it is replayed.
+# be given (a view of the flat gradient, say); what is not given is allocated on the call's stream.  Nothing here records
+# autograd nodes: inputs that require a gradient give outputs that do not, and the backward passes are calls of their own.
+# Work runs on `stream`, or on the current stream of the tensors' device.  A plan's workspace serves one call at a time:
+# calls that may overlap (two streams, two captured graphs replayed side by side) need a plan each, and a captured graph
+# needs its plan and its tensors for as long as it is replayed.
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # (torch.cuda.current_stream(i).cuda_stream and torch.cuda.current_device(), without the objects they make)
@@ -550,7 +551,8 @@ class LayerNormGradPlan:
 
 class VocabLossPlan:
     """Softmax cross entropy of hidden [tokens, dim] against the output layer's weight [vocab, dim] (bf16 or fp16),
-    forward and backward, without keeping the logits, for at most max_tokens tokens a call.
+    forward and backward, without keeping the logits, for at most max_tokens tokens a call.  The backward pass holds the
+    logits' gradients in `dtype`, whatever grad_weight's type is.
 
     pack: room to lay rows out again that are not whole 16-byte pieces (implied by a dim that is no multiple of 8).
     grads=False: forward only."""
@@ -591,8 +593,9 @@ class VocabLossPlan:
                  grad_loss: torch.Tensor, grad_hidden: Optional[torch.Tensor] = None,
                  grad_weight: Optional[torch.Tensor] = None, accumulate: bool = False, need_hidden: bool = True,
                  need_weight: bool = True, stream=None):
-        """(grad_hidden, grad_weight) for grad_loss (fp32, one a token, or one for all).  grad_weight is fp32 or of the
-        weight's type (default), written or added to (accumulate); need_hidden / need_weight=False leave one out."""
+        """(grad_hidden, grad_weight) for grad_loss (fp32, one a token, or one for all, which in fp16 saves a pass over
+        hidden).  grad_weight is fp32 or of the weight's type (default), written or added to (accumulate); need_hidden /
+        need_weight=False leave one out."""
         if not self.grads:
             raise ValueError("the plan was made with grads=False")
         call = _Call(hidden, stream)
