@@ -1151,8 +1151,8 @@ Space layout(uint64_t tokens, uint64_t vocab, uint64_t dim, bool pack, bool grad
   s.h = s.w + (pack ? up(vocab * pdim * 2, 256) : 0);
   s.rest = s.h + (pack ? up(tokens * pdim * 2, 256) : 0);
   uint64_t fwd = up(tokens * 4, 256) + stats_bytes_most(tokens, vocab);
-  uint64_t bwd = 256 + kReachBlocks * sizeof(Reach) + 2 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) + up(tokens * pdim * 2, 256) +
-                 up(piece_bytes_most(tokens, vocab), 256) + acc_bytes_most(tokens, dim);
+  uint64_t bwd = 256 + kReachBlocks * sizeof(Reach) + 2 * up(tokens * 4, 256) + up(4 * vocab + 4, 256) +
+                 up(tokens * pdim * 2, 256) + up(piece_bytes_most(tokens, vocab), 256) + acc_bytes_most(tokens, dim);
   s.bytes = s.rest + (grads ? std::max(fwd, bwd) : fwd) + 256;
   return s;
 }
